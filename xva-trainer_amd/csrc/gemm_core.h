@@ -45,10 +45,12 @@ __device__ __forceinline__ float bf2f(uint16_t h) { return __uint_as_float(((uin
 __device__ __forceinline__ uint32_t pack_bf2(float a, float b);
 __device__ __forceinline__ uint16_t f2bf(float f) { return (uint16_t)(pack_bf2(f, 0.f) & 0xffffu); }
 __device__ __forceinline__ float lrelu(float v, float s) { return v > 0.f ? v : v * s; }
-__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {   // round-to-nearest-even pair -> packed bf16x2
-    uint32_t r;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+// round-to-nearest-even pair -> packed bf16x2: one v_cvt_pk_bf16_f32.  By the compiler's conversion, not inline asm: a matrix instruction that reads the result
+// right behind it, or whose result it reads, needs wait states that the compiler only inserts around instructions it knows.
+__device__ __forceinline__ uint32_t pack_bf2(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 
 __device__ __forceinline__ float ld_elem(const void* p, int64_t idx, int dtype) {
