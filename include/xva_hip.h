@@ -713,6 +713,94 @@ int xva_sdp_dequant_fwd(const float* z_u, const float* dr, float* z0_log, float*
 int xva_sdp_dequant_bwd(const float* z_u, const float* dr, const float* d_z0_log, const float* d_logsig, float* d_z_u, const int32_t* lens, int B, int T,
                         void* stream);
 
+/* ----------------------------------------------------------------- sequence operators ---- */
+/* Blocks of a sequence model on time-major tensors, beside the reference's own (no call site of the reference: attention with positions inside it, group
+ * normalisation and recurrences are what a changed acoustic model asks for next).  dtype: 0 fp32, 1 bf16, 2 fp16; strides in elements, the last dimension
+ * contiguous; rows at or behind an item's length are not read and leave as zeros.  Every call only enqueues; buffers of one call in flight (workspace
+ * included) are not shared with another on a different stream, nor with another captured graph that may run beside it. */
+
+/* Rotary positions.  q (B, T, H, D), k (B, T, Hk, D) (null with Hk = 0); pair i of the first rd elements of a head turns by position * turns[i]:
+ * (a, b) -> gain (a cos - b sin, b cos + a sin), with (a, b) = elements (i, i + rd / 2), or (2 i, 2 i + 1) when `interleaved`; the other D - rd elements are
+ * copied.  turns: rd / 2 fractions of a turn per position as 64-bit fixed point, so angles are exact at any 64-bit position.  positions: int32 or int64
+ * (positions64) with strides over items and rows (0: the same for all), null: the row's index.  inverse: the angle negated — the gradient.
+ * In place: q_out == q and k_out == k with equal strides. */
+typedef struct {
+    const void *q, *k;
+    void *q_out, *k_out;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];   /* items, rows, heads */
+    const uint64_t* turns;
+    const void* positions;
+    int64_t pos_stride[2];
+    int32_t positions64, dtype, B, T, H, Hk, D, rd, interleaved, inverse;
+    float gain;
+} xva_rotary_args;
+int xva_rotary(const xva_rotary_args* p, void* stream);
+
+/* Group normalisation + activation, channels last.  x (B, T, C) in G groups of channels; statistics over an item's live rows and a group's channels;
+ * y = act(weight * xh + bias) (weight / bias fp32 (C), null: 1 / 0).  act: 0 none, 1 relu, 2 leaky relu (slope), 3 tanh, 4 silu, 5 gelu (erf).
+ * mean / rstd (B, G) are written by the forward and read by the backward.  Backward: x, dy -> out = dx, and dweight / dbias (overwritten; null: not wanted).
+ * At most 2048 groups, and 1024 vectors of 16 bytes in a row (1024 channels, where C, a stride or an address rules 16-byte accesses out), unless one
+ * group of an item fits a wave (T * C / G of at most 256 vectors). */
+typedef struct {
+    const void *x, *dy;
+    void* out;
+    int64_t x_stride[2], dy_stride[2], out_stride[2];                     /* items, rows */
+    const float *weight, *bias;
+    float *mean, *rstd, *dweight, *dbias;
+    const int32_t* lens;
+    int32_t dtype, B, T, C, G, act;
+    float eps, slope;
+} xva_group_norm_args;
+int64_t xva_group_norm_workspace_bytes(const xva_group_norm_args* p, int backward_pass);
+int xva_group_norm_act_fwd(const xva_group_norm_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+int xva_group_norm_act_bwd(const xva_group_norm_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Gated linear recurrence.  x, gate (B, T, C): f = sigmoid(gate), h_t = f_t h_{t-1} + (1 - f_t) x_t, or + x_t with unit_gain; `reverse`: from an item's last
+ * live row to its first.  h0 (B, C) fp32 (null: zeros); last (B, C) fp32 is the state behind the last step.  states: xva_recurrence_state_floats fp32, the
+ * state at the entry of each run of steps, written by the forward (null: no backward will come) and read by the backward.
+ * Backward: dh (B, T, C), dlast (B, C) fp32 (null: zeros) -> dx, dgate, dh0 (null: not wanted). */
+typedef struct {
+    const void *x, *gate;
+    void* h;
+    const float* h0;
+    float *last, *states;
+    const void* dh;
+    const float* dlast;
+    void *dx, *dgate;
+    float* dh0;
+    const int32_t* lens;
+    int64_t x_stride[2], gate_stride[2], h_stride[2], dh_stride[2], dx_stride[2], dgate_stride[2];   /* items, rows */
+    int32_t dtype, B, T, C, reverse, unit_gain;
+} xva_recurrence_args;
+int64_t xva_recurrence_workspace_bytes(int B, int T, int C);
+int64_t xva_recurrence_state_floats(int B, int T, int C);
+int xva_recurrence_fwd(const xva_recurrence_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+int xva_recurrence_bwd(const xva_recurrence_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Differential attention (bf16 / fp16).  q (B, Tq, H, 2, d), k (B, Tk, Hk, 2, d), v (B, Tk, Hk, 2 d), lam (H) fp32; d a multiple of 8 up to 64, H a multiple
+ * of Hk (query head h reads key head h / (H / Hk)); addresses 16-byte aligned, strides multiples of 8.  out (B, Tq, H, 2 d) =
+ * (softmax(scale q_1 k_1^T) - lam softmax(scale q_2 k_2^T)) v.  q_lens / k_lens (B): live queries and keys (null: all); causal: query i sees keys
+ * j <= i + k_len - q_len.  Rows that see nothing, and rows behind q_len, leave as zeros.
+ * For a backward pass the forward also writes maps (2, B, Tq, H, 2 d), each softmax's own output, and lse (2, B, H, Tq) fp32 (both null: no backward).
+ * Backward: dout -> dq, dk, dv (contiguous, the inputs' shapes) and dlam (H) fp32, all overwritten (B = 0 or Tq = 0: nothing is). */
+typedef struct {
+    const void *q, *k, *v;
+    const float* lam;
+    void *out, *maps;
+    float* lse;
+    const void* dout;
+    void *dq, *dk, *dv;
+    float* dlam;
+    const int32_t *q_lens, *k_lens;
+    int64_t q_stride[4], k_stride[4];                                      /* items, rows, heads, maps */
+    int64_t v_stride[3], out_stride[3], dout_stride[3];                    /* items, rows, heads */
+    int32_t dtype, B, Tq, Tk, H, Hk, d, causal;
+    float scale;
+} xva_diff_attention_args;
+int64_t xva_diff_attention_workspace_bytes(const xva_diff_attention_args* p, int backward_pass);
+int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

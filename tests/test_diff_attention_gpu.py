@@ -1,0 +1,251 @@
+"""Differential attention (csrc/diff_attention.hip) against the formulas in 64 bits.
+
+Roundings, u half a step of the 16-bit type (2^-8 bf16, 2^-11 fp16): each softmax weight is rounded once before it meets V, so an output is off by u (P_1 + |lam| P_2) |V|;
+the maps' own outputs, from which D comes, by that and one more rounding; each dS = P o (dP - D) by u of itself and P times D's error; P_1 - lam P_2 by u of itself;
+every result by u of itself.  fp32 work (scores, exponentials, sums): E of the magnitudes that meet."""
+import math
+
+import pytest
+import torch
+
+from seq_util import DTYPES, HALF, TINY, close, lengths
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -15      # scores of size |q| |k| sqrt(d) ~ 20 carry 20 x 2^-22 absolute into the exponent, with the roundings of the exponential and of the sums
+
+
+def _reference(q, k, v, lam, dout, ql, kl, causal, scale):
+    q, k, v, lam, dout = (t.detach().double().cpu() for t in (q, k, v, lam, dout))
+    u, tiny = HALF[_reference.dtype], TINY[_reference.dtype]
+    B, Tq, H, _, d = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    out, dq, dk, dv, dl = torch.zeros_like(dout), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(lam)
+    eo, eq, ek, ev, el = (torch.zeros_like(t) for t in (out, dq, dk, dv, dl))
+    for b in range(B):
+        nq, nk = (Tq if ql is None else int(ql[b])), (Tk if kl is None else int(kl[b]))
+        if nq == 0 or nk == 0:
+            continue
+        see = torch.ones(nq, nk, dtype=torch.bool)
+        if causal:
+            see = torch.arange(nk)[None] <= torch.arange(nq)[:, None] + nk - nq
+        for h in range(H):
+            hk = h // (H // Hk)
+            V, g = v[b, :nk, hk], dout[b, :nq, h]
+            P = []
+            for m in range(2):
+                s = (q[b, :nq, h, m] @ k[b, :nk, hk, m].T * scale).masked_fill(~see, -math.inf)
+                P.append(torch.nan_to_num(torch.softmax(s, -1), nan=0.0))
+            l, la = lam[h], lam[h].abs()
+            both, size = P[0] - l * P[1], P[0] + la * P[1]
+            out[b, :nq, h] = both @ V
+            eo[b, :nq, h] = (u + E) * (size @ V.abs()) + tiny * (1 + la) * (see.double() @ V.abs())
+            dP = g @ V.T
+            dl[h] -= (P[1] * dP).sum()
+            el[h] += E * (P[1] * (g.abs() @ V.abs().T)).sum()
+            dv[b, :nk, hk] += both.T @ g
+            ev[b, :nk, hk] += (u * both.abs() + E * size + tiny).T @ g.abs()
+            for m, c in ((0, torch.ones(())), (1, -l)):
+                D = (P[m] * dP).sum(-1, keepdim=True)
+                gv = g.abs() @ V.abs().T
+                eD = ((2 * u + E) * (P[m] * gv).sum(-1, keepdim=True)) + 2 * tiny * g.abs().sum(-1, keepdim=True) * (1 + V.abs().max() * see.sum(-1, keepdim=True))
+                dS = c * P[m] * (dP - D)
+                eS = c.abs() * P[m] * (eD + E * (gv + D.abs() + gv.mul(P[m]).sum(-1, keepdim=True))) + u * dS.abs() + tiny * (see.double())
+                dq[b, :nq, h, m] = scale * dS @ k[b, :nk, hk, m]
+                eq[b, :nq, h, m] = scale * eS @ k[b, :nk, hk, m].abs()
+                dk[b, :nk, hk, m] += scale * dS.T @ q[b, :nq, h, m]
+                ek[b, :nk, hk, m] += scale * eS.T @ q[b, :nq, h, m].abs()
+    refs, errs = (out, dq, dk, dv), (eo, eq, ek, ev)
+    return refs + (dl,), tuple(u * (r.abs() + e) + tiny + 1.01 * e for r, e in zip(refs, errs)) + (el + E * dl.abs(),)
+
+
+def _data(B, Tq, Tk, H, Hk, d, dt, seed=0, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed * 1000 + B * 77 + Tq * 13 + Tk * 7 + d)
+    n = lambda *s: (torch.randn(*s, device="cuda", generator=g) * size).to(DTYPES[dt])
+    return n(B, Tq, H, 2, d), n(B, Tk, Hk, 2, d), n(B, Tk, Hk, 2 * d), 0.5 + 0.2 * torch.randn(H, device="cuda", generator=g), n(B, Tq, H, 2 * d)
+
+
+def _run(q, k, v, lam, dout, ql=None, kl=None, causal=False, scale=None):
+    from xva_trainer_amd import seq_ops as S
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    cuda = lambda t: t.cuda() if t is not None else None
+    out = S.differential_attention(*leaves, causal=causal, scale=scale, q_lens=cuda(ql), k_lens=cuda(kl))
+    got = (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+    _reference.dtype = q.dtype
+    ref, err = _reference(q, k, v, lam, dout, ql, kl, causal, scale or q.shape[-1] ** -0.5)
+    for name, o, r, e in zip(("out", "dq", "dk", "dv", "dlam"), got, ref, err):
+        close(o, r, e, name)
+    with torch.no_grad():                        # the call without a gradient may take another path: the same bounds
+        alone = S.differential_attention(q, k, v, lam, causal=causal, scale=scale, q_lens=cuda(ql), k_lens=cuda(kl))
+    close(alone, ref[0], err[0], "out, no gradient")
+    return got
+
+
+SHAPES = [(1, 1, 1, 1, 1, 8), (2, 5, 5, 2, 1, 16), (1, 64, 64, 1, 1, 32), (2, 65, 65, 2, 2, 64), (1, 130, 130, 4, 2, 48), (2, 150, 150, 2, 2, 32), (1, 33, 200, 3, 1, 24),
+          (1, 200, 33, 2, 1, 40), (3, 17, 129, 4, 1, 56), (1, 300, 300, 1, 1, 64), (2, 1, 700, 4, 2, 64), (1, 3, 513, 8, 1, 16), (4, 1, 9, 2, 2, 32)]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ragged", [None, "some", "empty"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,d", SHAPES)
+def test_shapes(dt, causal, ragged, B, Tq, Tk, H, Hk, d):
+    kl = lengths(B, Tk, ragged)
+    ql = lengths(B, Tq, ragged) if Tq == Tk or ragged == "empty" else None
+    got = _run(*_data(B, Tq, Tk, H, Hk, d, dt), ql=ql, kl=kl, causal=causal)
+    if ql is not None:
+        dead = torch.arange(Tq)[None] >= ql[:, None]
+        assert (got[0].cpu()[dead] == 0).all() and (got[1].cpu()[dead] == 0).all()
+    if kl is not None:
+        dead = torch.arange(Tk)[None] >= kl[:, None]
+        assert (got[2].cpu()[dead] == 0).all() and (got[3].cpu()[dead] == 0).all()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Tq,Tk", [(1, 5000), (4, 3001), (700, 700)])
+def test_long_rows(causal, Tq, Tk):
+    _run(*_data(2, Tq, Tk, 4, 2, 64, "bf16", seed=1), causal=causal, kl=torch.tensor([Tk, Tk // 3], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("size,scale", [(4.0, None), (1.0, 2.0), (0.05, None)])
+def test_sharp_and_flat_rows(size, scale):
+    """Scores of hundreds (one key takes all), and of nothing (all keys alike)."""
+    global E
+    keep, E = E, E * max(1.0, size * size * (scale or 64 ** -0.5) * 8)      # scores grow by that much over the standard ones, and their fp32 error with them
+    try:
+        _run(*_data(1, 150, 150, 2, 1, 64, "bf16", seed=2, size=size), scale=scale, causal=True)
+    finally:
+        E = keep
+
+
+def test_a_lone_key_gives_its_value_and_no_score_gradient():
+    q, k, v, lam, dout = _data(3, 1, 1, 2, 2, 32, "bf16", seed=3)
+    got = _run(q, k, v, lam, dout)
+    ref = (v.double() * (1 - lam.double())[None, None, :, None])
+    assert (got[0].double() - ref).abs().max() <= 2.0 ** -8 * ref.abs().max()
+    # exact zeros but for the fp32 difference of two sums of the same 64 products, times keys of size 4
+    assert max(got[1].abs().max().item(), got[2].abs().max().item()) < 64 * 16 * 2.0 ** -22 * 4
+
+
+@pytest.mark.parametrize("Tq,Tk", [(70, 70), (1, 200), (90, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_what_lies_behind_an_item_is_not_read(Tq, Tk, causal):
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(4, Tq, Tk, 2, 1, 48, "bf16", seed=4)
+    kl = torch.tensor([Tk, Tk // 2, 0, 1], dtype=torch.int32)
+    ql = torch.tensor([Tq, max(1, Tq // 2), Tq, 0], dtype=torch.int32)
+    dq_, dk_ = (torch.arange(Tq)[None] >= ql[:, None]).cuda(), (torch.arange(Tk)[None] >= kl[:, None]).cuda()
+    outs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        leaves = [q.masked_fill(dq_[..., None, None, None], fill), k.masked_fill(dk_[..., None, None, None], fill), v.masked_fill(dk_[..., None, None], fill), lam.clone()]
+        leaves = [t.requires_grad_(True) for t in leaves]
+        out = S.differential_attention(*leaves, causal=causal, q_lens=ql.cuda(), k_lens=kl.cuda())
+        with torch.no_grad():
+            alone = S.differential_attention(*leaves, causal=causal, q_lens=ql.cuda(), k_lens=kl.cuda())
+        outs.append((out.detach(), alone) + torch.autograd.grad(out, leaves, dout.masked_fill(dq_[..., None, None], fill)))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+def test_views_of_a_projection_and_of_a_cache():
+    """q, k, v as slices of one projection; keys as the head of a longer cache; addresses and strides that the kernel needs copied."""
+    H, Hk, d = 4, 2, 32
+    whole = torch.randn(2, 90, H * 2 * d + Hk * 4 * d + 3, device="cuda").bfloat16()
+    lam, dout = torch.rand(H, device="cuda"), torch.randn(2, 90, H, 2 * d, device="cuda").bfloat16()
+    for at in (0, 1, 3):
+        w = whole[..., at:at + H * 2 * d + Hk * 4 * d]
+        q, k, v = w.split((H * 2 * d, Hk * 2 * d, Hk * 2 * d), -1)
+        _run(q.unflatten(-1, (H, 2, d)), k.unflatten(-1, (Hk, 2, d)), v.unflatten(-1, (Hk, 2 * d)), lam, dout)
+    cache = torch.randn(2, Hk, 300, 2, d, device="cuda").bfloat16().transpose(1, 2)
+    vals = torch.randn(2, Hk, 300, 2 * d, device="cuda").bfloat16().transpose(1, 2)
+    q = torch.randn(2, 1, H, 2, d, device="cuda").bfloat16()
+    _run(q, cache[:, :200], vals[:, :200], lam, dout[:, :1], kl=torch.tensor([200, 31], dtype=torch.int32), causal=True)
+    _run(q.expand(2, 70, H, 2, d), cache, vals, lam.bfloat16().float(), dout[:, :70].transpose(2, 3).contiguous().transpose(2, 3))
+
+
+def test_lam_of_other_types_and_signs():
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, _, dout = _data(2, 40, 40, 4, 4, 16, "fp16", seed=5)
+    for lam in (torch.zeros(4, device="cuda"), torch.tensor([-1.0, 2.0, 0.0, 1.0], device="cuda")):
+        _run(q, k, v, lam, dout)
+    lam = torch.tensor([0.1, 0.9, 0.3, 0.5], device="cuda").half().requires_grad_(True)
+    out = S.differential_attention(q, k, v, lam)
+    g, = torch.autograd.grad(out, lam, dout)
+    assert g.dtype == torch.float16
+    lam32 = lam.detach().float().requires_grad_(True)
+    g32, = torch.autograd.grad(S.differential_attention(q, k, v, lam32), lam32, dout)
+    assert torch.equal(g, g32.half())
+
+
+def test_the_gradient_by_differences():
+    """Against differences of the loss itself; outputs carry u of the weights' sums, so the step is large and the bound follows it."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(1, 48, 48, 2, 1, 32, "fp16", seed=6)
+    lam.requires_grad_(True)
+    vv = v.clone().requires_grad_(True)
+    out = S.differential_attention(q, k, vv, lam, causal=True)
+    gv, gl = torch.autograd.grad(out, (vv, lam), dout)
+    step = torch.randn_like(lam)
+    with torch.no_grad():                                            # linear in lam and in v
+        f = lambda l, x: (S.differential_attention(q, k, x, l, causal=True).double() * dout.double()).sum()
+        by_lam = (f(lam + step, v) - f(lam - step, v)) / 2
+        by_v = (f(lam, v + v) - f(lam, v - v)) / 2
+    noise = 2.0 ** -10 * (1 + lam.abs().max().item() + step.abs().max().item()) * dout.double().abs().sum().item() * v.abs().max().item()
+    n = dout.numel() ** 0.5 / dout.numel()                           # of independent roundings, ten deviations
+    assert abs(by_lam.item() - (gl * step).sum().item()) < 10 * n * noise
+    assert abs(by_v.item() - (gv.double() * v.double()).sum().item()) < 10 * n * noise
+
+
+def test_repeats_graph_and_streams():
+    from xva_trainer_amd import seq_ops as S
+    for Tq, Tk in ((200, 200), (1, 900)):
+        q, k, v, lam, dout = _data(2, Tq, Tk, 4, 2, 64, "bf16", seed=7)
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        kl = torch.tensor([Tk, Tk // 2], device="cuda", dtype=torch.int32)
+        def step():
+            out = S.differential_attention(*leaves, k_lens=kl)
+            with torch.no_grad():
+                alone = S.differential_attention(*leaves, k_lens=kl)
+            return (out.detach(), alone) + torch.autograd.grad(out, leaves, dout)
+        assert all(torch.equal(a, b) for a, b in zip(step(), step()))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for turn in range(4):
+            with torch.no_grad():
+                q.normal_(), k.normal_(), dout.normal_(), kl.random_(1, Tk + 1)
+            graph.replay()
+            eager = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, eager)), turn
+
+
+def test_empty():
+    from xva_trainer_amd import seq_ops as S
+    for B, Tq, Tk in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k, v, lam, dout = _data(B, Tq, Tk, 2, 1, 16, "bf16")
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        out = S.differential_attention(*leaves)
+        assert out.shape == (B, Tq, 2, 32) and (out == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(out, leaves, dout))
+
+
+def test_refusals():
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, _ = _data(2, 3, 4, 4, 2, 16, "bf16")
+    for bad in (lambda: S.differential_attention(q.float(), k.float(), v.float(), lam), lambda: S.differential_attention(q, k.half(), v, lam),
+                lambda: S.differential_attention(q, k, v[:, :3], lam), lambda: S.differential_attention(q[:, :, :3], k, v, lam[:3]),
+                lambda: S.differential_attention(q, k, v, lam[:3]), lambda: S.differential_attention(q[..., :12], k[..., :12], v[..., :24], lam),
+                lambda: S.differential_attention(q, k, v, lam.long()), lambda: S.differential_attention(q, k, v, lam, scale=0.0),
+                lambda: S.differential_attention(q, k, v, lam, scale=float("nan")), lambda: S.differential_attention(q, k, v, lam, k_lens=torch.tensor([1, 2])),
+                lambda: S.differential_attention(q, k, v, lam, q_lens=torch.tensor([1, 2, 3], device="cuda")), lambda: S.differential_attention(q.cpu(), k, v, lam),
+                lambda: S.differential_attention(q[:, :, :, 0], k, v, lam), lambda: S.differential_attention(torch.zeros(1, 2, 1, 2, 72, device="cuda").half(),
+                                                                                                          torch.zeros(1, 2, 1, 2, 72, device="cuda").half(),
+                                                                                                          torch.zeros(1, 2, 1, 144, device="cuda").half(), lam[:1])):
+        with pytest.raises(S.XvaError):
+            bad()

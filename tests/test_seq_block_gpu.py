@@ -1,0 +1,94 @@
+"""The sequence operators one after the other, as a block of an acoustic model uses them: group norm + silu -> q / k / v -> rotary positions -> differential attention ->
+each head's norm -> gate and input -> gated recurrence; ragged, with the gradient of every input and weight, against the same block in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from seq_util import lengths
+
+pytestmark = pytest.mark.gpu
+
+
+def _block(S, x, p, lens, H, Hk, d, plan, wide):
+    """`wide` computes the products; S the operators (the package's, or `Plain` below)."""
+    B, T, C = x.shape
+    h = S.group_norm_act(x, 8, p["w1"], p["b1"], lens=lens, act="silu")
+    q, k, v = wide(h, p["qkv"]).split((H * 2 * d, Hk * 2 * d, Hk * 2 * d), -1)
+    q, k = S.rotary(plan, q.unflatten(-1, (2 * H, d)), k.unflatten(-1, (2 * Hk, d)))
+    o = S.differential_attention(q.unflatten(2, (H, 2)), k.unflatten(2, (Hk, 2)), v.unflatten(-1, (Hk, 2 * d)), p["lam"], causal=True, q_lens=lens, k_lens=lens)
+    o = S.group_norm_act(o.reshape(B * T, H * 2 * d), H, p["w2"], None)
+    u, gate = wide(o.view(B, T, -1), p["ug"]).chunk(2, -1)
+    y, last = S.gated_recurrence(u, gate + 1, p["h0"], lens=lens)
+    return y, last
+
+
+class Plain:
+    @staticmethod
+    def group_norm_act(x, G, w, b, lens=None, act="none"):
+        flat = x.dim() == 2
+        x = x[:, None] if flat else x
+        B, T, C = x.shape
+        live = torch.ones(B, T, 1, 1, dtype=x.dtype) if lens is None else (torch.arange(T)[None] < lens[:, None])[..., None, None].to(x.dtype)
+        g = x.view(B, T, G, -1)
+        n = live.sum((1, 3), keepdim=True).clamp_min(1) * (C // G)
+        mu = (g * live).sum((1, 3), keepdim=True) / n
+        var = ((g - mu).square() * live).sum((1, 3), keepdim=True) / n
+        z = ((g - mu) * (var + 1e-5).rsqrt()).reshape(B, T, C) * w + (b if b is not None else 0)
+        y = (z * torch.sigmoid(z) if act == "silu" else z) * live[..., 0]
+        return y[:, 0] if flat else y
+
+    @staticmethod
+    def rotary(plan, q, k):
+        def turn(x):
+            ang = torch.arange(x.shape[1], dtype=x.dtype)[:, None, None] * torch.tensor(plan.frequencies, dtype=x.dtype)
+            n = len(plan.frequencies)
+            a, b, rest = x[..., :n], x[..., n:2 * n], x[..., 2 * n:]
+            return torch.cat((a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin(), rest), -1)
+        return turn(q), turn(k)
+
+    @staticmethod
+    def differential_attention(q, k, v, lam, causal, q_lens, k_lens):
+        T, share = q.shape[1], q.shape[2] // k.shape[2]
+        see = torch.arange(T)[None] <= torch.arange(T)[:, None]
+        see = see[None] & (torch.arange(T)[None, :, None] < q_lens[:, None, None])          # (causal: keys behind the length are behind every live query)
+        k, v = k.repeat_interleave(share, 2), v.repeat_interleave(share, 2)
+        s = torch.einsum("bihmd,bjhmd->bhmij", q, k) * q.shape[-1] ** -0.5
+        p = torch.nan_to_num(torch.softmax(s.masked_fill(~see[:, None, None], -math.inf), -1), nan=0.0)
+        return torch.einsum("bhij,bjhe->bihe", p[:, :, 0] - lam[:, None, None] * p[:, :, 1], v)
+
+    @staticmethod
+    def gated_recurrence(x, gate, h, lens):
+        f, out = torch.sigmoid(gate), []
+        for t in range(x.shape[1]):
+            live = (t < lens)[:, None]
+            h = torch.where(live, f[:, t] * h + (1 - f[:, t]) * x[:, t], h)
+            out.append(h * live)
+        return torch.stack(out, 1), h
+
+
+@pytest.mark.parametrize("dt,tol", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_block_forward_and_gradient(dt, tol):
+    """Norm of the difference over the norm of the result.  Each of the ~12 tensors between input and output is rounded once, u = half a step; a tensor of
+    independent roundings is off by at most u of its norm, and they pass through maps whose gains are a few at most (a norm over 64 values, differences of
+    softmax maps with lam < 1): 40 u bounds forward and gradients."""
+    from xva_trainer_amd import seq_ops as S
+    torch.manual_seed(11)
+    B, T, C, H, Hk, d = 3, 70, 64, 4, 2, 16
+    lens = lengths(B, T, "some")
+    p = {"w1": 1 + 0.1 * torch.randn(C), "b1": 0.1 * torch.randn(C), "qkv": torch.randn(H * 2 * d + Hk * 4 * d, C) * C ** -0.5, "lam": 0.2 + 0.1 * torch.rand(H),
+         "w2": 1 + 0.1 * torch.randn(H * 2 * d), "ug": torch.randn(2 * C, H * 2 * d) * (H * 2 * d) ** -0.5, "h0": torch.randn(B, C)}
+    p = {n: (t.to(dt).float() if n in ("qkv", "ug") else t) for n, t in p.items()}
+    x, dy, dl = torch.randn(B, T, C).to(dt), torch.randn(B, T, C).to(dt), torch.randn(B, C)
+    plan = S.RotaryPlan(16)
+    mine = {n: (t.to(dt) if n in ("qkv", "ug") else t).cuda().requires_grad_(True) for n, t in p.items()}
+    xm = x.cuda().requires_grad_(True)
+    outs = _block(S, xm, mine, lens.cuda(), H, Hk, d, plan, lambda a, w: (a.float() @ w.float().T).to(dt))
+    got = [o.detach() for o in outs] + list(torch.autograd.grad(outs, [xm] + list(mine.values()), (dy.cuda(), dl.cuda())))
+    ref64 = {n: t.double().requires_grad_(True) for n, t in p.items()}
+    x64 = x.double().requires_grad_(True)
+    outs64 = _block(Plain, x64, ref64, lens.long(), H, Hk, d, plan, lambda a, w: a @ w.T)
+    ref = [o.detach() for o in outs64] + list(torch.autograd.grad(outs64, [x64] + list(ref64.values()), (dy.double(), dl.double())))
+    for name, a, b in zip(["y", "last", "dx"] + ["d" + n for n in p], got, ref):
+        rel = ((a.double().cpu() - b).norm() / b.norm()).item()
+        assert rel < 40 * tol, (name, rel)

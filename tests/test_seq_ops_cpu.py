@@ -1,0 +1,134 @@
+"""The sequence operators without a GPU: plans, the C structs' layout, refusals at the C entry points and of host tensors."""
+import ctypes as C
+import math
+import os
+import subprocess
+
+import pytest
+import torch
+
+from xva_trainer_amd import _lib, seq_ops as S
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_plan_frequencies_as_turns():
+    for kw in ({}, {"scaling": "linear", "factor": 4.0}, {"scaling": "ntk", "factor": 8.0}, {"scaling": "yarn", "factor": 16.0}):
+        plan = S.RotaryPlan(64, device="cpu", **kw)
+        for f, t in zip(plan.frequencies, plan.turns.tolist()):
+            assert abs((t % 2 ** 64) / 2.0 ** 64 - f / (2 * math.pi)) <= 2.0 ** -52
+    base = S.RotaryPlan(64, device="cpu").frequencies
+    assert base[0] == 1.0 and math.isclose(base[16], 10000.0 ** -0.5)
+    ntk = S.RotaryPlan(64, device="cpu", scaling="ntk", factor=8.0).frequencies
+    assert ntk[0] == 1.0 and math.isclose(ntk[31], base[31] / 8.0)
+    yarn = S.RotaryPlan(64, device="cpu", scaling="yarn", factor=16.0)
+    assert yarn.frequencies[0] == base[0] and math.isclose(yarn.frequencies[31], base[31] / 16.0) and math.isclose(yarn.gain, 0.1 * math.log(16.0) + 1.0)
+    assert all(a >= b for a, b in zip(yarn.frequencies, yarn.frequencies[1:]))
+
+
+@pytest.mark.parametrize("bad", [dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, base=1.0),
+                                 dict(rotary_dim=8, factor=0.5)])
+def test_plan_refusals(bad):
+    with pytest.raises(S.XvaError):
+        S.RotaryPlan(device="cpu", **bad)
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros(1, 2, 2, 8)
+    for call in (lambda: S.rotary(S.RotaryPlan(8, device="cpu"), x), lambda: S.gated_recurrence(x[0], x[0]), lambda: S.group_norm_act(x[0], 2),
+                 lambda: S.differential_attention(x[:, :, None].bfloat16(), x[:, :, None].bfloat16(), torch.zeros(1, 2, 1, 16).bfloat16(), torch.zeros(1))):
+        with pytest.raises(S.XvaError, match="device tensors"):
+            call()
+
+
+STRUCTS = {"xva_rotary_args": S._RotaryArgs, "xva_group_norm_args": S._GroupNormArgs, "xva_recurrence_args": S._RecurrenceArgs,
+           "xva_diff_attention_args": S._DiffAttentionArgs}
+
+
+def test_structs_match_the_header(tmp_path):
+    """Size and every field's offset, as a C compiler lays the header out (arrays by their elements)."""
+    lines = []
+    for name, t in STRUCTS.items():
+        lines.append('printf("%%zu\\n", sizeof(%s));' % name)
+        fields = [f for f, _ in t._fields_]
+        for f in fields:
+            base = f.rstrip("0123456789")
+            array = base in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride", "pos_stride", "x_stride", "dy_stride", "out_stride", "dout_stride",
+                             "gate_stride", "h_stride", "dh_stride", "dx_stride", "dgate_stride")
+            at = "offsetof(%s, %s)" % (name, base if array else f)
+            lines.append('printf("%%zu\\n", %s + %s * sizeof(int64_t));' % (at, f[len(base):] if array else "0"))
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "xva_hip.h"\nint main(void) {\n%s\nreturn 0; }\n' % "\n".join(lines))
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    said = [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    mine = []
+    for t in STRUCTS.values():
+        mine.append(C.sizeof(t))
+        mine += [getattr(t, f).offset for f, _ in t._fields_]
+    assert said == mine
+
+
+A = 1 << 20        # an address for arguments that are refused before anything reads them
+
+
+def _diff(**kw):
+    base = dict(q=A, k=A, v=A, lam=A, out=A, dtype=1, B=1, Tq=4, Tk=4, H=2, Hk=1, d=16, causal=0, scale=0.25)
+    return S._DiffAttentionArgs(**{**base, **kw})
+
+
+@pytest.mark.parametrize("bad,says", [(dict(q=None), "null"), (dict(dtype=0), "dtype"), (dict(d=12), "head width"), (dict(d=72), "head width"), (dict(Hk=0), "Hk"),
+                                      (dict(H=3, Hk=2), "Hk"), (dict(B=-1), "B -1"), (dict(scale=0.0), "scale"), (dict(q=A + 2), "aligned"),
+                                      (dict(k_stride1=4), "strides"), (dict(out=None), "null"), (dict(lse=A), "null"), (dict(Tq=1 << 30), "Tq")])
+def test_diff_attention_refuses(bad, says):
+    assert _lib.lib.xva_diff_attention_fwd(C.byref(_diff(**bad)), None, 0, None) < 0
+    assert says in _lib.lib.xva_last_error().decode()
+
+
+def test_diff_attention_backward_refuses_a_small_workspace():
+    a = _diff(dout=A, maps=A, lse=A, dq=A, dk=A, dv=A, dlam=A)
+    need = _lib.lib.xva_diff_attention_workspace_bytes(C.byref(a), 1)
+    assert need > 0
+    assert _lib.lib.xva_diff_attention_bwd(C.byref(a), A, need - 1, None) == -3
+    assert _lib.lib.xva_diff_attention_bwd(C.byref(a), None, need, None) == -3
+    assert _lib.lib.xva_diff_attention_bwd(C.byref(_diff()), A, need, None) < 0
+
+
+@pytest.mark.parametrize("bad,says", [(dict(q=None), "null"), (dict(turns=None), "null"), (dict(dtype=3), "dtype"), (dict(rd=3), "rotary width"), (dict(rd=34), "rotary width"),
+                                      (dict(D=9000), "rotary width"), (dict(k=None), "null keys"), (dict(q_out=A), "in place"), (dict(q_out=A, k_out=A), "other strides"),
+                                      (dict(B=1 << 20, T=1 << 12), "tokens"), (dict(H=0), "H 0")])
+def test_rotary_refuses(bad, says):
+    base = dict(q=A, k=A, q_out=2 * A, k_out=2 * A, turns=A, dtype=0, B=1, T=2, H=2, Hk=1, D=32, rd=32, gain=1.0, q_stride0=64)
+    assert _lib.lib.xva_rotary(C.byref(S._RotaryArgs(**{**base, **bad})), None) < 0
+    assert says in _lib.lib.xva_last_error().decode()
+
+
+@pytest.mark.parametrize("bad,says", [(dict(x=None), "null"), (dict(mean=None), "null"), (dict(dtype=-1), "dtype"), (dict(G=5), "groups"), (dict(G=0), "groups"),
+                                      (dict(act=9), "activation"), (dict(eps=-1.0), "eps"), (dict(T=500, C=16384, G=2), "vectors"), (dict(T=500, C=4096, G=4096), "2048 groups"),
+                                      (dict(T=500, C=1025, G=1), "vectors")])
+def test_group_norm_refuses(bad, says):
+    base = dict(x=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3, C=32, G=4, act=0, eps=1e-5)
+    assert _lib.lib.xva_group_norm_act_fwd(C.byref(S._GroupNormArgs(**{**base, **bad})), None, 0, None) < 0
+    assert says in _lib.lib.xva_last_error().decode()
+
+
+def test_group_norm_refuses_a_small_workspace():
+    a = S._GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3000, C=32, G=4, act=0, eps=1e-5)
+    for bwd, call in ((0, _lib.lib.xva_group_norm_act_fwd), (1, _lib.lib.xva_group_norm_act_bwd)):
+        need = _lib.lib.xva_group_norm_workspace_bytes(C.byref(a), bwd)
+        assert need > 0 and call(C.byref(a), A, need - 1, None) == -3
+
+
+@pytest.mark.parametrize("bad,says", [(dict(x=None), "null"), (dict(last=None), "null"), (dict(dtype=5), "dtype"), (dict(C=0), "C 0"), (dict(T=-1), "T -1"),
+                                      (dict(B=1 << 20, C=1 << 12), "B ")])
+def test_recurrence_refuses(bad, says):
+    base = dict(x=A, gate=A, h=A, last=A, dtype=0, B=2, T=3, C=8)
+    assert _lib.lib.xva_recurrence_fwd(C.byref(S._RecurrenceArgs(**{**base, **bad})), None, 0, None) < 0
+    assert says in _lib.lib.xva_last_error().decode()
+
+
+def test_recurrence_refuses_a_small_workspace():
+    need = _lib.lib.xva_recurrence_workspace_bytes(1, 30000, 64)
+    assert need > 0
+    assert _lib.lib.xva_recurrence_fwd(C.byref(S._RecurrenceArgs(x=A, gate=A, h=A, last=A, dtype=0, B=1, T=30000, C=64)), A, need - 1, None) == -3
+    assert _lib.lib.xva_recurrence_bwd(C.byref(S._RecurrenceArgs(x=A, gate=A, dtype=0, B=1, T=30000, C=64)), A, need, None) < 0

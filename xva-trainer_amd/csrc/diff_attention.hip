@@ -1,0 +1,696 @@
+// diff_attention.hip — differential attention: the difference of two softmax maps over shared values, 16-bit operands (gfx950).
+//
+//   S_m = scale q_m k_m^T (m = 1, 2),  P_m = softmax(S_m) over the visible keys,  O = (P_1 - lam P_2) V,  lam a learned number of each head
+//   dP = dO V^T,  D_m = rowsum(dO o P_m V),  dS_1 = P_1 o (dP - D_1),  dS_2 = -lam P_2 o (dP - D_2)
+//   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dV = (P_1 - lam P_2)^T dO,  dlam = - sum P_2 o dP
+//   Key heads may be fewer than query heads (their gradients add up); a query of an item with ql queries and kl keys sees keys j < kl, and with `causal`
+//   j <= i + kl - ql.  A row that sees nothing leaves as zeros and gives no gradient.
+//
+// Bound: MFMA and the exponentials beside it.  Flash-style: no score leaves the chip.
+//   forward : a workgroup takes 128 queries of a head, 32 to a wave; the two maps run their own online softmax over 64-key tiles and share every fragment of
+//             V (one LDS read feeds both maps' products).  Base-2 exponentials, the scale folded in; the running maximum is only moved when a tile exceeds it
+//             by 2^8, so the accumulators are rescaled in the first tiles and hardly ever after.
+//   backward: dK / dV by key block and dq by query block, each rebuilding the maps from the saved logsumexp; no atomics, so results repeat bit for bit.
+//             dP is shared by both maps, and dV takes P_1 - lam P_2 in one product: 16 d + 12 d multiply-adds x 2 a pair and head (d: width of one map's
+//             query).  dlam is summed from fp32 P_2 o dP beside dq, not from rounded outputs.
+// Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands (the accumulators are fp32; sums, maxima and logsumexp stay fp32).
+//
+// Tiles: 64 rows x 64 columns of 16-bit values (attn_tile.h).  d <= 32: one image holds both maps' 32 columns side by side; d <= 64: one image for each map.
+// V and dO (2 d wide): one or two images.  Columns behind d read a zero page, rows behind the last live one read that one with P = 0.
+#include "attn_tile.h"
+#include "../../include/xva_hip.h"
+
+namespace {
+using namespace xva_glds;
+using xva_attn::Frag;
+using xva_attn::TILE;
+using xva_attn::pack_rows;
+
+struct Args {
+    const uint16_t *q, *k, *v, *dout;
+    uint16_t *out, *maps, *dq, *dk, *dv;
+    const float* lam;
+    float *lse, *D, *dlam_part;
+    const int32_t *ql, *kl;
+    int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
+    int B, Tq, Tk, H, Hk, share, d, causal;
+    float scale, c;                               // c = scale log2 e
+};
+// contiguous results: out-of-line maps (2, B, Tq, H, 2 d), dq (B, Tq, H, 2, d), dk (B, Tk, Hk, 2, d), dv (B, Tk, Hk, 2 d); lse, D (2, B, H, Tq), base 2
+
+template <int D16> struct Shape {
+    static constexpr int NI = D16 <= 2 ? 1 : 2;   // 64-column images of a q / k tile, and of a v / dO tile
+    static constexpr int KH = NI;                 // 32-wide MFMA steps over d of one map
+    static constexpr int VH = NI * 2;             // 32-wide MFMA steps over 2 d
+    static constexpr int DT = D16;                // 16-column tiles of one map's d
+    static constexpr int VT = D16 * 2;            // 16-column tiles of 2 d
+};
+
+__device__ __forceinline__ int len_of(const int32_t* l, int b, int T) { return l ? min(max(l[b], 0), T) : T; }
+
+// column of chunk c (8 columns) of image im of a q / k tile -> (map, first d index)
+template <int NI> __device__ __forceinline__ void qk_chunk(int im, int c, int& map, int& d0) {
+    if constexpr (NI == 2) { map = im; d0 = c * 8; } else { map = c >> 2; d0 = (c & 3) * 8; }
+}
+
+// DMA of the NI images of a q / k tile: rows row0 .. row0 + 63, clamped to rmax (>= 0); 4 waves, 2 instructions an image each
+template <int NI>
+__device__ __forceinline__ void dma_qk(const uint16_t* base, int64_t ld, int64_t map_stride, int d, int row0, int rmax, XVA_LDS uint8_t* tile, int lane, int wave) {
+#pragma unroll
+    for (int im = 0; im < NI; ++im)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int Q = q * 4 + wave, r = Q * 8 + (lane >> 3), p = lane & 7;
+            const int c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
+            int map, d0;
+            qk_chunk<NI>(im, c, map, d0);
+            const uint16_t* src = d0 < d ? base + (int64_t)min(row0 + r, rmax) * ld + map * map_stride + d0 : reinterpret_cast<const uint16_t*>(g_zero_page);
+            __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(tile + im * TILE + Q * 1024), 16, 0, 0);
+        }
+}
+template <int NI>
+__device__ __forceinline__ void dma_v(const uint16_t* base, int64_t ld, int d, int row0, int rmax, XVA_LDS uint8_t* tile, int lane, int wave) {
+#pragma unroll
+    for (int im = 0; im < NI; ++im)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int Q = q * 4 + wave, r = Q * 8 + (lane >> 3), p = lane & 7;
+            const int c = im * 64 + (((((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1)) * 8);
+            const uint16_t* src = c < 2 * d ? base + (int64_t)min(row0 + r, rmax) * ld + c : reinterpret_cast<const uint16_t*>(g_zero_page);
+            __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(tile + im * TILE + Q * 1024), 16, 0, 0);
+        }
+}
+// 8 elements at column d0 of a row as an MFMA operand, zero behind `width`
+__device__ __forceinline__ bf16x8 ld_edge(const uint16_t* row, int d0, int width) {
+    const uint4 z = {0, 0, 0, 0};
+    return __builtin_bit_cast(bf16x8, d0 < width ? *reinterpret_cast<const uint4*>(row + d0) : z);
+}
+// image and 32-column half of MFMA step kh of map m
+template <int NI> __device__ __forceinline__ int qk_image(int m) { return NI == 2 ? m : 0; }
+template <int NI> __device__ __forceinline__ int qk_half(int m, int kh) { return NI == 2 ? kh : m; }
+// image and 16-column tile of d tile dt of map m
+template <int NI> __device__ __forceinline__ int qk_tile(int m, int dt) { return NI == 2 ? dt : m * 2 + dt; }
+
+#define MFMA(x, y, z) mma16<F16>(x, y, z)
+#define ZERO4 ((f32x4){0.f, 0.f, 0.f, 0.f})
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ================================================================================ forward ====
+template <int D16, bool F16, bool TRAIN>
+__global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
+    using S = Shape<D16>;
+    constexpr int NI = S::NI;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE];       // {K V} x 2
+    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
+    // the last query blocks see most keys under `causal`: they start first
+    const int nqb = gridDim.x / (a.B * a.H);
+    const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
+    const int h = bh % a.H, b = bh / a.H, q0 = qblk * 128;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
+    const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+    const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+    const uint16_t* qp = a.q + b * a.qb + h * a.qh;
+    const int wrow = q0 + wave * 32;
+    // keys that some query of the workgroup / of the wave sees, and that every query of the wave sees
+    auto seen_by = [&](int row) { return a.causal ? max(min(kl, row + off + 1), 0) : kl; };
+    const int wg_keys = q0 < ql ? seen_by(min(q0 + 127, ql - 1)) : 0;
+    const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
+    const int whole_keys = seen_by(wrow);
+    const int tiles = (wg_keys + 63) / 64;
+    Frag fr; fr.init(lane);
+    bf16x8 qf[2][2][S::KH];
+    int limit[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int row = wrow + rt * 16 + i;
+        limit[rt] = row < ql ? seen_by(row) : 0;
+        const uint16_t* qr = qp + (int64_t)min(row, max(ql - 1, 0)) * a.qt;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = tiles ? ld_edge(qr + m * a.qm, kh * 32 + g * 8, a.d) : ld_edge(qr, 1, 0);
+    }
+    f32x4 o[2][2][S::VT];
+    float mx[2][2], sum[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            mx[m][rt] = -INFINITY; sum[m][rt] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] = ZERO4;
+        }
+    if (tiles) {
+        dma_qk<NI>(kp, a.kt, a.km, a.d, 0, kl - 1, smem, lane, wave);
+        dma_v<NI>(vp, a.vt, a.d, 0, kl - 1, smem + NI * TILE, lane, wave);
+    }
+    __syncthreads();
+    for (int jb = 0; jb < tiles; ++jb) {
+        const XVA_LDS uint8_t* Kt = smem + (jb & 1) * 2 * NI * TILE;
+        const XVA_LDS uint8_t* Vt = Kt + NI * TILE;
+        if (jb + 1 < tiles) {
+            XVA_LDS uint8_t* next = smem + ((jb & 1) ^ 1) * 2 * NI * TILE;
+            dma_qk<NI>(kp, a.kt, a.km, a.d, (jb + 1) * 64, kl - 1, next, lane, wave);
+            dma_v<NI>(vp, a.vt, a.d, (jb + 1) * 64, kl - 1, next + NI * TILE, lane, wave);
+        }
+        if (jb * 64 < wave_keys) {
+            const bool whole = (jb + 1) * 64 <= whole_keys;
+            bf16x8 pf[2][2][2];
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                f32x4 s[2][4];
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt) {
+                    s[0][kt] = ZERO4; s[1][kt] = ZERO4;
+#pragma unroll
+                    for (int kh = 0; kh < S::KH; ++kh) {
+                        const bf16x8 kf = fr.read_kc(Kt + qk_image<NI>(m) * TILE, kt, qk_half<NI>(m, kh));
+                        s[0][kt] = MFMA(kf, qf[m][0][kh], s[0][kt]);           // [key g * 4 + r][row lane & 15]
+                        s[1][kt] = MFMA(kf, qf[m][1][kh], s[1][kt]);
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (jb * 64 + kt * 16 + g * 4 + r >= limit[rt]) s[rt][kt][r] = -INFINITY;
+                }
+                float top[2];
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
+                    float t = -INFINITY;
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) t = fmaxf(t, s[rt][kt][r]);
+                    t = fmaxf(t, __shfl_xor(t, 16, 64));
+                    top[rt] = fmaxf(t, __shfl_xor(t, 32, 64));
+                }
+                // (top > mx = -inf also where a first key shows up: the difference is +inf)
+                const bool grew = (top[0] - mx[m][0]) * a.c > 8.f || (top[1] - mx[m][1]) * a.c > 8.f;
+                if (__any(grew)) {
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt) {
+                        const float now = fmaxf(mx[m][rt], top[rt]);
+                        const float alpha = mx[m][rt] == now ? 1.f : exp2_((mx[m][rt] - now) * a.c);
+                        mx[m][rt] = now;
+                        sum[m][rt] *= alpha;
+#pragma unroll
+                        for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] *= alpha;
+                    }
+                }
+#pragma unroll
+                for (int rt = 0; rt < 2; ++rt) {
+                    const float base = mx[m][rt] == -INFINITY ? 0.f : mx[m][rt] * a.c;
+#pragma unroll
+                    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = exp2_(s[rt][kt][r] * a.c - base);
+                            sum[m][rt] += p;
+                            s[rt][kt][r] = p;
+                        }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) pf[m][rt][t] = pack_rows<F16>(s[rt][2 * t], s[rt][2 * t + 1]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int dt = 0; dt < S::VT; ++dt) {
+                    const bf16x8 vf = fr.read_tr(Vt + (dt >> 2) * TILE, dt & 3, t);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int rt = 0; rt < 2; ++rt) o[m][rt][dt] = MFMA(vf, pf[m][rt][t], o[m][rt][dt]);     // [column g * 4 + r][row lane & 15]
+                }
+        }
+        __syncthreads();
+    }
+    const float lam = a.lam[h];
+    const int w = 2 * a.d;
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int row = wrow + rt * 16 + i;
+        float inv[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float l = sum[m][rt];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            const bool seen = limit[rt] > 0;
+            inv[m] = seen ? 1.f / l : 0.f;
+            if (TRAIN && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? mx[m][rt] * a.c + __log2f(l) : INFINITY;
+        }
+        if (row >= a.Tq) continue;
+        uint16_t* out = a.out + b * a.ob + row * a.ot + h * a.oh;
+        uint16_t* m0 = TRAIN ? a.maps + (((int64_t)b * a.Tq + row) * a.H + h) * w : nullptr;
+        const int64_t plane = (int64_t)a.B * a.Tq * a.H * w;
+#pragma unroll
+        for (int dt = 0; dt < S::VT; ++dt) {
+            const int col = dt * 16 + g * 4;
+            if (col >= w) continue;
+            float u[4], v[4], r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u[e] = limit[rt] > 0 ? o[0][rt][dt][e] * inv[0] : 0.f;
+                v[e] = limit[rt] > 0 ? o[1][rt][dt][e] * inv[1] : 0.f;
+                r[e] = u[e] - lam * v[e];
+            }
+            *reinterpret_cast<uint2*>(out + col) = make_uint2(pack2<F16>(r[0], r[1]), pack2<F16>(r[2], r[3]));
+            if (TRAIN) {
+                *reinterpret_cast<uint2*>(m0 + col) = make_uint2(pack2<F16>(u[0], u[1]), pack2<F16>(u[2], u[3]));
+                *reinterpret_cast<uint2*>(m0 + plane + col) = make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
+            }
+        }
+    }
+}
+
+// ================================================================================ backward ====
+// D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns
+template <bool F16>
+__global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
+    const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tq * a.H;
+    const int c = (threadIdx.x & 15) * 8, w = 2 * a.d;
+    float s[2] = {0.f, 0.f};
+    const int64_t bt = id / a.H;
+    const int h = (int)(id - bt * a.H), b = (int)(bt / a.Tq), t = (int)(bt - (int64_t)b * a.Tq);
+    if (id < rows && c < w && t < len_of(a.ql, b, a.Tq)) {
+        const uint4 gr = *reinterpret_cast<const uint4*>(a.dout + b * a.gb + t * a.gt + h * a.gh + c);
+        const uint32_t gw[4] = {gr.x, gr.y, gr.z, gr.w};
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            const uint4 od = *reinterpret_cast<const uint4*>(a.maps + (m * rows + id) * w + c);
+            const uint32_t ow[4] = {od.x, od.y, od.z, od.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float g0, g1, o0, o1;
+                unpack2<F16>(gw[e], g0, g1); unpack2<F16>(ow[e], o0, o1);
+                s[m] += g0 * o0 + g1 * o1;
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        s[m] += __shfl_xor(s[m], 1, 64); s[m] += __shfl_xor(s[m], 2, 64); s[m] += __shfl_xor(s[m], 4, 64); s[m] += __shfl_xor(s[m], 8, 64);
+    }
+    if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = s[threadIdx.x & 1];
+}
+
+// dK, dV of 128 keys of a key head, 32 to a wave, over the query heads that share it and their 64-query tiles
+template <int D16, bool F16>
+__global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
+    using S = Shape<D16>;
+    constexpr int NI = S::NI;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE + 2 * 1024];     // {Q dO} x 2 | {lse1 lse2 D1 D2} x 2
+    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
+    XVA_LDS uint8_t* stat = smem + 4 * NI * TILE;
+    const int kblk = blockIdx.x / (a.B * a.Hk), bh = blockIdx.x % (a.B * a.Hk);                // (the first keys are seen by most queries: they start first)
+    const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 128;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql;
+    const int wkey = k0 + wave * 32, w = 2 * a.d;
+    Frag fr; fr.init(lane);
+    // queries that see a key of the workgroup: from `first` on
+    const int first = a.causal ? max(k0 - off, 0) : 0;
+    const bool any = k0 < kl && first < ql;
+    const int t0 = first / 64, per_head = any ? (ql + 63) / 64 - t0 : 0, total = per_head * a.share;
+    bf16x8 kf[2][2][S::KH], vf[2][S::VH];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        const int key = min(wkey + kt * 16 + i, max(kl - 1, 0));
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kh = 0; kh < S::KH; ++kh) kf[m][kt][kh] = ld_edge(a.k + b * a.kb + hk * a.kh + m * a.km + key * a.kt, kh * 32 + g * 8, any ? a.d : 0);
+#pragma unroll
+        for (int kh = 0; kh < S::VH; ++kh) vf[kt][kh] = ld_edge(a.v + b * a.vb + hk * a.vh + key * a.vt, kh * 32 + g * 8, any ? w : 0);
+    }
+    f32x4 dk[2][2][S::DT], dv[2][S::VT];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < S::DT; ++dt) dk[m][kt][dt] = ZERO4;
+#pragma unroll
+        for (int dt = 0; dt < S::VT; ++dt) dv[kt][dt] = ZERO4;
+    }
+    auto fetch = [&](int it, int buf) {
+        const int hs = it / per_head, h = hk * a.share + hs, row0 = (t0 + it - hs * per_head) * 64;
+        XVA_LDS uint8_t* to = smem + buf * 2 * NI * TILE;
+        dma_qk<NI>(a.q + b * a.qb + h * a.qh, a.qt, a.qm, a.d, row0, ql - 1, to, lane, wave);
+        dma_v<NI>(a.dout + b * a.gb + h * a.gh, a.gt, a.d, row0, ql - 1, to + NI * TILE, lane, wave);
+        const float* src = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + min(row0 + lane, ql - 1);
+        __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(stat + buf * 1024 + wave * 256), 4, 0, 0);
+    };
+    if (total) fetch(0, 0);
+    __syncthreads();
+    for (int it = 0; it < total; ++it) {
+        const int hs = it / per_head, row0 = (t0 + it - hs * per_head) * 64;
+        const float lam = a.lam[hk * a.share + hs];
+        if (it + 1 < total) fetch(it + 1, (it & 1) ^ 1);
+        const XVA_LDS uint8_t* Qt = smem + (it & 1) * 2 * NI * TILE;
+        const XVA_LDS uint8_t* Ot = Qt + NI * TILE;
+        const XVA_LDS uint8_t* st = stat + (it & 1) * 1024;
+        // every row of the tile sees every key of the wave
+        const bool whole = row0 + 64 <= ql && wkey + 32 <= kl && (!a.causal || wkey + 31 <= row0 + off);
+        const bool none = wkey >= kl || (a.causal && wkey > row0 + 63 + off);
+        if (!none) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 s[2][2][2], dp[2][2];                 // [map][row tile][key tile], [row g * 4 + r][key lane & 15]
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int rt = 2 * t + u;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) { s[0][u][kt] = ZERO4; s[1][u][kt] = ZERO4; dp[u][kt] = ZERO4; }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int kh = 0; kh < S::KH; ++kh) {
+                            const bf16x8 qf = fr.read_kc(Qt + qk_image<NI>(m) * TILE, rt, qk_half<NI>(m, kh));
+#pragma unroll
+                            for (int kt = 0; kt < 2; ++kt) s[m][u][kt] = MFMA(qf, kf[m][kt][kh], s[m][u][kt]);
+                        }
+#pragma unroll
+                    for (int kh = 0; kh < S::VH; ++kh) {
+                        const bf16x8 of = fr.read_kc(Ot + (kh >> 1) * TILE, rt, kh & 1);
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt) dp[u][kt] = MFMA(of, vf[kt][kh], dp[u][kt]);
+                    }
+                }
+                bf16x8 pf[2], df[2][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int rt = 2 * t + u;
+                    const XVA_LDS uint8_t* at = st + (rt * 16 + g * 4) * 4;
+                    const f32x4 L1 = *reinterpret_cast<const XVA_LDS f32x4*>(at), L2 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 256);
+                    const f32x4 D1 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 512), D2 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float p1 = exp2_(s[0][u][kt][r] * a.c - L1[r]), p2 = exp2_(s[1][u][kt][r] * a.c - L2[r]);
+                            if (!whole) {
+                                const int row = row0 + rt * 16 + g * 4 + r, key = wkey + kt * 16 + i;
+                                const bool ok = row < ql && key < kl && (!a.causal || key <= row + off);
+                                p1 = ok ? p1 : 0.f; p2 = ok ? p2 : 0.f;
+                            }
+                            p2 *= -lam;
+                            const float x = dp[u][kt][r];
+                            s[0][u][kt][r] = p1 * (x - D1[r]);
+                            s[1][u][kt][r] = p2 * (x - D2[r]);
+                            dp[u][kt][r] = p1 + p2;
+                        }
+                }
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    pf[kt] = pack_rows<F16>(dp[0][kt], dp[1][kt]);
+                    df[0][kt] = pack_rows<F16>(s[0][0][kt], s[0][1][kt]);
+                    df[1][kt] = pack_rows<F16>(s[1][0][kt], s[1][1][kt]);
+                }
+#pragma unroll
+                for (int dt = 0; dt < S::VT; ++dt) {
+                    const bf16x8 of = fr.read_tr(Ot + (dt >> 2) * TILE, dt & 3, t);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) dv[kt][dt] = MFMA(of, pf[kt], dv[kt][dt]);                  // [column g * 4 + r][key lane & 15]
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int dt = 0; dt < S::DT; ++dt) {
+                        const bf16x8 qf = fr.read_tr(Qt + qk_image<NI>(m) * TILE, qk_tile<NI>(m, dt), t);
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt) dk[m][kt][dt] = MFMA(qf, df[m][kt], dk[m][kt][dt]);
+                    }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        const int key = wkey + kt * 16 + i;
+        if (key >= a.Tk) continue;
+        const int64_t row = ((int64_t)b * a.Tk + key) * a.Hk + hk;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < S::DT; ++dt)
+                if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + g * 4, dk[m][kt][dt], a.scale);
+#pragma unroll
+        for (int dt = 0; dt < S::VT; ++dt)
+            if (dt * 16 + g * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + g * 4, dv[kt][dt], 1.f);
+    }
+}
+
+// dq of 128 queries of a head, 32 to a wave, and their part of dlam
+template <int D16, bool F16>
+__global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
+    using S = Shape<D16>;
+    constexpr int NI = S::NI;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE];
+    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
+    const int nqb = gridDim.x / (a.B * a.H);
+    const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
+    const int h = bh % a.H, b = bh / a.H, q0 = qblk * 128;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, i = lane & 15;
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
+    const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+    const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+    const int wrow = q0 + wave * 32, w = 2 * a.d;
+    auto seen_by = [&](int row) { return a.causal ? max(min(kl, row + off + 1), 0) : kl; };
+    const int wg_keys = q0 < ql ? seen_by(min(q0 + 127, ql - 1)) : 0;
+    const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
+    const int whole_keys = seen_by(wrow);
+    const int tiles = (wg_keys + 63) / 64;
+    Frag fr; fr.init(lane);
+    bf16x8 qf[2][2][S::KH], of[2][S::VH];
+    int limit[2];
+    float L[2][2], Dr[2][2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int row = wrow + rt * 16 + i, safe = min(row, max(ql - 1, 0));
+        limit[rt] = row < ql ? seen_by(row) : 0;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = ld_edge(a.q + b * a.qb + h * a.qh + m * a.qm + safe * a.qt, kh * 32 + g * 8, tiles ? a.d : 0);
+            const int64_t at = (((int64_t)m * a.B + b) * a.H + h) * a.Tq + safe;
+            L[m][rt] = a.lse[at]; Dr[m][rt] = a.D[at];
+        }
+#pragma unroll
+        for (int kh = 0; kh < S::VH; ++kh) of[rt][kh] = ld_edge(a.dout + b * a.gb + h * a.gh + safe * a.gt, kh * 32 + g * 8, tiles ? w : 0);
+    }
+    f32x4 dq[2][2][S::DT];
+    float dl = 0.f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int dt = 0; dt < S::DT; ++dt) dq[m][rt][dt] = ZERO4;
+    if (tiles) {
+        dma_qk<NI>(kp, a.kt, a.km, a.d, 0, kl - 1, smem, lane, wave);
+        dma_v<NI>(vp, a.vt, a.d, 0, kl - 1, smem + NI * TILE, lane, wave);
+    }
+    __syncthreads();
+    for (int jb = 0; jb < tiles; ++jb) {
+        const XVA_LDS uint8_t* Kt = smem + (jb & 1) * 2 * NI * TILE;
+        const XVA_LDS uint8_t* Vt = Kt + NI * TILE;
+        if (jb + 1 < tiles) {
+            XVA_LDS uint8_t* next = smem + ((jb & 1) ^ 1) * 2 * NI * TILE;
+            dma_qk<NI>(kp, a.kt, a.km, a.d, (jb + 1) * 64, kl - 1, next, lane, wave);
+            dma_v<NI>(vp, a.vt, a.d, (jb + 1) * 64, kl - 1, next + NI * TILE, lane, wave);
+        }
+        if (jb * 64 < wave_keys) {
+            const bool whole = (jb + 1) * 64 <= whole_keys && wrow + 32 <= ql;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x4 s[2][2][2], dp[2][2];                 // [map][key tile][row tile], [key g * 4 + r][row lane & 15]
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int kt = 2 * t + u;
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt) { s[0][u][rt] = ZERO4; s[1][u][rt] = ZERO4; dp[u][rt] = ZERO4; }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int kh = 0; kh < S::KH; ++kh) {
+                            const bf16x8 kf = fr.read_kc(Kt + qk_image<NI>(m) * TILE, kt, qk_half<NI>(m, kh));
+#pragma unroll
+                            for (int rt = 0; rt < 2; ++rt) s[m][u][rt] = MFMA(kf, qf[m][rt][kh], s[m][u][rt]);
+                        }
+#pragma unroll
+                    for (int kh = 0; kh < S::VH; ++kh) {
+                        const bf16x8 vf = fr.read_kc(Vt + (kh >> 1) * TILE, kt, kh & 1);
+#pragma unroll
+                        for (int rt = 0; rt < 2; ++rt) dp[u][rt] = MFMA(vf, of[rt][kh], dp[u][rt]);
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float p1 = exp2_(s[0][u][rt][r] * a.c - L[0][rt]), p2 = exp2_(s[1][u][rt][r] * a.c - L[1][rt]);
+                            if (!whole) {
+                                const bool ok = jb * 64 + kt * 16 + g * 4 + r < limit[rt];
+                                p1 = ok ? p1 : 0.f; p2 = ok ? p2 : 0.f;
+                            }
+                            const float x = dp[u][rt][r];
+                            dl += p2 * x;
+                            s[0][u][rt][r] = p1 * (x - Dr[0][rt]);
+                            s[1][u][rt][r] = p2 * (x - Dr[1][rt]);
+                        }
+                }
+                bf16x8 df[2][2];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int rt = 0; rt < 2; ++rt) df[m][rt] = pack_rows<F16>(s[m][0][rt], s[m][1][rt]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int dt = 0; dt < S::DT; ++dt) {
+                        const bf16x8 kf = fr.read_tr(Kt + qk_image<NI>(m) * TILE, qk_tile<NI>(m, dt), t);
+#pragma unroll
+                        for (int rt = 0; rt < 2; ++rt) dq[m][rt][dt] = MFMA(kf, df[m][rt], dq[m][rt][dt]);       // [column g * 4 + r][row lane & 15]
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    const float lam = a.lam[h];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const int row = wrow + rt * 16 + i;
+        if (row >= a.Tq) continue;
+        uint16_t* dst = a.dq + (((int64_t)b * a.Tq + row) * a.H + h) * w;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int dt = 0; dt < S::DT; ++dt)
+                if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(dst + m * a.d + dt * 16 + g * 4, dq[m][rt][dt], m ? -lam * a.scale : a.scale);
+    }
+    // (the tile loop has ended with a barrier)
+    XVA_LDS float* red = (XVA_LDS float*)smem_raw;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) dl += __shfl_xor(dl, o, 64);
+    if (lane == 0) red[wave] = dl;
+    __syncthreads();
+    if (threadIdx.x == 0) a.dlam_part[((int64_t)h * a.B + b) * nqb + qblk] = red[0] + red[1] + red[2] + red[3];
+}
+
+// dlam[h] = - sum of the head's parts, in a fixed order
+__global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ part, float* __restrict__ dlam, int n) {
+    __shared__ float sh[16];
+    float v = 0.f;
+    for (int k = threadIdx.x; k < n; k += 256) v += part[(int64_t)blockIdx.x * n + k];
+    v = xva_block_sum(v, sh);
+    if (threadIdx.x == 0) dlam[blockIdx.x] = -v;
+}
+#undef MFMA
+
+// -------------------------------------------------------------------------------- host ----
+int check(const xva_diff_attention_args* p, const char* who) {
+    XVA_CHECK_ARG(p, "%s: null argument", who);
+    XVA_CHECK_ARG(p->dtype == 1 || p->dtype == 2, "%s: dtype %d (bf16 or fp16)", who, p->dtype);
+    XVA_CHECK_ARG(p->B >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->Tq < (1 << 30) && p->Tk < (1 << 30) && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0,
+                  "%s: B %d Tq %d Tk %d H %d Hk %d", who, p->B, p->Tq, p->Tk, p->H, p->Hk);
+    XVA_CHECK_ARG(p->d >= 8 && p->d <= 64 && p->d % 8 == 0, "%s: head width %d (a multiple of 8 up to 64)", who, p->d);
+    XVA_CHECK_ARG(p->scale > 0.f, "%s: scale %g", who, p->scale);
+    if (p->B == 0 || p->Tq == 0) return XVA_OK;
+    XVA_CHECK_ARG(p->q && p->lam && (p->Tk == 0 || (p->k && p->v)), "%s: null argument", who);
+    uintptr_t ptrs = (uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out | (uintptr_t)p->dout;
+    int64_t all = 0;
+    for (int e = 0; e < 4; ++e) all |= p->q_stride[e] | p->k_stride[e];
+    for (int e = 0; e < 3; ++e) all |= p->v_stride[e] | p->out_stride[e] | p->dout_stride[e];
+    XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
+    const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 127) / 128);
+    XVA_CHECK_ARG(wgs < (1ll << 31) && kwgs < (1ll << 31), "%s: too many blocks", who);
+    return XVA_OK;
+}
+Args args_of(const xva_diff_attention_args* p) {
+    Args a = {};
+    a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v; a.dout = (const uint16_t*)p->dout;
+    a.out = (uint16_t*)p->out; a.maps = (uint16_t*)p->maps; a.dq = (uint16_t*)p->dq; a.dk = (uint16_t*)p->dk; a.dv = (uint16_t*)p->dv;
+    a.lam = p->lam; a.lse = p->lse; a.ql = p->q_lens; a.kl = p->k_lens;
+    a.qb = p->q_stride[0]; a.qt = p->q_stride[1]; a.qh = p->q_stride[2]; a.qm = p->q_stride[3];
+    a.kb = p->k_stride[0]; a.kt = p->k_stride[1]; a.kh = p->k_stride[2]; a.km = p->k_stride[3];
+    a.vb = p->v_stride[0]; a.vt = p->v_stride[1]; a.vh = p->v_stride[2];
+    a.ob = p->out_stride[0]; a.ot = p->out_stride[1]; a.oh = p->out_stride[2];
+    a.gb = p->dout_stride[0]; a.gt = p->dout_stride[1]; a.gh = p->dout_stride[2];
+    a.B = p->B; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.share = p->H / p->Hk; a.d = p->d; a.causal = p->causal;
+    a.scale = p->scale; a.c = p->scale * 1.44269504088896341f;
+    return a;
+}
+template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
+    const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128));
+    if (train) fwd_kernel<D16, F16, true><<<grid, 256, 0, st>>>(a);
+    else fwd_kernel<D16, F16, false><<<grid, 256, 0, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_t st) {
+    const int nqb = (a.Tq + 127) / 128;
+    const int64_t rows = (int64_t)a.B * a.Tq * a.H;
+    rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    if (a.Tk > 0) {
+        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 127) / 128)), 256, 0, st>>>(a);
+        XVA_LAUNCH_CHECK();
+    }
+    dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb), 256, 0, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    dlam_kernel<<<a.H, 256, 0, st>>>(a.dlam_part, dlam, a.B * nqb);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
+    if (!bwd) return 0;
+    return ((int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128)) * 4;
+}
+}   // namespace
+
+extern "C" int64_t xva_diff_attention_workspace_bytes(const xva_diff_attention_args* p, int backward_pass) {
+    return p && p->B >= 0 && p->Tq >= 0 && p->H >= 1 ? workspace(p, backward_pass != 0) : -1;
+}
+
+#define XVA_DIFF_BY_SHAPE(call)                                                          \
+    switch ((p->d + 15) / 16 * 2 + (p->dtype == 2)) {                                    \
+        case 2: return call(1, false); case 3: return call(1, true);                     \
+        case 4: return call(2, false); case 5: return call(2, true);                     \
+        case 6: return call(3, false); case 7: return call(3, true);                     \
+        case 8: return call(4, false); default: return call(4, true);                    \
+    }
+
+extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws, int64_t ws_bytes, void* stream) {
+    XVA_TRY(check(p, "xva_diff_attention_fwd"));
+    if (p->B == 0 || p->Tq == 0) return XVA_OK;
+    XVA_CHECK_ARG(p->out && (p->maps == nullptr) == (p->lse == nullptr), "xva_diff_attention_fwd: null argument");
+    const Args a = args_of(p);
+#define CALL(D16, F16) forward<D16, F16>(a, p->maps != nullptr, (hipStream_t)stream)
+    XVA_DIFF_BY_SHAPE(CALL)
+#undef CALL
+}
+extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws, int64_t ws_bytes, void* stream) {
+    XVA_TRY(check(p, "xva_diff_attention_bwd"));
+    if (p->B == 0 || p->Tq == 0) return XVA_OK;
+    XVA_CHECK_ARG(p->dout && p->maps && p->lse && p->dq && p->dlam && (p->Tk == 0 || (p->dk && p->dv)), "xva_diff_attention_bwd: null argument");
+    if (ws_bytes < workspace(p, true) || !ws) {
+        xva_set_error("xva_diff_attention_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)workspace(p, true));
+        return XVA_ERR_WS;
+    }
+    Args a = args_of(p);
+    a.D = (float*)ws;
+    a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
+#define CALL(D16, F16) backward<D16, F16>(a, p->dlam, (hipStream_t)stream)
+    XVA_DIFF_BY_SHAPE(CALL)
+#undef CALL
+}

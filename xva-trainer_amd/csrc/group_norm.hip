@@ -1,0 +1,673 @@
+// group_norm.hip — group normalisation with an activation over time-major sequences (B, T, C), channels contiguous (gfx950).
+//
+//   item b, group g of n = C / G channels, N = lens[b] * n live values:
+//   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) r, z = xh w + bias, y = act(z)
+//   dz = dy act'(z);  dw = sum dz xh, dbias = sum dz (over items and rows);  dx = r (w dz - mean(w dz) - xh mean(w dz xh))
+// Rows at or behind an item's length count for nothing: they are not read, and leave as zeros.
+//
+// Bound: HBM.  Two forms, by the size of one (item, group) slab of T x n values:
+//   * a slab that fits the registers of (part of) one wave — each head's norm behind an attention (T = 1), short items: `slab` kernels.  A slab lies over a
+//     power of two of lanes, so every reduction is a few shuffles; x is read once.  dw / dbias stay in the lanes' registers over all the items that a
+//     workgroup passes, leave as one partial row per workgroup and are added in a fixed order.
+//   * longer ones: `tile` kernels over chunks of rows (all channels of a row, so loads are whole lines whatever n is): statistics of each chunk, then one
+//     pass that joins them and writes.  The second read of x is as close behind the first as the size allows.
+// Statistics are two-pass inside a register tile and joined by the exact update of mean and squared deviations (Chan, Golub, LeVeque), so a mean that is
+// large against the deviation costs nothing.  Everything is held in fp32; sums over rows are made in a fixed order, so results repeat bit for bit.
+#include "xva_common.h"
+#include "../../include/xva_hip.h"
+#include "seq_vec.h"
+
+namespace {
+using xva_seq::load_v;
+using xva_seq::store_v;
+
+enum { NONE, RELU, LRELU, TANH, SILU, GELU };
+
+struct Args {
+    const void* x; const void* dy; void* out;              // out: y or dx
+    const float* w; const float* bias;
+    const int32_t* lens;
+    float* mean; float* rstd;                              // (B, G)
+    float* part;                                           // partial results of the first kernel
+    float* item;                                           // (B, 2, C): sums of dz and dz xh of each item
+    float* dw; float* db;
+    int64_t xb, xt, db_, dt_, ob, ot;                      // strides of x, dy and out
+    int B, T, C, G, n, act;
+    float eps, slope;
+    int rows_per_chunk, chunks;
+};
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act, float slope) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float v = z[e];
+        switch (act) {
+            case RELU: z[e] = v > 0.f ? v : (v != v ? v : 0.f); break;
+            case LRELU: z[e] = v > 0.f ? v : slope * v; break;
+            case TANH: z[e] = tanhf(v); break;
+            case SILU: z[e] = v / (1.f + __expf(-v)); break;
+            case GELU: z[e] = 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); break;
+            default: break;
+        }
+    }
+}
+__device__ __forceinline__ float slope_of(float v, int act, float slope) {
+    switch (act) {
+        case RELU: return v > 0.f ? 1.f : 0.f;
+        case LRELU: return v > 0.f ? 1.f : slope;
+        case TANH: { const float t = tanhf(v); return 1.f - t * t; }
+        case SILU: { const float s = sigmoid(v); return s + s * v * (1.f - s); }
+        case GELU: return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * __expf(-0.5f * v * v);
+        default: return 1.f;
+    }
+}
+__device__ __forceinline__ int live_rows(const Args& a, int b) {
+    return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
+}
+// sum over aligned runs of `width` (a power of two) lanes, in every lane
+__device__ __forceinline__ float lanes_sum(float v, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// ================================================================================ slab form ====
+// LPG lanes hold one slab, NV vectors of V values each: vector j = k * LPG + lane of the slab is row j / (n / V), channels (j % (n / V)) * V ...
+// A workgroup holds 256 / LPG slabs: GPB groups of 256 / (LPG * GPB) items, and walks over the items.
+struct SlabPlan { int lpg, gpb, ipb, gy; };
+
+template <int DT, int V, int NV, bool BWD>
+__global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
+    extern __shared__ float sums[];                        // BWD: [256 lanes][NV][2][V]
+    const int lane = threadIdx.x & (s.lpg - 1), slot = threadIdx.x / s.lpg;
+    const int gl = slot % s.gpb, il = slot / s.gpb;
+    const int g = blockIdx.y * s.gpb + gl;
+    const bool mine = il < s.ipb && g < a.G;
+    const int nv = a.n / V, vecs = a.T * nv;
+    int row[NV], ch[NV];
+    float w[NV][V], bias[NV][V], sw[NV][V], sb[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int j = k * s.lpg + lane;
+        row[k] = j < vecs ? j / nv : a.T;                  // a.T: no such row
+        ch[k] = min(g, a.G - 1) * a.n + (j < vecs ? (j % nv) * V : 0);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[k][e] = a.w ? a.w[ch[k] + e] : 1.f;
+            bias[k][e] = a.bias ? a.bias[ch[k] + e] : 0.f;
+            sw[k][e] = sb[k][e] = 0.f;
+        }
+    }
+    for (int64_t b0 = (int64_t)blockIdx.x * s.ipb; b0 < a.B; b0 += (int64_t)gridDim.x * s.ipb) {
+        const int64_t b = b0 + il;
+        const bool on = mine && b < a.B;
+        const int len = on ? live_rows(a, (int)b) : 0;
+        float x[NV][V];
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (row[k] < len) load_v<DT, V>(a.x, b * a.xb + (int64_t)row[k] * a.xt + ch[k], x[k]);
+            else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[k][e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += x[k][e];
+        }
+        const float inv_n = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
+        float mean, rstd;
+        if constexpr (!BWD) {
+            mean = lanes_sum(sum, s.lpg) * inv_n;
+            float sq = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) { const float d = row[k] < len ? x[k][e] - mean : 0.f; sq += d * d; }
+            rstd = rsqrtf(lanes_sum(sq, s.lpg) * inv_n + a.eps);
+            if (on && lane == 0) { a.mean[b * a.G + g] = mean; a.rstd[b * a.G + g] = rstd; }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (!on || row[k] >= a.T) continue;
+                float z[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] = (x[k][e] - mean) * rstd * w[k][e] + bias[k][e];
+                activate<V>(z, a.act, a.slope);
+                if (row[k] >= len) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) z[e] = 0.f;
+                }
+                store_v<DT, V>(a.out, b * a.ob + (int64_t)row[k] * a.ot + ch[k], z);
+            }
+        } else {
+            mean = on ? a.mean[b * a.G + g] : 0.f;
+            rstd = on ? a.rstd[b * a.G + g] : 0.f;
+            float dz[NV][V];
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (row[k] < len) load_v<DT, V>(a.dy, b * a.db_ + (int64_t)row[k] * a.dt_ + ch[k], dz[k]);
+                else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) dz[k][e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = row[k] < len ? (x[k][e] - mean) * rstd : 0.f;
+                    const float d = dz[k][e] * slope_of(xh * w[k][e] + bias[k][e], a.act, a.slope);
+                    x[k][e] = xh;
+                    sw[k][e] += d * xh; sb[k][e] += d;
+                    dz[k][e] = d * w[k][e];
+                    s1 += dz[k][e]; s2 += dz[k][e] * xh;
+                }
+            }
+            s1 = lanes_sum(s1, s.lpg) * inv_n;
+            s2 = lanes_sum(s2, s.lpg) * inv_n;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (!on || row[k] >= a.T) continue;
+                float d[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] = row[k] < len ? rstd * (dz[k][e] - s1 - x[k][e] * s2) : 0.f;
+                store_v<DT, V>(a.out, b * a.ob + (int64_t)row[k] * a.ot + ch[k], d);
+            }
+        }
+    }
+    if constexpr (BWD) {
+        // the lanes that hold one channel (its items and rows) are added in a fixed order: partial row (blockIdx.x) of (2, C)
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sums[((threadIdx.x * NV + k) * 2) * V + e] = mine ? sb[k][e] : 0.f;
+                sums[((threadIdx.x * NV + k) * 2 + 1) * V + e] = mine ? sw[k][e] : 0.f;
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < s.gpb * a.n; c += 256) {
+            const int cg = c / a.n, cc = c - cg * a.n, v = cc / V, e = cc - v * V;
+            if (blockIdx.y * s.gpb + cg >= a.G) continue;
+            float t1 = 0.f, t2 = 0.f;
+            for (int i = 0; i < s.ipb; ++i)
+                for (int r = 0; r < a.T; ++r) {
+                    const int j = r * nv + v, k = j / s.lpg, th = (i * s.gpb + cg) * s.lpg + j - k * s.lpg;
+                    t1 += sums[((th * NV + k) * 2) * V + e];
+                    t2 += sums[((th * NV + k) * 2 + 1) * V + e];
+                }
+            const int c_all = blockIdx.y * s.gpb * a.n + c;
+            a.part[((int64_t)blockIdx.x * 2) * a.C + c_all] = t1;
+            a.part[((int64_t)blockIdx.x * 2 + 1) * a.C + c_all] = t2;
+        }
+    }
+}
+
+// ================================================================================ tile form ====
+// A thread owns one vector of V channels and every `step`-th row of its chunk; lc = C / V vectors side by side, step = blockDim.x / lc rows at once.
+constexpr int NR = 8;      // rows of a thread in one register tile
+
+struct Tile {
+    int lc, step, v, r; bool on;
+    __device__ __forceinline__ Tile(int C, int V) {
+        lc = C / V; step = blockDim.x / lc;
+        r = threadIdx.x / lc; v = threadIdx.x - r * lc;
+        on = r < step;
+    }
+};
+// per-thread sums -> red[row slot][channel]
+template <int V> __device__ __forceinline__ void put(float* red, const Tile& t, int C, const float (&s)[V]) {
+    if (t.on) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) red[t.r * C + t.v * V + e] = s[e];
+    }
+}
+// group sums of red into out[g], by runs of `run` lanes (a power of two)
+__device__ __forceinline__ void group_sums(const float* red, float* out, const Tile& t, int C, int G, int n, int run) {
+    const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
+    for (int g0 = 0; g0 < G; g0 += per) {
+        const int g = g0 + threadIdx.x / run;
+        float v = 0.f;
+        if (g < G)
+            for (int sl = 0; sl < t.step; ++sl)
+                for (int c = lane; c < n; c += run) v += red[sl * C + g * n + c];
+        v = lanes_sum(v, run);
+        if (g < G && lane == 0) out[g] = v;
+    }
+}
+__device__ __forceinline__ int run_of(int n) { int r = 1; while (r < n && r < 64) r <<= 1; return r; }
+
+// statistics of one chunk: part[(b * chunks + chunk) * G + g] = (mean, sum of squared deviations)
+template <int DT, int V>
+__global__ __launch_bounds__(1024) void tile_stats_kernel(Args a) {
+    extern __shared__ float lds[];
+    const Tile t(a.C, V);
+    float* red = lds;                          // step * C
+    float* mean = red + t.step * a.C;          // G: running mean, then squared deviations
+    float* m2 = mean + a.G;
+    float* now = m2 + a.G;                     // G: this tile's sums
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.n);
+    const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, len);
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) mean[g] = m2[g] = 0.f;
+    float before = 0.f;                        // rows joined so far
+    int mine[V];                               // groups of this thread's channels
+#pragma unroll
+    for (int e = 0; e < V; ++e) mine[e] = t.on ? (t.v * V + e) / a.n : 0;
+    const int64_t base = (int64_t)b * a.xb + t.v * V;
+    for (int r0 = first; r0 < end; r0 += t.step * NR) {
+        float f[NR][V], s[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const int r = r0 + k * t.step + t.r;
+            if (t.on && r < end) load_v<DT, V>(a.x, base + (int64_t)r * a.xt, f[k]);
+            else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[k][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NR; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += f[k][e];
+        __syncthreads();
+        put<V>(red, t, a.C, s);
+        __syncthreads();
+        group_sums(red, now, t, a.C, a.G, a.n, run);
+        __syncthreads();
+        const float rows = (float)min(end - r0, t.step * NR), inv = 1.f / (rows * (float)a.n);
+        float mu[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) { mu[e] = t.on ? now[mine[e]] * inv : 0.f; s[e] = 0.f; }
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            if (r0 + k * t.step + t.r < end) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) { const float d = f[k][e] - mu[e]; s[e] += d * d; }
+            }
+        }
+        put<V>(red, t, a.C, s);
+        // join with the tiles before: the mean first, while `now` still holds the sums
+        const float share = rows / (before + rows);
+        for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
+            const float d = now[g] * inv - mean[g];
+            m2[g] += d * d * before * share * (float)a.n;
+            mean[g] += d * share;
+        }
+        __syncthreads();
+        group_sums(red, now, t, a.C, a.G, a.n, run);
+        __syncthreads();
+        for (int g = threadIdx.x; g < a.G; g += blockDim.x) m2[g] += now[g];
+        before += rows;
+    }
+    __syncthreads();
+    float2* out = reinterpret_cast<float2*>(a.part) + (int64_t)blockIdx.x * a.G;
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) out[g] = make_float2(mean[g], m2[g]);
+}
+
+// joins the chunks' statistics (every workgroup for itself: a few hundred bytes), then normalises its chunk
+template <int DT, int V>
+__global__ __launch_bounds__(1024) void tile_apply_kernel(Args a) {
+    extern __shared__ float lds[];
+    float* mean = lds;
+    float* rstd = lds + a.G;
+    const Tile t(a.C, V);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.chunks);
+    const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, a.T);
+    const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
+    const float2* part = reinterpret_cast<const float2*>(a.part) + (int64_t)b * a.chunks * a.G;
+    const float inv = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
+    for (int g0 = 0; g0 < a.G; g0 += per) {
+        const int g = g0 + threadIdx.x / run;
+        float2 p = make_float2(0.f, 0.f);
+        float rows = 0.f;
+        if (g < a.G && lane < a.chunks) {
+            rows = (float)min(max(len - lane * a.rows_per_chunk, 0), a.rows_per_chunk);
+            if (rows > 0.f) p = part[lane * a.G + g];
+        }
+        const float mu = lanes_sum(p.x * (rows * (float)a.n), run) * inv;
+        const float d = p.x - mu;
+        const float var = lanes_sum(p.y + d * d * (rows * (float)a.n), run) * inv;
+        if (g < a.G && lane == 0) {
+            mean[g] = mu; rstd[g] = rsqrtf(var + a.eps);
+            if (chunk == 0) { a.mean[(int64_t)b * a.G + g] = mean[g]; a.rstd[(int64_t)b * a.G + g] = rstd[g]; }
+        }
+    }
+    __syncthreads();
+    if (!t.on) return;
+    float mu[V], w[V], bias[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const int c = t.v * V + e, g = c / a.n;
+        mu[e] = mean[g];
+        w[e] = rstd[g] * (a.w ? a.w[c] : 1.f);
+        bias[e] = a.bias ? a.bias[c] : 0.f;
+    }
+    const int64_t xo = (int64_t)b * a.xb + t.v * V, oo = (int64_t)b * a.ob + t.v * V;
+    int r = first + t.r;
+    for (; r + 3 * t.step < min(end, len); r += 4 * t.step) {
+        float f[4][V];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load_v<DT, V>(a.x, xo + (int64_t)(r + k * t.step) * a.xt, f[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[k][e] = (f[k][e] - mu[e]) * w[e] + bias[e];
+            activate<V>(f[k], a.act, a.slope);
+            store_v<DT, V>(a.out, oo + (int64_t)(r + k * t.step) * a.ot, f[k]);
+        }
+    }
+    for (; r < end; r += t.step) {
+        float f[V];
+        if (r < len) {
+            load_v<DT, V>(a.x, xo + (int64_t)r * a.xt, f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = (f[e] - mu[e]) * w[e] + bias[e];
+            activate<V>(f, a.act, a.slope);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = 0.f;
+        }
+        store_v<DT, V>(a.out, oo + (int64_t)r * a.ot, f);
+    }
+}
+
+// sums of dz and dz xh of one chunk: part[(b * chunks + chunk) * 2 C + which * C + c]
+template <int DT, int V>
+__global__ __launch_bounds__(1024) void tile_dsum_kernel(Args a) {
+    extern __shared__ float red[];
+    const Tile t(a.C, V);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b);
+    const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, len);
+    float s1[V], s2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+    if (t.on) {
+        float mu[V], rs[V], w[V], bias[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int c = t.v * V + e, g = c / a.n;
+            mu[e] = a.mean[(int64_t)b * a.G + g]; rs[e] = a.rstd[(int64_t)b * a.G + g];
+            w[e] = a.w ? a.w[c] : 1.f; bias[e] = a.bias ? a.bias[c] : 0.f;
+        }
+        const int64_t xo = (int64_t)b * a.xb + t.v * V, po = (int64_t)b * a.db_ + t.v * V;
+        for (int r0 = first + t.r; r0 < end; r0 += 4 * t.step) {
+            float f[4][V], d[4][V];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = r0 + k * t.step;
+                if (r < end) { load_v<DT, V>(a.x, xo + (int64_t)r * a.xt, f[k]); load_v<DT, V>(a.dy, po + (int64_t)r * a.dt_, d[k]); }
+                else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[k][e] = d[k][e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = (f[k][e] - mu[e]) * rs[e], dz = d[k][e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
+                    s1[e] += dz; s2[e] += r0 + k * t.step < end ? dz * xh : 0.f;
+                }
+        }
+    }
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+        put<V>(red, t, a.C, which ? s2 : s1);
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
+            float v = 0.f;
+            for (int sl = 0; sl < t.step; ++sl) v += red[sl * a.C + c];
+            out[which * a.C + c] = v;
+        }
+    }
+}
+
+// (rows, 2, C) partial sums -> per-item sums (items of `per_item` rows; null: not wanted) and the totals db = sum of [0], dw = sum of [1].
+// 32 channels x 32 item slots to a workgroup; the slots are added in order.
+__global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ part, int items, int per_item, int C, float* __restrict__ item, float* __restrict__ dw,
+                                                    float* __restrict__ db) {
+    __shared__ float red[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), slot = threadIdx.x >> 5, which = blockIdx.y;
+    float total = 0.f;
+    if (c < C)
+        for (int b = slot; b < items; b += 32) {
+            float v = 0.f;
+            for (int k = 0; k < per_item; ++k) v += part[(((int64_t)b * per_item + k) * 2 + which) * C + c];
+            if (item) item[((int64_t)b * 2 + which) * C + c] = v;
+            total += v;
+        }
+    float* out = which ? dw : db;
+    red[slot][threadIdx.x & 31] = total;
+    __syncthreads();
+    if (out && threadIdx.x < 32 && c < C) {
+        float v = 0.f;
+        for (int k = 0; k < 32; ++k) v += red[k][threadIdx.x];
+        out[c] = v;
+    }
+}
+
+template <int DT, int V>
+__global__ __launch_bounds__(1024) void tile_dx_kernel(Args a) {
+    extern __shared__ float lds[];
+    float* m1 = lds;                       // means of w dz and w dz xh of each group
+    float* m2 = lds + a.G;
+    const Tile t(a.C, V);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.n);
+    const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, a.T);
+    const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
+    const float* item = a.item + (int64_t)b * 2 * a.C;
+    const float inv = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
+    for (int g0 = 0; g0 < a.G; g0 += per) {
+        const int g = g0 + threadIdx.x / run;
+        float v1 = 0.f, v2 = 0.f;
+        if (g < a.G)
+            for (int c = g * a.n + lane; c < (g + 1) * a.n; c += run) {
+                const float w = a.w ? a.w[c] : 1.f;
+                v1 += w * item[c]; v2 += w * item[a.C + c];
+            }
+        v1 = lanes_sum(v1, run); v2 = lanes_sum(v2, run);
+        if (g < a.G && lane == 0) { m1[g] = v1 * inv; m2[g] = v2 * inv; }
+    }
+    __syncthreads();
+    if (!t.on) return;
+    float mu[V], rs[V], w[V], bias[V], k1[V], k2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const int c = t.v * V + e, g = c / a.n;
+        mu[e] = a.mean[(int64_t)b * a.G + g]; rs[e] = a.rstd[(int64_t)b * a.G + g];
+        w[e] = a.w ? a.w[c] : 1.f; bias[e] = a.bias ? a.bias[c] : 0.f;
+        k1[e] = m1[g]; k2[e] = m2[g];
+    }
+    const int64_t xo = (int64_t)b * a.xb + t.v * V, po = (int64_t)b * a.db_ + t.v * V, oo = (int64_t)b * a.ob + t.v * V;
+    for (int r0 = first + t.r; r0 < end; r0 += 2 * t.step) {
+        float f[2][V], d[2][V];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int r = r0 + k * t.step;
+            if (r < end && r < len) { load_v<DT, V>(a.x, xo + (int64_t)r * a.xt, f[k]); load_v<DT, V>(a.dy, po + (int64_t)r * a.dt_, d[k]); }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int r = r0 + k * t.step;
+            if (r >= end) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (r < len) {
+                    const float xh = (f[k][e] - mu[e]) * rs[e], dz = d[k][e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
+                    f[k][e] = rs[e] * (w[e] * dz - k1[e] - xh * k2[e]);
+                } else f[k][e] = 0.f;
+            }
+            store_v<DT, V>(a.out, oo + (int64_t)r * a.ot, f[k]);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------- plan ----
+struct Plan {
+    int v;                                  // elements of a vector: 16 bytes, or one
+    bool slab; int nv; SlabPlan s; int slab_wgs;
+    int threads, rows_per_chunk, chunks;
+};
+
+int pow2_at_least(int64_t x) { int r = 1; while (r < x) r <<= 1; return r; }
+
+bool make_plan(const xva_group_norm_args* p, bool vec, Plan* out) {
+    Plan& q = *out;
+    const int wide = p->dtype == 0 ? 4 : 8, n = p->C / p->G;
+    q.v = vec && p->C % wide == 0 ? wide : 1;
+    // slab form: a (item, group) slab of whole vectors (of one value, where 16 bytes would straddle groups) within 64 lanes x 4 vectors
+    const int sv = n % q.v == 0 ? q.v : 1;
+    const int64_t vecs = (int64_t)p->T * (n / sv);
+    q.slab = vecs <= 256;
+    if (q.slab) {
+        q.v = sv;
+        q.nv = vecs <= 64 ? 1 : (vecs <= 128 ? 2 : 4);
+        q.s.lpg = pow2_at_least((vecs + q.nv - 1) / q.nv);
+        const int slots = 256 / q.s.lpg;
+        q.s.gpb = p->G < slots ? p->G : slots;
+        q.s.ipb = slots / q.s.gpb;
+        q.s.gy = (p->G + q.s.gpb - 1) / q.s.gpb;
+        // one workgroup for every `ipb` items up to eight to a CU; the backward's partial rows are as many
+        const int64_t want = (p->B + q.s.ipb - 1) / q.s.ipb;
+        int64_t most = 2048 / q.s.gy;
+        if (most < 64) most = 64;
+        q.slab_wgs = (int)(want < most ? want : most);
+        return true;
+    }
+    const int lc = p->C / q.v;
+    if (lc > 1024 || p->G > 2048) return false;        // (a row in one workgroup, its groups in the LDS)
+    q.threads = lc <= 256 ? 256 : (lc + 63) / 64 * 64;
+    const int step = q.threads / lc;
+    // chunks of whole register tiles: enough of them for four workgroups to a CU, at most 64 of an item (one lane each when they are joined)
+    const int tile = step * NR;
+    int64_t tiles = (p->T + tile - 1) / tile;
+    int64_t want = (1024 + p->B - 1) / p->B;
+    if (want > 64) want = 64;
+    if (want > tiles) want = tiles;
+    const int64_t each = (tiles + want - 1) / want;
+    q.rows_per_chunk = (int)(each * tile);
+    q.chunks = (int)((p->T + q.rows_per_chunk - 1) / q.rows_per_chunk);
+    return true;
+}
+
+bool aligned(const xva_group_norm_args* p, bool bwd) {
+    const int wide = p->dtype == 0 ? 4 : 8;
+    int64_t all = p->x_stride[0] | p->x_stride[1] | p->out_stride[0] | p->out_stride[1];
+    uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->out;
+    if (bwd) { all |= p->dy_stride[0] | p->dy_stride[1]; ptrs |= (uintptr_t)p->dy; }
+    return all % wide == 0 && ptrs % 16 == 0;
+}
+
+int check(const xva_group_norm_args* p, const char* who) {
+    XVA_CHECK_ARG(p, "%s: null argument", who);
+    XVA_CHECK_ARG(p->dtype >= 0 && p->dtype <= 2, "%s: dtype %d", who, p->dtype);
+    XVA_CHECK_ARG(p->B >= 0 && p->B < (1 << 30) && p->T >= 0 && p->C >= 1 && p->C <= 65536 && p->G >= 1 && p->C % p->G == 0, "%s: B %d T %d C %d in %d groups", who, p->B, p->T, p->C, p->G);
+    XVA_CHECK_ARG(p->act >= NONE && p->act <= GELU, "%s: activation %d", who, p->act);
+    XVA_CHECK_ARG(p->eps >= 0.f, "%s: eps %g", who, p->eps);
+    XVA_CHECK_ARG(p->B == 0 || p->T == 0 || (p->x && p->out && p->mean && p->rstd), "%s: null argument", who);
+    return XVA_OK;
+}
+
+Args args_of(const xva_group_norm_args* p, const Plan& q) {
+    Args a = {};
+    a.x = p->x; a.dy = p->dy; a.out = p->out; a.w = p->weight; a.bias = p->bias; a.lens = p->lens; a.mean = p->mean; a.rstd = p->rstd;
+    a.dw = p->dweight; a.db = p->dbias;
+    a.xb = p->x_stride[0]; a.xt = p->x_stride[1]; a.ob = p->out_stride[0]; a.ot = p->out_stride[1]; a.db_ = p->dy_stride[0]; a.dt_ = p->dy_stride[1];
+    a.B = p->B; a.T = p->T; a.C = p->C; a.G = p->G; a.n = p->C / p->G; a.act = p->act; a.eps = p->eps; a.slope = p->slope;
+    a.rows_per_chunk = q.rows_per_chunk; a.chunks = q.chunks;
+    return a;
+}
+
+int64_t workspace(const xva_group_norm_args* p, bool bwd) {
+    // (over both vector widths: which one runs depends on addresses and strides)
+    int64_t most = 0;
+    for (int vec = 0; vec < 2; ++vec) {
+        Plan q = {};
+        if (!make_plan(p, vec != 0, &q)) continue;
+        int64_t f;
+        if (q.slab) f = bwd ? (int64_t)q.slab_wgs * 2 * p->C : 0;
+        else f = bwd ? (int64_t)p->B * (q.chunks + 1) * 2 * p->C : (int64_t)p->B * q.chunks * 2 * p->G;
+        if (f > most) most = f;
+    }
+    return most * 4;
+}
+
+template <int DT, int V, bool BWD> int slab_launch(const Args& a, const Plan& q, hipStream_t st) {
+    const dim3 grid(q.slab_wgs, q.s.gy);
+    const size_t lds = BWD ? (size_t)256 * q.nv * 2 * V * 4 : 0;
+    if (q.nv == 1) slab_kernel<DT, V, 1, BWD><<<grid, 256, lds, st>>>(a, q.s);
+    else if (q.nv == 2) slab_kernel<DT, V, 2, BWD><<<grid, 256, lds, st>>>(a, q.s);
+    else slab_kernel<DT, V, 4, BWD><<<grid, 256, lds, st>>>(a, q.s);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+
+template <int DT, int V> int forward(Args& a, const Plan& q, hipStream_t st) {
+    if (q.slab) return slab_launch<DT, V, false>(a, q, st);
+    const dim3 grid((unsigned)(a.B * q.chunks));
+    const int step = q.threads / (a.C / V);
+    tile_stats_kernel<DT, V><<<grid, q.threads, ((size_t)step * a.C + 3 * a.G) * 4, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    tile_apply_kernel<DT, V><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+
+int join(const Args& a, int items, int per_item, hipStream_t st) {
+    join_kernel<<<dim3((a.C + 31) / 32, 2), 1024, 0, st>>>(a.part, items, per_item, a.C, a.item, a.dw, a.db);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+
+template <int DT, int V> int backward(Args& a, const Plan& q, hipStream_t st) {
+    if (q.slab) {
+        XVA_TRY((slab_launch<DT, V, true>(a, q, st)));
+        return a.dw || a.db ? join(a, q.slab_wgs, 1, st) : XVA_OK;
+    }
+    const dim3 grid((unsigned)(a.B * q.chunks));
+    const int step = q.threads / (a.C / V);
+    a.item = a.part + (int64_t)a.B * q.chunks * 2 * a.C;
+    tile_dsum_kernel<DT, V><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    XVA_TRY(join(a, a.B, q.chunks, st));
+    tile_dx_kernel<DT, V><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    XVA_LAUNCH_CHECK();
+    return XVA_OK;
+}
+
+int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void* stream, const char* who) {
+    XVA_TRY(check(p, who));
+    XVA_CHECK_ARG(!bwd || p->dy || p->B == 0 || p->T == 0, "%s: null gradient", who);
+    hipStream_t st = (hipStream_t)stream;
+    Plan q = {};
+    XVA_CHECK_ARG(make_plan(p, aligned(p, bwd), &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
+    XVA_CHECK_ARG(q.slab || (int64_t)p->B * q.chunks < (1ll << 31), "%s: %d items of %d rows", who, p->B, p->T);
+    if (ws_bytes < workspace(p, bwd)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)workspace(p, bwd)); return XVA_ERR_WS; }
+    if (p->B == 0 || p->T == 0) {
+        if (bwd) {
+            if (p->dweight) { void* d[1] = {p->dweight}; const int64_t n[1] = {(int64_t)p->C * 4}; XVA_TRY(xva_zero_spans(d, n, 1, stream)); }
+            if (p->dbias) { void* d[1] = {p->dbias}; const int64_t n[1] = {(int64_t)p->C * 4}; XVA_TRY(xva_zero_spans(d, n, 1, stream)); }
+        }
+        return XVA_OK;
+    }
+    Args a = args_of(p, q);
+    a.part = (float*)ws;
+    const bool v1 = q.v == 1;
+#define GN(DT, V) (bwd ? backward<DT, V>(a, q, st) : forward<DT, V>(a, q, st))
+    if (p->dtype == 0) return v1 ? GN(0, 1) : GN(0, 4);
+    if (p->dtype == 1) return v1 ? GN(1, 1) : GN(1, 8);
+    return v1 ? GN(2, 1) : GN(2, 8);
+#undef GN
+}
+}   // namespace
+
+extern "C" int64_t xva_group_norm_workspace_bytes(const xva_group_norm_args* p, int backward_pass) {
+    if (!p || p->G < 1 || p->C < 1 || p->C % p->G || p->B < 0 || p->T < 0) return -1;
+    return workspace(p, backward_pass != 0);
+}
+extern "C" int xva_group_norm_act_fwd(const xva_group_norm_args* p, void* ws, int64_t ws_bytes, void* stream) {
+    return run(p, false, ws, ws_bytes, stream, "xva_group_norm_act_fwd");
+}
+extern "C" int xva_group_norm_act_bwd(const xva_group_norm_args* p, void* ws, int64_t ws_bytes, void* stream) {
+    return run(p, true, ws, ws_bytes, stream, "xva_group_norm_act_bwd");
+}
