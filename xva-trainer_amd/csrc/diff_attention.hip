@@ -16,7 +16,7 @@
 // Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands (the accumulators are fp32; sums, maxima and logsumexp stay fp32).
 //
 // Tiles: 64 rows x 64 columns of 16-bit values (attn_tile.h).  d <= 32: one image holds both maps' 32 columns side by side; d <= 64: one image for each map.
-// V and dO (2 d wide): one or two images.  Columns behind d read a zero page, rows behind the last live one read that one with P = 0.
+// V and dO (2 d wide): one or two images.  Rows behind the last live one read that one, with P = 0.
 #include "attn_tile.h"
 #include "../../include/xva_hip.h"
 
@@ -36,7 +36,9 @@ struct Args {
     int B, Tq, Tk, H, Hk, share, d, causal;
     float scale, c;                               // c = scale log2 e
 };
-// contiguous results: out-of-line maps (2, B, Tq, H, 2 d), dq (B, Tq, H, 2, d), dk (B, Tk, Hk, 2, d), dv (B, Tk, Hk, 2 d); lse, D (2, B, H, Tq), base 2
+// contiguous results: out-of-line maps (2, B, Tq, H, 2 d), dq (B, Tq, H, 2, d), dk (B, Tk, Hk, 2, d), dv (B, Tk, Hk, 2 d)
+// lse (2, B, H, Tq): minus the row's logarithm of sums, in units of unscaled scores (-inf: the row sees nothing), so P = exp2(c (S + lse)); D (2, B, H, Tq): -D_1
+// and D_1 - D_2.  Both are what dkv's matrix products start from.
 
 template <int D16> struct Shape {
     static constexpr int NI = D16 <= 2 ? 1 : 2;   // 64-column images of a q / k tile, and of a v / dO tile
@@ -48,38 +50,48 @@ template <int D16> struct Shape {
 
 __device__ __forceinline__ int len_of(const int32_t* l, int b, int T) { return l ? min(max(l[b], 0), T) : T; }
 
-// column of chunk c (8 columns) of image im of a q / k tile -> (map, first d index)
-template <int NI> __device__ __forceinline__ void qk_chunk(int im, int c, int& map, int& d0) {
-    if constexpr (NI == 2) { map = im; d0 = c * 8; } else { map = c >> 2; d0 = (c & 3) * 8; }
-}
-
-// DMA of the NI images of a q / k tile: rows row0 .. row0 + 63, clamped to rmax (>= 0); 4 waves, 2 instructions an image each
-template <int NI>
-__device__ __forceinline__ void dma_qk(const uint16_t* base, int64_t ld, int64_t map_stride, int d, int row0, int rmax, XVA_LDS uint8_t* tile, int lane, int wave) {
+// Where this lane's two 16-byte pieces of an image come from: rows r and r + 32 of the tile, one column (the swizzle repeats every 8 rows).  Columns behind the
+// width read the row's first ones: they meet zeros in the other operand, or results that nobody stores, and a row that is not finite is lost through its
+// live columns already.
+template <int NI> struct Src {
+    int r, qk[NI], v[NI];                         // row, and the column's element offset: a q / k tile's with the map's
+    __device__ __forceinline__ Src(int lane, int wave, int d, int64_t map_stride) {
+        r = wave * 8 + (lane >> 3);
+        const int p = lane & 7, c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
 #pragma unroll
-    for (int im = 0; im < NI; ++im)
+        for (int im = 0; im < NI; ++im) {
+            const int map = NI == 2 ? im : c >> 2, d0 = (NI == 2 ? c : c & 3) * 8, e0 = im * 64 + c * 8;
+            qk[im] = map * (int)map_stride + (d0 < d ? d0 : 0);
+            v[im] = e0 < 2 * d ? e0 : 0;
+        }
+    }
+    // rows row0 .. row0 + 63, clamped to rmax (>= 0)
+    __device__ __forceinline__ void fetch(const uint16_t* base, int64_t ld, const int (&col)[NI], int row0, int rmax, XVA_LDS uint8_t* tile, int wave) const {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            const int Q = q * 4 + wave, r = Q * 8 + (lane >> 3), p = lane & 7;
-            const int c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
-            int map, d0;
-            qk_chunk<NI>(im, c, map, d0);
-            const uint16_t* src = d0 < d ? base + (int64_t)min(row0 + r, rmax) * ld + map * map_stride + d0 : reinterpret_cast<const uint16_t*>(g_zero_page);
-            __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(tile + im * TILE + Q * 1024), 16, 0, 0);
-        }
-}
-template <int NI>
-__device__ __forceinline__ void dma_v(const uint16_t* base, int64_t ld, int d, int row0, int rmax, XVA_LDS uint8_t* tile, int lane, int wave) {
+            const uint16_t* row = base + (int64_t)min(row0 + q * 32 + r, rmax) * ld;
 #pragma unroll
-    for (int im = 0; im < NI; ++im)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int Q = q * 4 + wave, r = Q * 8 + (lane >> 3), p = lane & 7;
-            const int c = im * 64 + (((((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1)) * 8);
-            const uint16_t* src = c < 2 * d ? base + (int64_t)min(row0 + r, rmax) * ld + c : reinterpret_cast<const uint16_t*>(g_zero_page);
-            __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(tile + im * TILE + Q * 1024), 16, 0, 0);
+            for (int im = 0; im < NI; ++im)
+                __builtin_amdgcn_global_load_lds((const XVA_GLB void*)(row + col[im]), (XVA_LDS void*)(tile + im * TILE + (q * 4 + wave) * 1024), 16, 0, 0);
         }
-}
+    }
+};
+// `lane`, but unknown to the compiler: what is computed from it inside a loop is not kept in registers across the loop (where the accumulators leave none)
+__device__ __forceinline__ int again(int lane) { asm volatile("" : "+v"(lane)); return lane; }
+// LDS offsets of this lane's fragments.  A fragment's other 32-column half and its other 16-column tiles are an XOR away (the swizzle XORs windows, attn_tile.h).
+struct Lane {
+    uint32_t kc, tr;
+    __device__ __forceinline__ Lane(int lane, uint32_t at) { Frag fr; fr.init(lane); kc = fr.kc[0] + at; tr = fr.tr[0] + at; }
+    // as Frag's, of image `im` of a buffer: rows it * 16 .. + 15 / columns dt * 16 .. + 15 of rows 32 t ..
+    __device__ __forceinline__ bf16x8 rows(const XVA_LDS uint8_t* smem, int im, int it, int kh) const {
+        return *reinterpret_cast<const XVA_LDS bf16x8*>(smem + (kc ^ (kh * 64)) + (im * TILE + it * 2048));
+    }
+    __device__ __forceinline__ bf16x8 cols(const XVA_LDS uint8_t* smem, int im, int dt, int t) const {
+        const XVA_LDS uint8_t* a = smem + (tr ^ (dt * 32)) + (im * TILE + t * 4096);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((XVA_LDS s16x4*)a), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((XVA_LDS s16x4*)(a + 2048));
+        return __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
 // 8 elements at column d0 of a row as an MFMA operand, zero behind `width`
 __device__ __forceinline__ bf16x8 ld_edge(const uint16_t* row, int d0, int width) {
     const uint4 z = {0, 0, 0, 0};
@@ -91,8 +103,18 @@ template <int NI> __device__ __forceinline__ int qk_half(int m, int kh) { return
 // image and 16-column tile of d tile dt of map m
 template <int NI> __device__ __forceinline__ int qk_tile(int m, int dt) { return NI == 2 ? dt : m * 2 + dt; }
 
+// Tiles 0 .. n - 1 with their two LDS buffers by turns.  The buffers are two arrays and the loop is written out for both, so that the compiler sees that the
+// reads of one tile do not touch the bytes that the next tile's loads are bringing in, and does not wait for those before the reads.
+#define XVA_TWO_BUFFERS(n, tile)                                                          \
+    for (int two = 0; two < (n); two += 2) {                                              \
+        tile(two, (const XVA_LDS uint8_t*)even, (XVA_LDS uint8_t*)odd);                   \
+        if (two + 1 < (n)) tile(two + 1, (const XVA_LDS uint8_t*)odd, (XVA_LDS uint8_t*)even); \
+    }
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define MFMA(x, y, z) mma16<F16>(x, y, z)
 #define ZERO4 ((f32x4){0.f, 0.f, 0.f, 0.f})
+// p[i] of an input that is the same in every lane, by a scalar load (a vector load would be waited for together with the tiles in flight)
+__device__ __forceinline__ float uniform(const float* p, int i) { return reinterpret_cast<const __attribute__((address_space(4))) float*>((uintptr_t)p)[i]; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ================================================================================ forward ====
@@ -100,8 +122,7 @@ template <int D16, bool F16, bool TRAIN>
 __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE];       // {K V} x 2
-    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
+    __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];       // {K V} of the even and of the odd tiles (see XVA_TWO_BUFFERS)
     // the last query blocks see most keys under `causal`: they start first
     const int nqb = gridDim.x / (a.B * a.H);
     const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
@@ -119,13 +140,13 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
     const int whole_keys = seen_by(wrow);
     const int tiles = (wg_keys + 63) / 64;
-    Frag fr; fr.init(lane);
+    Lane fr(lane, 0);
     bf16x8 qf[2][2][S::KH];
-    int limit[2];
+    // keys that row tile rt's row of this lane sees
+    auto limit = [&](int rt) { const int row = wrow + rt * 16 + (again(lane) & 15); return row < ql ? seen_by(row) : 0; };
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
-        limit[rt] = row < ql ? seen_by(row) : 0;
         const uint16_t* qr = qp + (int64_t)min(row, max(ql - 1, 0)) * a.qt;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -143,109 +164,104 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
             for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] = ZERO4;
         }
     if (tiles) {
-        dma_qk<NI>(kp, a.kt, a.km, a.d, 0, kl - 1, smem, lane, wave);
-        dma_v<NI>(vp, a.vt, a.d, 0, kl - 1, smem + NI * TILE, lane, wave);
+        const Src<NI> src(lane, wave, a.d, a.km);
+        src.fetch(kp, a.kt, src.qk, 0, kl - 1, (XVA_LDS uint8_t*)even, wave);
+        src.fetch(vp, a.vt, src.v, 0, kl - 1, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
-    for (int jb = 0; jb < tiles; ++jb) {
-        const XVA_LDS uint8_t* Kt = smem + (jb & 1) * 2 * NI * TILE;
-        const XVA_LDS uint8_t* Vt = Kt + NI * TILE;
+    auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         if (jb + 1 < tiles) {
-            XVA_LDS uint8_t* next = smem + ((jb & 1) ^ 1) * 2 * NI * TILE;
-            dma_qk<NI>(kp, a.kt, a.km, a.d, (jb + 1) * 64, kl - 1, next, lane, wave);
-            dma_v<NI>(vp, a.vt, a.d, (jb + 1) * 64, kl - 1, next + NI * TILE, lane, wave);
+            const Src<NI> src(again(lane), wave, a.d, a.km);
+            src.fetch(kp, a.kt, src.qk, (jb + 1) * 64, kl - 1, next, wave);
+            src.fetch(vp, a.vt, src.v, (jb + 1) * 64, kl - 1, next + NI * TILE, wave);
         }
         if (jb * 64 < wave_keys) {
             const bool whole = (jb + 1) * 64 <= whole_keys;
-            bf16x8 pf[2][2][2];
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                f32x4 s[2][4];
+            for (int t = 0; t < 2; ++t) {                     // 32 keys at a time
+                bf16x8 pf[2][2];
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) {
-                    s[0][kt] = ZERO4; s[1][kt] = ZERO4;
+                for (int m = 0; m < 2; ++m) {
+                    f32x4 s[2][2];
 #pragma unroll
-                    for (int kh = 0; kh < S::KH; ++kh) {
-                        const bf16x8 kf = fr.read_kc(Kt + qk_image<NI>(m) * TILE, kt, qk_half<NI>(m, kh));
-                        s[0][kt] = MFMA(kf, qf[m][0][kh], s[0][kt]);           // [key g * 4 + r][row lane & 15]
-                        s[1][kt] = MFMA(kf, qf[m][1][kh], s[1][kt]);
+                    for (int u = 0; u < 2; ++u) {
+                        s[0][u] = ZERO4; s[1][u] = ZERO4;
+#pragma unroll
+                        for (int kh = 0; kh < S::KH; ++kh) {
+                            const bf16x8 kf = fr.rows(smem, qk_image<NI>(m), 2 * t + u, qk_half<NI>(m, kh));
+                            s[0][u] = MFMA(kf, qf[m][0][kh], s[0][u]);         // [key g * 4 + r][row lane & 15]
+                            s[1][u] = MFMA(kf, qf[m][1][kh], s[1][u]);
+                        }
                     }
-                }
-                if (!whole) {
+                    if (!whole) {
+#pragma unroll
+                        for (int rt = 0; rt < 2; ++rt) {
+                            const int left = limit(rt) - (jb * 64 + t * 32 + g * 4);
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) s[rt][u][r] = u * 16 + r < left ? s[rt][u][r] : -INFINITY;
+                        }
+                    }
+                    float top[2];                             // of this lane's keys
 #pragma unroll
                     for (int rt = 0; rt < 2; ++rt)
+                        top[rt] = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
+                                        fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+                    // (a first key: the difference is +inf; nothing seen yet: it is NaN)
+                    if (__any((top[0] - mx[m][0]) * a.c > 8.f || (top[1] - mx[m][1]) * a.c > 8.f)) {
 #pragma unroll
-                        for (int kt = 0; kt < 4; ++kt)
+                        for (int rt = 0; rt < 2; ++rt) {
+                            float now = fmaxf(top[rt], __shfl_xor(top[rt], 16, 64));
+                            now = fmaxf(fmaxf(now, __shfl_xor(now, 32, 64)), mx[m][rt]);
+                            const float alpha = mx[m][rt] == now ? 1.f : exp2_((mx[m][rt] - now) * a.c);
+                            mx[m][rt] = now;
+                            sum[m][rt] *= alpha;
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (jb * 64 + kt * 16 + g * 4 + r >= limit[rt]) s[rt][kt][r] = -INFINITY;
-                }
-                float top[2];
-#pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    float t = -INFINITY;
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) t = fmaxf(t, s[rt][kt][r]);
-                    t = fmaxf(t, __shfl_xor(t, 16, 64));
-                    top[rt] = fmaxf(t, __shfl_xor(t, 32, 64));
-                }
-                // (top > mx = -inf also where a first key shows up: the difference is +inf)
-                const bool grew = (top[0] - mx[m][0]) * a.c > 8.f || (top[1] - mx[m][1]) * a.c > 8.f;
-                if (__any(grew)) {
+                            for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] *= alpha;
+                        }
+                    }
 #pragma unroll
                     for (int rt = 0; rt < 2; ++rt) {
-                        const float now = fmaxf(mx[m][rt], top[rt]);
-                        const float alpha = mx[m][rt] == now ? 1.f : exp2_((mx[m][rt] - now) * a.c);
-                        mx[m][rt] = now;
-                        sum[m][rt] *= alpha;
+                        const float base = mx[m][rt] == -INFINITY ? 0.f : mx[m][rt] * a.c;
 #pragma unroll
-                        for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] *= alpha;
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float p = exp2_(s[rt][u][r] * a.c - base);
+                                sum[m][rt] += p;
+                                s[rt][u][r] = p;
+                            }
+                        pf[m][rt] = pack_rows<F16>(s[rt][0], s[rt][1]);
                     }
                 }
 #pragma unroll
-                for (int rt = 0; rt < 2; ++rt) {
-                    const float base = mx[m][rt] == -INFINITY ? 0.f : mx[m][rt] * a.c;
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float p = exp2_(s[rt][kt][r] * a.c - base);
-                            sum[m][rt] += p;
-                            s[rt][kt][r] = p;
-                        }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) pf[m][rt][t] = pack_rows<F16>(s[rt][2 * t], s[rt][2 * t + 1]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
                 for (int dt = 0; dt < S::VT; ++dt) {
-                    const bf16x8 vf = fr.read_tr(Vt + (dt >> 2) * TILE, dt & 3, t);
+                    const bf16x8 vf = fr.cols(smem, NI + (dt >> 2), dt & 3, t);
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int rt = 0; rt < 2; ++rt) o[m][rt][dt] = MFMA(vf, pf[m][rt][t], o[m][rt][dt]);     // [column g * 4 + r][row lane & 15]
+                        for (int rt = 0; rt < 2; ++rt) o[m][rt][dt] = MFMA(vf, pf[m][rt], o[m][rt][dt]);        // [column g * 4 + r][row lane & 15]
                 }
+            }
         }
         __syncthreads();
-    }
-    const float lam = a.lam[h];
+    };
+    XVA_TWO_BUFFERS(tiles, tile)
+    const float lam = uniform(a.lam, h);
     const int w = 2 * a.d;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
+        const bool seen = limit(rt) > 0;
         float inv[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             float l = sum[m][rt];
             l += __shfl_xor(l, 16, 64);
             l += __shfl_xor(l, 32, 64);
-            const bool seen = limit[rt] > 0;
             inv[m] = seen ? 1.f / l : 0.f;
-            if (TRAIN && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? mx[m][rt] * a.c + __log2f(l) : INFINITY;
+            if (TRAIN && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m][rt] + __log2f(l) / a.c) : -INFINITY;
         }
         if (row >= a.Tq) continue;
         uint16_t* out = a.out + b * a.ob + row * a.ot + h * a.oh;
@@ -258,8 +274,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
             float u[4], v[4], r[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                u[e] = limit[rt] > 0 ? o[0][rt][dt][e] * inv[0] : 0.f;
-                v[e] = limit[rt] > 0 ? o[1][rt][dt][e] * inv[1] : 0.f;
+                u[e] = seen ? o[0][rt][dt][e] * inv[0] : 0.f;
+                v[e] = seen ? o[1][rt][dt][e] * inv[1] : 0.f;
                 r[e] = u[e] - lam * v[e];
             }
             *reinterpret_cast<uint2*>(out + col) = make_uint2(pack2<F16>(r[0], r[1]), pack2<F16>(r[2], r[3]));
@@ -299,24 +315,28 @@ __global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
     for (int m = 0; m < 2; ++m) {
         s[m] += __shfl_xor(s[m], 1, 64); s[m] += __shfl_xor(s[m], 2, 64); s[m] += __shfl_xor(s[m], 4, 64); s[m] += __shfl_xor(s[m], 8, 64);
     }
-    if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = s[threadIdx.x & 1];
+    if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
 }
 
-// dK, dV of 128 keys of a key head, 32 to a wave, over the query heads that share it and their 64-query tiles
+// dK, dV of 64 keys of a key head over the query heads that share it and their 64-query tiles.  Waves: two halves of the keys x two halves of a tile's
+// queries; the queries' halves are added at the end through LDS.  (128 keys to a workgroup, 32 to a wave over all rows: half as many workgroups, which
+// leaves long causal sequences waiting for the first keys' ones.)
 template <int D16, bool F16>
 __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE + 2 * 1024];     // {Q dO} x 2 | {lse1 lse2 D1 D2} x 2
-    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
-    XVA_LDS uint8_t* stat = smem + 4 * NI * TILE;
+    // (the widest heads' accumulators leave too few registers for all of V's fragments: a spilled one would be waited for together with the tiles in flight)
+    constexpr int AWAY = D16 == 4 ? 3 : 0;                                                    // V fragments of the second key tile kept in LDS
+    constexpr int STAT = 2 * NI * TILE;                                                        // {Q dO | lse1 lse2 D1 D2} of the even and of the odd tiles
+    __shared__ __attribute__((aligned(1024))) uint8_t even[STAT + 1024], odd[STAT + 1024];
+    __shared__ __attribute__((aligned(16))) uint8_t away_raw[AWAY ? AWAY * 4096 : 16];
     const int kblk = blockIdx.x / (a.B * a.Hk), bh = blockIdx.x % (a.B * a.Hk);                // (the first keys are seen by most queries: they start first)
-    const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 128;
+    const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, i = lane & 15;
+    const int g = lane >> 4, i = lane & 15, t = wave >> 1;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql;
-    const int wkey = k0 + wave * 32, w = 2 * a.d;
-    Frag fr; fr.init(lane);
+    const int wkey = k0 + (wave & 1) * 32, w = 2 * a.d;
+    Lane fr(lane, t * 4096);
     // queries that see a key of the workgroup: from `first` on
     const int first = a.causal ? max(k0 - off, 0) : 0;
     const bool any = k0 < kl && first < ql;
@@ -332,6 +352,10 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
 #pragma unroll
         for (int kh = 0; kh < S::VH; ++kh) vf[kt][kh] = ld_edge(a.v + b * a.vb + hk * a.vh + key * a.vt, kh * 32 + g * 8, any ? w : 0);
     }
+    XVA_LDS bf16x8* away = (XVA_LDS bf16x8*)away_raw + wave * AWAY * 64 + lane;
+#pragma unroll
+    for (int e = 0; e < AWAY; ++e) away[e * 64] = vf[1][S::VH - 1 - e];
+    auto v_of = [&](int kt, int kh) { return kt == 1 && kh >= S::VH - AWAY ? away[(S::VH - 1 - kh) * 64] : vf[kt][kh]; };
     f32x4 dk[2][2][S::DT], dv[2][S::VT];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -342,111 +366,124 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
 #pragma unroll
         for (int dt = 0; dt < S::VT; ++dt) dv[kt][dt] = ZERO4;
     }
-    auto fetch = [&](int it, int buf) {
-        const int hs = it / per_head, h = hk * a.share + hs, row0 = (t0 + it - hs * per_head) * 64;
-        XVA_LDS uint8_t* to = smem + buf * 2 * NI * TILE;
-        dma_qk<NI>(a.q + b * a.qb + h * a.qh, a.qt, a.qm, a.d, row0, ql - 1, to, lane, wave);
-        dma_v<NI>(a.dout + b * a.gb + h * a.gh, a.gt, a.d, row0, ql - 1, to + NI * TILE, lane, wave);
-        const float* src = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + min(row0 + lane, ql - 1);
-        __builtin_amdgcn_global_load_lds((const XVA_GLB void*)src, (XVA_LDS void*)(stat + buf * 1024 + wave * 256), 4, 0, 0);
+    auto fetch = [&](int hs, int row0, XVA_LDS uint8_t* to) {
+        const int h = hk * a.share + hs, lane_ = again(lane);
+        const Src<NI> src(lane_, wave, a.d, a.qm);
+        src.fetch(a.q + b * a.qb + h * a.qh, a.qt, src.qk, row0, ql - 1, to, wave);
+        src.fetch(a.dout + b * a.gb + h * a.gh, a.gt, src.v, row0, ql - 1, to + NI * TILE, wave);
+        const float* from = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + min(row0 + lane_, ql - 1);
+        __builtin_amdgcn_global_load_lds((const XVA_GLB void*)from, (XVA_LDS void*)(to + STAT + wave * 256), 4, 0, 0);
     };
-    if (total) fetch(0, 0);
+    if (total) fetch(0, t0 * 64, (XVA_LDS uint8_t*)even);
     __syncthreads();
-    for (int it = 0; it < total; ++it) {
-        const int hs = it / per_head, row0 = (t0 + it - hs * per_head) * 64;
-        const float lam = a.lam[hk * a.share + hs];
-        if (it + 1 < total) fetch(it + 1, (it & 1) ^ 1);
-        const XVA_LDS uint8_t* Qt = smem + (it & 1) * 2 * NI * TILE;
-        const XVA_LDS uint8_t* Ot = Qt + NI * TILE;
-        const XVA_LDS uint8_t* st = stat + (it & 1) * 1024;
-        // every row of the tile sees every key of the wave
-        const bool whole = row0 + 64 <= ql && wkey + 32 <= kl && (!a.causal || wkey + 31 <= row0 + off);
-        const bool none = wkey >= kl || (a.causal && wkey > row0 + 63 + off);
+    int hs = 0, qtile = t0;
+    auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
+        const int row0 = qtile * 64;
+        const float lam = uniform(a.lam, hk * a.share + hs);
+        if (++qtile == t0 + per_head) { qtile = t0; ++hs; }
+        if (it + 1 < total) fetch(hs, qtile * 64, next);
+        const int wrow = row0 + t * 32;                       // this wave's 32 rows
+        const bool whole = wrow + 32 <= ql && wkey + 32 <= kl && (!a.causal || wkey + 31 <= wrow + off);      // every row sees every key
+        const bool none = wkey >= kl || wrow >= ql || (a.causal && wkey > wrow + 31 + off);
         if (!none) {
+            u32x4 pk[3][2];                                   // P_1 - lam P_2, dS_1, dS_2 of each key tile, 32 rows in the permuted order
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x4 s[2][2][2], dp[2][2];                 // [map][row tile][key tile], [row g * 4 + r][key lane & 15]
+            for (int u = 0; u < 2; ++u) {
+                // -D_1 under dP, lse under the scores
+                const XVA_LDS uint8_t* at = smem + STAT + t * 128 + g * 16 + u * 64;
+                const f32x4 nD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 512);
+                f32x4 s[2][2], dp[2];                         // [map][key tile], [row g * 4 + r][key lane & 15]
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int rt = 2 * t + u;
+                for (int kh = 0; kh < S::VH; ++kh) {
+                    const bf16x8 of = fr.rows(smem, NI + (kh >> 1), u, kh & 1);
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) { s[0][u][kt] = ZERO4; s[1][u][kt] = ZERO4; dp[u][kt] = ZERO4; }
+                    for (int kt = 0; kt < 2; ++kt) dp[kt] = MFMA(of, v_of(kt, kh), kh ? dp[kt] : nD);
+                }
 #pragma unroll
-                    for (int m = 0; m < 2; ++m)
+                for (int m = 0; m < 2; ++m) {
+                    const f32x4 nL = *reinterpret_cast<const XVA_LDS f32x4*>(at + m * 256);
 #pragma unroll
-                        for (int kh = 0; kh < S::KH; ++kh) {
-                            const bf16x8 qf = fr.read_kc(Qt + qk_image<NI>(m) * TILE, rt, qk_half<NI>(m, kh));
+                    for (int kh = 0; kh < S::KH; ++kh) {
+                        const bf16x8 qf = fr.rows(smem, qk_image<NI>(m), u, qk_half<NI>(m, kh));
 #pragma unroll
-                            for (int kt = 0; kt < 2; ++kt) s[m][u][kt] = MFMA(qf, kf[m][kt][kh], s[m][u][kt]);
-                        }
-#pragma unroll
-                    for (int kh = 0; kh < S::VH; ++kh) {
-                        const bf16x8 of = fr.read_kc(Ot + (kh >> 1) * TILE, rt, kh & 1);
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) dp[u][kt] = MFMA(of, vf[kt][kh], dp[u][kt]);
+                        for (int kt = 0; kt < 2; ++kt) s[m][kt] = MFMA(qf, kf[m][kt][kh], kh ? s[m][kt] : nL);
                     }
                 }
-                bf16x8 pf[2], df[2][2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int rt = 2 * t + u;
-                    const XVA_LDS uint8_t* at = st + (rt * 16 + g * 4) * 4;
-                    const f32x4 L1 = *reinterpret_cast<const XVA_LDS f32x4*>(at), L2 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 256);
-                    const f32x4 D1 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 512), D2 = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768);
+                if (!whole) {
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float p1 = exp2_(s[0][u][kt][r] * a.c - L1[r]), p2 = exp2_(s[1][u][kt][r] * a.c - L2[r]);
-                            if (!whole) {
-                                const int row = row0 + rt * 16 + g * 4 + r, key = wkey + kt * 16 + i;
-                                const bool ok = row < ql && key < kl && (!a.causal || key <= row + off);
-                                p1 = ok ? p1 : 0.f; p2 = ok ? p2 : 0.f;
-                            }
-                            p2 *= -lam;
-                            const float x = dp[u][kt][r];
-                            s[0][u][kt][r] = p1 * (x - D1[r]);
-                            s[1][u][kt][r] = p2 * (x - D2[r]);
-                            dp[u][kt][r] = p1 + p2;
+                            const int row = wrow + u * 16 + g * 4 + r, key = wkey + kt * 16 + i;
+                            const bool ok = (row < ql) & (key < kl) & (!a.causal | (key <= row + off));
+                            s[0][kt][r] = ok ? s[0][kt][r] : -INFINITY;
+                            s[1][kt][r] = ok ? s[1][kt][r] : -INFINITY;
                         }
                 }
+                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    pf[kt] = pack_rows<F16>(dp[0][kt], dp[1][kt]);
-                    df[0][kt] = pack_rows<F16>(s[0][0][kt], s[0][1][kt]);
-                    df[1][kt] = pack_rows<F16>(s[1][0][kt], s[1][1][kt]);
-                }
+                for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int dt = 0; dt < S::VT; ++dt) {
-                    const bf16x8 of = fr.read_tr(Ot + (dt >> 2) * TILE, dt & 3, t);
-#pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) dv[kt][dt] = MFMA(of, pf[kt], dv[kt][dt]);                  // [column g * 4 + r][key lane & 15]
-                }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int dt = 0; dt < S::DT; ++dt) {
-                        const bf16x8 qf = fr.read_tr(Qt + qk_image<NI>(m) * TILE, qk_tile<NI>(m, dt), t);
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt) dk[m][kt][dt] = MFMA(qf, df[m][kt], dk[m][kt][dt]);
+                    for (int r = 0; r < 4; ++r) {
+                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = -lam * exp2_(s[1][kt][r] * a.c), x = dp[kt][r];
+                        s[0][kt][r] = p1 * x;
+                        s[1][kt][r] = p2 * (x + dD[r]);
+                        dp[kt][r] = p1 + p2;
                     }
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        pk[0][kt][2 * u + e] = pack2<F16>(dp[kt][2 * e], dp[kt][2 * e + 1]);
+                        pk[1][kt][2 * u + e] = pack2<F16>(s[0][kt][2 * e], s[0][kt][2 * e + 1]);
+                        pk[2][kt][2 * u + e] = pack2<F16>(s[1][kt][2 * e], s[1][kt][2 * e + 1]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);            // (16 rows at a time: registers)
             }
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt) {
+                const bf16x8 of = fr.cols(smem, NI + (dt >> 2), dt & 3, 0);
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) dv[kt][dt] = MFMA(of, __builtin_bit_cast(bf16x8, pk[0][kt]), dv[kt][dt]);                  // [column g * 4 + r][key lane & 15]
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int dt = 0; dt < S::DT; ++dt) {
+                    const bf16x8 qf = fr.cols(smem, qk_image<NI>(m), qk_tile<NI>(m, dt), 0);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) dk[m][kt][dt] = MFMA(qf, __builtin_bit_cast(bf16x8, pk[1 + m][kt]), dk[m][kt][dt]);
+                }
         }
         __syncthreads();
-    }
+    };
+    XVA_TWO_BUFFERS(total, tile)
+    // the second half of the queries hands its sums over: 16 bytes a lane and accumulator
+    XVA_LDS f32x4* xch = (XVA_LDS f32x4*)((wave & 1) ? odd : even) + lane;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
+        if (t == 1) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int dt = 0; dt < S::DT; ++dt) xch[(m * S::DT + dt) * 64] = dk[m][kt][dt];
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt) xch[(2 * S::DT + dt) * 64] = dv[kt][dt];
+        }
+        __syncthreads();
         const int key = wkey + kt * 16 + i;
-        if (key >= a.Tk) continue;
-        const int64_t row = ((int64_t)b * a.Tk + key) * a.Hk + hk;
+        if (t == 0 && key < a.Tk) {
+            const int64_t row = ((int64_t)b * a.Tk + key) * a.Hk + hk;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int dt = 0; dt < S::DT; ++dt)
-                if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + g * 4, dk[m][kt][dt], a.scale);
+                for (int dt = 0; dt < S::DT; ++dt)
+                    if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + g * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale);
 #pragma unroll
-        for (int dt = 0; dt < S::VT; ++dt)
-            if (dt * 16 + g * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + g * 4, dv[kt][dt], 1.f);
+            for (int dt = 0; dt < S::VT; ++dt)
+                if (dt * 16 + g * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + g * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], 1.f);
+        }
+        __syncthreads();
     }
 }
 
@@ -455,8 +492,7 @@ template <int D16, bool F16>
 __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem_raw[4 * NI * TILE];
-    XVA_LDS uint8_t* smem = (XVA_LDS uint8_t*)smem_raw;
+    __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];
     const int nqb = gridDim.x / (a.B * a.H);
     const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
     const int h = bh % a.H, b = bh / a.H, q0 = qblk * 128;
@@ -471,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
     const int whole_keys = seen_by(wrow);
     const int tiles = (wg_keys + 63) / 64;
-    Frag fr; fr.init(lane);
+    Lane fr(lane, 0);
     bf16x8 qf[2][2][S::KH], of[2][S::VH];
     int limit[2];
     float L[2][2], Dr[2][2];
@@ -484,8 +520,10 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
 #pragma unroll
             for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = ld_edge(a.q + b * a.qb + h * a.qh + m * a.qm + safe * a.qt, kh * 32 + g * 8, tiles ? a.d : 0);
             const int64_t at = (((int64_t)m * a.B + b) * a.H + h) * a.Tq + safe;
-            L[m][rt] = a.lse[at]; Dr[m][rt] = a.D[at];
+            L[m][rt] = -a.lse[at] * a.c; Dr[m][rt] = a.D[at];
         }
+        Dr[0][rt] = -Dr[0][rt];
+        Dr[1][rt] = Dr[0][rt] - Dr[1][rt];
 #pragma unroll
         for (int kh = 0; kh < S::VH; ++kh) of[rt][kh] = ld_edge(a.dout + b * a.gb + h * a.gh + safe * a.gt, kh * 32 + g * 8, tiles ? w : 0);
     }
@@ -498,17 +536,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
 #pragma unroll
             for (int dt = 0; dt < S::DT; ++dt) dq[m][rt][dt] = ZERO4;
     if (tiles) {
-        dma_qk<NI>(kp, a.kt, a.km, a.d, 0, kl - 1, smem, lane, wave);
-        dma_v<NI>(vp, a.vt, a.d, 0, kl - 1, smem + NI * TILE, lane, wave);
+        const Src<NI> src(lane, wave, a.d, a.km);
+        src.fetch(kp, a.kt, src.qk, 0, kl - 1, (XVA_LDS uint8_t*)even, wave);
+        src.fetch(vp, a.vt, src.v, 0, kl - 1, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
-    for (int jb = 0; jb < tiles; ++jb) {
-        const XVA_LDS uint8_t* Kt = smem + (jb & 1) * 2 * NI * TILE;
-        const XVA_LDS uint8_t* Vt = Kt + NI * TILE;
+    auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         if (jb + 1 < tiles) {
-            XVA_LDS uint8_t* next = smem + ((jb & 1) ^ 1) * 2 * NI * TILE;
-            dma_qk<NI>(kp, a.kt, a.km, a.d, (jb + 1) * 64, kl - 1, next, lane, wave);
-            dma_v<NI>(vp, a.vt, a.d, (jb + 1) * 64, kl - 1, next + NI * TILE, lane, wave);
+            const Src<NI> src(again(lane), wave, a.d, a.km);
+            src.fetch(kp, a.kt, src.qk, (jb + 1) * 64, kl - 1, next, wave);
+            src.fetch(vp, a.vt, src.v, (jb + 1) * 64, kl - 1, next + NI * TILE, wave);
         }
         if (jb * 64 < wave_keys) {
             const bool whole = (jb + 1) * 64 <= whole_keys && wrow + 32 <= ql;
@@ -524,25 +561,31 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
                         for (int kh = 0; kh < S::KH; ++kh) {
-                            const bf16x8 kf = fr.read_kc(Kt + qk_image<NI>(m) * TILE, kt, qk_half<NI>(m, kh));
+                            const bf16x8 kf = fr.rows(smem, qk_image<NI>(m), kt, qk_half<NI>(m, kh));
 #pragma unroll
                             for (int rt = 0; rt < 2; ++rt) s[m][u][rt] = MFMA(kf, qf[m][rt][kh], s[m][u][rt]);
                         }
 #pragma unroll
                     for (int kh = 0; kh < S::VH; ++kh) {
-                        const bf16x8 vf = fr.read_kc(Vt + (kh >> 1) * TILE, kt, kh & 1);
+                        const bf16x8 vf = fr.rows(smem, NI + (kh >> 1), kt, kh & 1);
 #pragma unroll
                         for (int rt = 0; rt < 2; ++rt) dp[u][rt] = MFMA(vf, of[rt][kh], dp[u][rt]);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const bool ok = jb * 64 + kt * 16 + g * 4 + r < limit[rt];
+                                s[0][u][rt][r] = ok ? s[0][u][rt][r] : -INFINITY;
+                                s[1][u][rt][r] = ok ? s[1][u][rt][r] : -INFINITY;
+                            }
                     }
 #pragma unroll
                     for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            float p1 = exp2_(s[0][u][rt][r] * a.c - L[0][rt]), p2 = exp2_(s[1][u][rt][r] * a.c - L[1][rt]);
-                            if (!whole) {
-                                const bool ok = jb * 64 + kt * 16 + g * 4 + r < limit[rt];
-                                p1 = ok ? p1 : 0.f; p2 = ok ? p2 : 0.f;
-                            }
+                            const float p1 = exp2_(s[0][u][rt][r] * a.c - L[0][rt]), p2 = exp2_(s[1][u][rt][r] * a.c - L[1][rt]);
                             const float x = dp[u][rt][r];
                             dl += p2 * x;
                             s[0][u][rt][r] = p1 * (x - Dr[0][rt]);
@@ -558,15 +601,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int dt = 0; dt < S::DT; ++dt) {
-                        const bf16x8 kf = fr.read_tr(Kt + qk_image<NI>(m) * TILE, qk_tile<NI>(m, dt), t);
+                        const bf16x8 kf = fr.cols(smem, qk_image<NI>(m), qk_tile<NI>(m, dt), t);
 #pragma unroll
                         for (int rt = 0; rt < 2; ++rt) dq[m][rt][dt] = MFMA(kf, df[m][rt], dq[m][rt][dt]);       // [column g * 4 + r][row lane & 15]
                     }
             }
         }
         __syncthreads();
-    }
-    const float lam = a.lam[h];
+    };
+    XVA_TWO_BUFFERS(tiles, tile)
+    const float lam = uniform(a.lam, h);
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
@@ -579,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
                 if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(dst + m * a.d + dt * 16 + g * 4, dq[m][rt][dt], m ? -lam * a.scale : a.scale);
     }
     // (the tile loop has ended with a barrier)
-    XVA_LDS float* red = (XVA_LDS float*)smem_raw;
+    XVA_LDS float* red = (XVA_LDS float*)even;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) dl += __shfl_xor(dl, o, 64);
     if (lane == 0) red[wave] = dl;
@@ -611,8 +655,9 @@ int check(const xva_diff_attention_args* p, const char* who) {
     int64_t all = 0;
     for (int e = 0; e < 4; ++e) all |= p->q_stride[e] | p->k_stride[e];
     for (int e = 0; e < 3; ++e) all |= p->v_stride[e] | p->out_stride[e] | p->dout_stride[e];
+    XVA_CHECK_ARG(p->q_stride[3] < (1 << 30) && p->q_stride[3] > -(1 << 30) && p->k_stride[3] < (1 << 30) && p->k_stride[3] > -(1 << 30), "%s: maps further than 2^30 elements apart", who);
     XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
-    const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 127) / 128);
+    const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
     XVA_CHECK_ARG(wgs < (1ll << 31) && kwgs < (1ll << 31), "%s: too many blocks", who);
     return XVA_OK;
 }
@@ -643,7 +688,7 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
     rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
     if (a.Tk > 0) {
-        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 127) / 128)), 256, 0, st>>>(a);
+        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64)), 256, 0, st>>>(a);
         XVA_LAUNCH_CHECK();
     }
     dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb), 256, 0, st>>>(a);
