@@ -287,6 +287,236 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     }
 }
 
+// ================================================================================ forward, few queries ====
+// Up to 32 rows (query heads of a key head x queries) against a long cache: the work is reading k and v once, so the rows of all heads that share a key head sit
+// in one matrix tile and the keys are what is cut up.  A workgroup takes a chunk of keys, its waves the chunk's 32-key tiles by turns, each with its own softmax
+// and its own buffers (nothing waits for another wave): k straight to registers in the fragments' layout, v through LDS for its transposed fragments, both one
+// tile ahead.  The waves' results join in LDS, the chunks' (where there are several) in a second kernel.
+// Partial results of a chunk: (max, sum) of [2][rows], then [2][rows][2 d] sums of exp2(c (S - max)) V.
+template <int D16, bool F16, int RT>
+__global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(Args a, float* __restrict__ part, int chunk, int nsplit) {
+    using S = Shape<D16>;
+    constexpr int NI = S::NI, HALF = TILE / 2, W = NI * 64;                    // bytes of a 32-row image; padded width of v
+    __shared__ __attribute__((aligned(1024))) uint8_t even[4 * NI * HALF], odd[4 * NI * HALF];
+    __shared__ float stat[4][2][RT * 16][2];
+    const int split = blockIdx.x % nsplit, bh = blockIdx.x / nsplit, hk = bh % a.Hk, b = bh / a.Hk;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, i = lane & 15, w = 2 * a.d, R = a.share * a.Tq;
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql;
+    const int k0 = split * chunk, k1 = min(k0 + chunk, kl);
+    const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
+    const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
+    bf16x8 qf[2][RT][S::KH];
+    int limit[RT];                                                             // keys that the lane's row sees
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = rt * 16 + i, hs = r / a.Tq, t = r - hs * a.Tq;
+        const bool row = r < R && t < ql;
+        limit[rt] = row ? (a.causal ? max(min(kl, t + off + 1), 0) : kl) : 0;
+        const uint16_t* qr = a.q + b * a.qb + (row ? t : 0) * a.qt + (hk * a.share + (row ? hs : 0)) * a.qh;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = ld_edge(qr + m * a.qm, kh * 32 + g * 8, row ? a.d : 0);
+    }
+    f32x4 o[2][RT][S::VT];
+    float mx[2][RT], sum[2][RT];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            mx[m][rt] = -INFINITY; sum[m][rt] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] = ZERO4;
+        }
+    const Lane fr(lane, wave * NI * HALF);
+    bf16x8 kf[2][2][S::KH], kn[2][2][S::KH];                                   // this tile's and the next one's
+    auto fetch = [&](int key0, XVA_LDS uint8_t* to, bf16x8 (&into)[2][2][S::KH]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint16_t* row = kp + (int64_t)min(key0 + u * 16 + i, k1 - 1) * a.kt;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int kh = 0; kh < S::KH; ++kh) {
+                    const int d0 = kh * 32 + g * 8;                            // (behind d: columns that meet q's zeros; a load on every way, see below)
+                    into[m][u][kh] = xva_attn::ld_frag(row + m * a.km + (d0 < a.d ? d0 : 0));
+                }
+        }
+        const int p = lane & 7;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = q * 8 + (lane >> 3), c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
+            const uint16_t* row = vp + (int64_t)min(key0 + r, k1 - 1) * a.vt;
+#pragma unroll
+            for (int im = 0; im < NI; ++im) {
+                const int e0 = im * 64 + c * 8;
+                __builtin_amdgcn_global_load_lds((const XVA_GLB void*)(row + (e0 < w ? e0 : 0)), (XVA_LDS void*)(to + (wave * NI + im) * HALF + q * 1024), 16, 0, 0);
+            }
+        }
+    };
+    auto tile = [&](int key0, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next, bf16x8 (&kc)[2][2][S::KH], bf16x8 (&kx)[2][2][S::KH]) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // the other buffer's last reads have arrived
+        fetch(key0 + 128, next, kx);
+        bf16x8 pf[2][RT];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            f32x4 s[RT][2];
+            bool grew = false;
+            float top[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    s[rt][u] = ZERO4;
+#pragma unroll
+                    for (int kh = 0; kh < S::KH; ++kh) s[rt][u] = MFMA(kc[m][u][kh], qf[m][rt][kh], s[rt][u]);       // [key g * 4 + r][row lane & 15]
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[rt][u][r] = key0 + u * 16 + g * 4 + r < min(limit[rt], k1) ? s[rt][u][r] : -INFINITY;
+                }
+                top[rt] = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
+                                fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+                grew |= (top[rt] - mx[m][rt]) * a.c > 8.f;
+            }
+            if (__any(grew)) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    float now = fmaxf(top[rt], __shfl_xor(top[rt], 16, 64));
+                    now = fmaxf(fmaxf(now, __shfl_xor(now, 32, 64)), mx[m][rt]);
+                    const float alpha = mx[m][rt] == now ? 1.f : exp2_((mx[m][rt] - now) * a.c);
+                    mx[m][rt] = now;
+                    sum[m][rt] *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] *= alpha;
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float base = mx[m][rt] == -INFINITY ? 0.f : mx[m][rt] * a.c;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = exp2_(s[rt][u][r] * a.c - base);
+                        sum[m][rt] += p;
+                        s[rt][u][r] = p;
+                    }
+                pf[m][rt] = pack_rows<F16>(s[rt][0], s[rt][1]);
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < S::VT; ++dt) {
+            const XVA_LDS uint8_t* at = smem + (fr.tr ^ ((dt & 3) * 32)) + (dt >> 2) * HALF;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((XVA_LDS s16x4*)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((XVA_LDS s16x4*)(at + 2048));
+            const bf16x8 vf = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) o[m][rt][dt] = MFMA(vf, pf[m][rt], o[m][rt][dt]);                    // [column g * 4 + r][row lane & 15]
+        }
+    };
+    const int mine = k0 + wave * 32;
+    // A tile is fetched behind the last one too (its rows clamped to the chunk's last): on every way through the loop the same number of loads is in flight, so
+    // that the compiler can wait for the older ones alone.
+    if (mine < k1) {
+        fetch(mine, (XVA_LDS uint8_t*)even, kf);
+        for (int key0 = mine;; key0 += 256) {
+            tile(key0, (const XVA_LDS uint8_t*)even, (XVA_LDS uint8_t*)odd, kf, kn);
+            if (key0 + 128 >= k1) break;
+            tile(key0 + 128, (const XVA_LDS uint8_t*)odd, (XVA_LDS uint8_t*)even, kn, kf);
+            if (key0 + 256 >= k1) break;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                           // (the last fetch's bytes land before the buffers are used for the results)
+    // the waves' maxima and sums
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float l = sum[m][rt];
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            if (g == 0) { stat[wave][m][rt * 16 + i][0] = mx[m][rt]; stat[wave][m][rt * 16 + i][1] = l; }
+        }
+    __syncthreads();
+    // a map and 16 rows at a time: every wave's sums relative to the common maximum, [wave][row][column] in LDS, added and taken on by 16 x 16 threads
+    XVA_LDS float* x = (XVA_LDS float*)even;
+    const int row = threadIdx.x >> 4, col = (threadIdx.x & 15) * (W / 16);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float first[W / 16];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) top = fmaxf(top, stat[v][m][rt * 16 + i][0]);
+            const float scale = mx[m][rt] == -INFINITY ? 0.f : exp2_((mx[m][rt] - top) * a.c);
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt) *reinterpret_cast<XVA_LDS f32x4*>(x + (wave * 16 + i) * W + dt * 16 + g * 4) = o[m][rt][dt] * scale;
+            __syncthreads();
+            const int r = rt * 16 + row;
+            float rtop = -INFINITY, l = 0.f, acc[W / 16];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) rtop = fmaxf(rtop, stat[v][m][r][0]);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) l += stat[v][m][r][0] == -INFINITY ? 0.f : stat[v][m][r][1] * exp2_((stat[v][m][r][0] - rtop) * a.c);
+#pragma unroll
+            for (int e = 0; e < W / 16; ++e) acc[e] = x[row * W + col + e] + x[(16 + row) * W + col + e] + x[(32 + row) * W + col + e] + x[(48 + row) * W + col + e];
+            if (r < R && col < w) {
+                if (nsplit > 1) {
+                    float* to = part + (int64_t)blockIdx.x * 2 * R * (w + 2);
+                    if (col == 0) { to[(m * R + r) * 2] = rtop; to[(m * R + r) * 2 + 1] = l; }
+#pragma unroll
+                    for (int e = 0; e < W / 16; ++e)
+                        if (col + e < w) to[4 * R + (int64_t)(m * R + r) * w + col + e] = acc[e];
+                } else {
+                    const float inv = rtop == -INFINITY ? 0.f : 1.f / l;
+                    if (m == 0) {
+#pragma unroll
+                        for (int e = 0; e < W / 16; ++e) first[e] = rtop == -INFINITY ? 0.f : acc[e] * inv;
+                    } else {
+                        const int hs = r / a.Tq, h = hk * a.share + hs;
+                        const float by = a.lam[h];
+                        uint16_t* out = a.out + b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh;
+#pragma unroll
+                        for (int e = 0; e < W / 16; e += 2)
+                            if (col + e < w)
+                                *reinterpret_cast<uint32_t*>(out + col + e) = pack2<F16>(first[e] - by * (rtop == -INFINITY ? 0.f : acc[e] * inv),
+                                                                                         first[e + 1] - by * (rtop == -INFINITY ? 0.f : acc[e + 1] * inv));
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// joins the chunks of a row; 2 d threads have a column each
+template <bool F16>
+__global__ __launch_bounds__(128) void few_join_kernel(Args a, const float* __restrict__ part, int nsplit) {
+    const int w = 2 * a.d, col = threadIdx.x, R = a.share * a.Tq;
+    const int id = blockIdx.x, bh = id / R, r = id - bh * R, hk = bh % a.Hk, b = bh / a.Hk;
+    const int64_t each = (int64_t)2 * R * (w + 2);
+    const float* p = part + (int64_t)bh * nsplit * each;
+    if (col >= w) return;
+    float res[2];
+    for (int m = 0; m < 2; ++m) {
+        float top = -INFINITY, l = 0.f, acc = 0.f;
+        for (int k = 0; k < nsplit; ++k) top = fmaxf(top, p[k * each + (m * R + r) * 2]);
+        if (top != -INFINITY)
+            for (int k = 0; k < nsplit; ++k) {
+                const float mx = p[k * each + (m * R + r) * 2];
+                if (mx == -INFINITY) continue;
+                const float by = exp2_((mx - top) * a.c);
+                l += p[k * each + (m * R + r) * 2 + 1] * by;
+                acc += p[k * each + 4 * R + (int64_t)(m * R + r) * w + col] * by;
+            }
+        res[m] = top == -INFINITY ? 0.f : acc / l;
+    }
+    const int hs = r / a.Tq, h = hk * a.share + hs;
+    a.out[b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh + col] = cvt16<F16>(res[0] - a.lam[h] * res[1]);
+}
+
 // ================================================================================ backward ====
 // D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns
 template <bool F16>
@@ -330,7 +560,11 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     constexpr int STAT = 2 * NI * TILE;                                                        // {Q dO | lse1 lse2 D1 D2} of the even and of the odd tiles
     __shared__ __attribute__((aligned(1024))) uint8_t even[STAT + 1024], odd[STAT + 1024];
     __shared__ __attribute__((aligned(16))) uint8_t away_raw[AWAY ? AWAY * 4096 : 16];
-    const int kblk = blockIdx.x / (a.B * a.Hk), bh = blockIdx.x % (a.B * a.Hk);                // (the first keys are seen by most queries: they start first)
+    // Under `causal` the first keys are seen by most queries: they start first.  Where all workgroups are on the card at once, two to a CU, the second of a CU
+    // is one from the other end, so that each CU has as much to do as another.
+    unsigned id = blockIdx.x;
+    if (a.causal && gridDim.x <= 512 && id >= 256) id = gridDim.x - 1 - (id - 256);
+    const int kblk = id / (unsigned)(a.B * a.Hk), bh = id % (unsigned)(a.B * a.Hk);
     const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15, t = wave >> 1;
@@ -675,6 +909,33 @@ Args args_of(const xva_diff_attention_args* p) {
     a.scale = p->scale; a.c = p->scale * 1.44269504088896341f;
     return a;
 }
+// Few rows: keys of a chunk, a multiple of the 128 that the four waves take in one turn; about 1024 workgroups (four to a CU: items of a ragged batch end early),
+// none with less than 128 keys
+struct Few { bool on; int chunk, nsplit; };
+Few few_plan(const xva_diff_attention_args* p) {
+    Few f = {p->maps == nullptr && (int64_t)p->H / p->Hk * p->Tq <= 32 && p->Tk > 0 && p->B > 0 && p->Tq > 0, 0, 1};
+    if (!f.on) return f;
+    const int64_t heads = (int64_t)p->B * p->Hk, want = (1024 + heads - 1) / heads;
+    int64_t chunk = (p->Tk + want - 1) / want;
+    chunk = (chunk + 127) / 128 * 128;
+    f.chunk = (int)chunk;
+    f.nsplit = (int)((p->Tk + chunk - 1) / chunk);
+    return f;
+}
+int64_t few_floats(const xva_diff_attention_args* p, const Few& f) {
+    return f.on && f.nsplit > 1 ? (int64_t)p->B * p->H * p->Tq * f.nsplit * 2 * (2 * p->d + 2) : 0;
+}
+template <int D16, bool F16> int few(const Args& a, const Few& f, float* part, hipStream_t st) {
+    const unsigned grid = (unsigned)(a.B * a.Hk * f.nsplit);
+    if (a.share * a.Tq <= 16) few_kernel<D16, F16, 1><<<grid, 256, 0, st>>>(a, part, f.chunk, f.nsplit);
+    else few_kernel<D16, F16, 2><<<grid, 256, 0, st>>>(a, part, f.chunk, f.nsplit);
+    XVA_LAUNCH_CHECK();
+    if (f.nsplit > 1) {
+        few_join_kernel<F16><<<(unsigned)(a.B * a.H * a.Tq), 128, 0, st>>>(a, part, f.nsplit);
+        XVA_LAUNCH_CHECK();
+    }
+    return XVA_OK;
+}
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
     const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128));
     if (train) fwd_kernel<D16, F16, true><<<grid, 256, 0, st>>>(a);
@@ -698,7 +959,7 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
     return XVA_OK;
 }
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
-    if (!bwd) return 0;
+    if (!bwd) return few_floats(p, few_plan(p)) * 4;
     return ((int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128)) * 4;
 }
 }   // namespace
@@ -720,7 +981,14 @@ extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws
     if (p->B == 0 || p->Tq == 0) return XVA_OK;
     XVA_CHECK_ARG(p->out && (p->maps == nullptr) == (p->lse == nullptr), "xva_diff_attention_fwd: null argument");
     const Args a = args_of(p);
-#define CALL(D16, F16) forward<D16, F16>(a, p->maps != nullptr, (hipStream_t)stream)
+    const Few f = few_plan(p);
+    const int64_t need = few_floats(p, f) * 4;
+    if (ws_bytes < need || (need && !ws)) {
+        xva_set_error("xva_diff_attention_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+        return XVA_ERR_WS;
+    }
+    XVA_CHECK_ARG((int64_t)p->B * p->Hk * f.nsplit < (1ll << 31) && (!f.on || (int64_t)p->B * p->H * p->Tq < (1ll << 31)), "xva_diff_attention_fwd: too many blocks");
+#define CALL(D16, F16) (f.on ? few<D16, F16>(a, f, (float*)ws, (hipStream_t)stream) : forward<D16, F16>(a, p->maps != nullptr, (hipStream_t)stream))
     XVA_DIFF_BY_SHAPE(CALL)
 #undef CALL
 }
