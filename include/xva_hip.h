@@ -778,7 +778,8 @@ int xva_recurrence_fwd(const xva_recurrence_args* p, void* workspace, int64_t wo
 int xva_recurrence_bwd(const xva_recurrence_args* p, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Differential attention (bf16 / fp16).  q (B, Tq, H, 2, d), k (B, Tk, Hk, 2, d), v (B, Tk, Hk, 2 d), lam (H) fp32; d a multiple of 8 up to 64, H a multiple
- * of Hk (query head h reads key head h / (H / Hk)); addresses 16-byte aligned, strides multiples of 8.  out (B, Tq, H, 2 d) =
+ * of Hk (query head h reads key head h / (H / Hk)); addresses 16-byte aligned, strides multiples of 8, those of rows and maps
+ * under 2^24.  out (B, Tq, H, 2 d) =
  * (softmax(scale q_1 k_1^T) - lam softmax(scale q_2 k_2^T)) v.  q_lens / k_lens (B): live queries and keys (null: all); causal: query i sees keys
  * j <= i + k_len - q_len.  Rows that see nothing, and rows behind q_len, leave as zeros.
  * For a backward pass the forward also writes maps (2, B, Tq, H, 2 d), each softmax's own output, and lse (2, B, H, Tq) fp32 (both null: no backward).

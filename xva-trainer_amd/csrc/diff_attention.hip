@@ -50,30 +50,40 @@ template <int D16> struct Shape {
 
 __device__ __forceinline__ int len_of(const int32_t* l, int b, int T) { return l ? min(max(l[b], 0), T) : T; }
 
+// 16 bytes to LDS from `rows` + `off` bytes, within the `bytes` that are there.  A buffer load: the compiler counts it like any load, where the global form's wait
+// would be for everything in flight.
+__device__ __forceinline__ void load_lds(const uint16_t* rows, uint32_t bytes, uint32_t off, XVA_LDS uint8_t* to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)rows, 0, bytes, 0x00027000), (XVA_LDS void*)to, 16, off, 0, 0, 0);
+}
 // Where this lane's two 16-byte pieces of an image come from: rows r and r + 32 of the tile, one column (the swizzle repeats every 8 rows).  Columns behind the
 // width read the row's first ones: they meet zeros in the other operand, or results that nobody stores, and a row that is not finite is lost through its
 // live columns already.
 template <int NI> struct Src {
-    int r, qk[NI], v[NI];                         // row, and the column's element offset: a q / k tile's with the map's
+    uint32_t r, qk[NI], v[NI];                    // row, and the column's byte offset in each image: a q / k tile's (one image: with the map's), a v / dO tile's
     __device__ __forceinline__ Src(int lane, int wave, int d, int64_t map_stride) {
         r = wave * 8 + (lane >> 3);
         const int p = lane & 7, c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
 #pragma unroll
         for (int im = 0; im < NI; ++im) {
-            const int map = NI == 2 ? im : c >> 2, d0 = (NI == 2 ? c : c & 3) * 8, e0 = im * 64 + c * 8;
-            qk[im] = map * (int)map_stride + (d0 < d ? d0 : 0);
-            v[im] = e0 < 2 * d ? e0 : 0;
+            const int d0 = (NI == 2 ? c : c & 3) * 8, e0 = im * 64 + c * 8;
+            qk[im] = 2u * ((NI == 2 ? 0u : (uint32_t)(c >> 2) * (uint32_t)map_stride) + (d0 < d ? d0 : 0));
+            v[im] = 2u * (e0 < 2 * d ? e0 : 0);
         }
     }
-    // rows row0 .. row0 + 63, clamped to rmax (>= 0)
-    __device__ __forceinline__ void fetch(const uint16_t* base, int64_t ld, const int (&col)[NI], int row0, int rmax, XVA_LDS uint8_t* tile, int wave) const {
+    // the `left` (>= 1) rows from `rows` on, clamped to the last of them; images `apart` elements from each other, `width` elements behind a row's first one
+    __device__ __forceinline__ void fetch(const uint16_t* rows, int64_t ld, int64_t apart, int64_t width, const uint32_t (&col)[NI], int left, XVA_LDS uint8_t* tile, int wave) const {
+        const uint32_t ldb = (uint32_t)ld * 2u, bytes = (uint32_t)(min(left, 64) - 1) * ldb + (uint32_t)width * 2u;
+        const uint32_t at[2] = {min(r, (uint32_t)left - 1) * ldb, min(r + 32, (uint32_t)left - 1) * ldb};
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const uint16_t* row = base + (int64_t)min(row0 + q * 32 + r, rmax) * ld;
+        for (int im = 0; im < NI; ++im)
 #pragma unroll
-            for (int im = 0; im < NI; ++im)
-                __builtin_amdgcn_global_load_lds((const XVA_GLB void*)(row + col[im]), (XVA_LDS void*)(tile + im * TILE + (q * 4 + wave) * 1024), 16, 0, 0);
-        }
+            for (int q = 0; q < 2; ++q) load_lds(rows + im * apart, bytes, at[q] + col[im], tile + im * TILE + (q * 4 + wave) * 1024);
+    }
+    __device__ __forceinline__ void fetch_qk(const uint16_t* rows, int64_t ld, int64_t map_stride, int d, int left, XVA_LDS uint8_t* tile, int wave) const {
+        fetch(rows, ld, NI == 2 ? map_stride : 0, NI == 2 ? d : map_stride + d, qk, left, tile, wave);
+    }
+    __device__ __forceinline__ void fetch_v(const uint16_t* rows, int64_t ld, int d, int left, XVA_LDS uint8_t* tile, int wave) const {
+        fetch(rows, ld, 0, 2 * d, v, left, tile, wave);
     }
 };
 // `lane`, but unknown to the compiler: what is computed from it inside a loop is not kept in registers across the loop (where the accumulators leave none)
@@ -165,15 +175,16 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
         }
     if (tiles) {
         const Src<NI> src(lane, wave, a.d, a.km);
-        src.fetch(kp, a.kt, src.qk, 0, kl - 1, (XVA_LDS uint8_t*)even, wave);
-        src.fetch(vp, a.vt, src.v, 0, kl - 1, (XVA_LDS uint8_t*)even + NI * TILE, wave);
+        src.fetch_qk(kp, a.kt, a.km, a.d, kl, (XVA_LDS uint8_t*)even, wave);
+        src.fetch_v(vp, a.vt, a.d, kl, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
     auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         if (jb + 1 < tiles) {
             const Src<NI> src(again(lane), wave, a.d, a.km);
-            src.fetch(kp, a.kt, src.qk, (jb + 1) * 64, kl - 1, next, wave);
-            src.fetch(vp, a.vt, src.v, (jb + 1) * 64, kl - 1, next + NI * TILE, wave);
+            const int row0 = (jb + 1) * 64;
+            src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, next, wave);
+            src.fetch_v(vp + row0 * a.vt, a.vt, a.d, kl - row0, next + NI * TILE, wave);
         }
         if (jb * 64 < wave_keys) {
             const bool whole = (jb + 1) * 64 <= whole_keys;
@@ -344,14 +355,15 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
                 }
         }
         const int p = lane & 7;
+        const uint32_t left = max(k1 - key0, 1), ldb = (uint32_t)a.vt * 2u, bytes = (min(left, 32u) - 1) * ldb + w * 2;
+        const uint16_t* rows = vp + min(key0, k1 - 1) * a.vt;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int r = q * 8 + (lane >> 3), c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
-            const uint16_t* row = vp + (int64_t)min(key0 + r, k1 - 1) * a.vt;
+            const uint32_t r = q * 8 + (lane >> 3), c = (((p >> 1) ^ ((r >> 1) & 3)) << 1) | (p & 1);
 #pragma unroll
             for (int im = 0; im < NI; ++im) {
                 const int e0 = im * 64 + c * 8;
-                __builtin_amdgcn_global_load_lds((const XVA_GLB void*)(row + (e0 < w ? e0 : 0)), (XVA_LDS void*)(to + (wave * NI + im) * HALF + q * 1024), 16, 0, 0);
+                load_lds(rows, bytes, min(r, left - 1) * ldb + 2 * (e0 < w ? e0 : 0), to + (wave * NI + im) * HALF + q * 1024);
             }
         }
     };
@@ -491,30 +503,57 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
     }
 }
 
-// joins the chunks of a row; 2 d threads have a column each
+// joins the chunks of a row: weights of the chunks first, into LDS, then eight slots of chunks beside each other over the columns (four to a thread)
+constexpr int MAX_SPLIT = 1024;
 template <bool F16>
-__global__ __launch_bounds__(128) void few_join_kernel(Args a, const float* __restrict__ part, int nsplit) {
-    const int w = 2 * a.d, col = threadIdx.x, R = a.share * a.Tq;
+__global__ __launch_bounds__(256) void few_join_kernel(Args a, const float* __restrict__ part, int nsplit) {
+    __shared__ float by[2][MAX_SPLIT], sh[16];
+    __shared__ f32x4 sums[2][8][32];
+    const int w = 2 * a.d, R = a.share * a.Tq;
     const int id = blockIdx.x, bh = id / R, r = id - bh * R, hk = bh % a.Hk, b = bh / a.Hk;
     const int64_t each = (int64_t)2 * R * (w + 2);
     const float* p = part + (int64_t)bh * nsplit * each;
-    if (col >= w) return;
-    float res[2];
+    float inv[2];
+#pragma unroll
     for (int m = 0; m < 2; ++m) {
-        float top = -INFINITY, l = 0.f, acc = 0.f;
-        for (int k = 0; k < nsplit; ++k) top = fmaxf(top, p[k * each + (m * R + r) * 2]);
-        if (top != -INFINITY)
-            for (int k = 0; k < nsplit; ++k) {
-                const float mx = p[k * each + (m * R + r) * 2];
-                if (mx == -INFINITY) continue;
-                const float by = exp2_((mx - top) * a.c);
-                l += p[k * each + (m * R + r) * 2 + 1] * by;
-                acc += p[k * each + 4 * R + (int64_t)(m * R + r) * w + col] * by;
-            }
-        res[m] = top == -INFINITY ? 0.f : acc / l;
+        float top = -INFINITY, l = 0.f;
+        for (int k = threadIdx.x; k < nsplit; k += 256) top = fmaxf(top, by[m][k] = p[k * each + (m * R + r) * 2]);
+        top = xva_block_max(top, sh);
+        for (int k = threadIdx.x; k < nsplit; k += 256) {
+            const float e = by[m][k] == -INFINITY ? 0.f : exp2_((by[m][k] - top) * a.c);
+            by[m][k] = e;
+            l += e * p[k * each + (m * R + r) * 2 + 1];
+        }
+        l = xva_block_sum(l, sh);
+        inv[m] = top == -INFINITY ? 0.f : 1.f / l;
     }
-    const int hs = r / a.Tq, h = hk * a.share + hs;
-    a.out[b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh + col] = cvt16<F16>(res[0] - a.lam[h] * res[1]);
+    __syncthreads();
+    const int slot = threadIdx.x >> 5, col = (threadIdx.x & 31) * 4;
+    if (col < w) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            f32x4 acc = ZERO4;
+            const float* q = p + 4 * R + (int64_t)(m * R + r) * w + col;
+#pragma unroll 4
+            for (int k = slot; k < nsplit; k += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[e] += q[k * each + e] * by[m][k];
+            sums[m][slot][threadIdx.x & 31] = acc;
+        }
+    }
+    __syncthreads();
+    if (slot == 0 && col < w) {
+        f32x4 t[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            t[m] = sums[m][0][threadIdx.x];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) t[m] += sums[m][k][threadIdx.x];
+            t[m] *= inv[m];
+        }
+        const int hs = r / a.Tq, h = hk * a.share + hs;
+        xva_attn::st4<F16>(a.out + b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh + col, t[0] - a.lam[h] * t[1], 1.f);
+    }
 }
 
 // ================================================================================ backward ====
@@ -603,10 +642,11 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     auto fetch = [&](int hs, int row0, XVA_LDS uint8_t* to) {
         const int h = hk * a.share + hs, lane_ = again(lane);
         const Src<NI> src(lane_, wave, a.d, a.qm);
-        src.fetch(a.q + b * a.qb + h * a.qh, a.qt, src.qk, row0, ql - 1, to, wave);
-        src.fetch(a.dout + b * a.gb + h * a.gh, a.gt, src.v, row0, ql - 1, to + NI * TILE, wave);
-        const float* from = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + min(row0 + lane_, ql - 1);
-        __builtin_amdgcn_global_load_lds((const XVA_GLB void*)from, (XVA_LDS void*)(to + STAT + wave * 256), 4, 0, 0);
+        src.fetch_qk(a.q + b * a.qb + h * a.qh + row0 * a.qt, a.qt, a.qm, a.d, ql - row0, to, wave);
+        src.fetch_v(a.dout + b * a.gb + h * a.gh + row0 * a.gt, a.gt, a.d, ql - row0, to + NI * TILE, wave);
+        const float* from = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + row0;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)min(ql - row0, 64) * 4u, 0x00027000),
+                                                 (XVA_LDS void*)(to + STAT + wave * 256), 4, min(lane_, ql - row0 - 1) * 4, 0, 0, 0);
     };
     if (total) fetch(0, t0 * 64, (XVA_LDS uint8_t*)even);
     __syncthreads();
@@ -644,11 +684,12 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
                     }
                 }
                 if (!whole) {
+                    const int l = again(lane);
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const int row = wrow + u * 16 + g * 4 + r, key = wkey + kt * 16 + i;
+                            const int row = wrow + u * 16 + (l >> 4) * 4 + r, key = wkey + kt * 16 + (l & 15);
                             const bool ok = (row < ql) & (key < kl) & (!a.causal | (key <= row + off));
                             s[0][kt][r] = ok ? s[0][kt][r] : -INFINITY;
                             s[1][kt][r] = ok ? s[1][kt][r] : -INFINITY;
@@ -692,8 +733,9 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
         __syncthreads();
     };
     XVA_TWO_BUFFERS(total, tile)
+    const int l = again(lane), ge = l >> 4, ie = l & 15;
     // the second half of the queries hands its sums over: 16 bytes a lane and accumulator
-    XVA_LDS f32x4* xch = (XVA_LDS f32x4*)((wave & 1) ? odd : even) + lane;
+    XVA_LDS f32x4* xch = (XVA_LDS f32x4*)((wave & 1) ? odd : even) + l;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
         if (t == 1) {
@@ -705,17 +747,17 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
             for (int dt = 0; dt < S::VT; ++dt) xch[(2 * S::DT + dt) * 64] = dv[kt][dt];
         }
         __syncthreads();
-        const int key = wkey + kt * 16 + i;
+        const int key = wkey + kt * 16 + ie;
         if (t == 0 && key < a.Tk) {
             const int64_t row = ((int64_t)b * a.Tk + key) * a.Hk + hk;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int dt = 0; dt < S::DT; ++dt)
-                    if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + g * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale);
+                    if (dt * 16 + ge * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + ge * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale);
 #pragma unroll
             for (int dt = 0; dt < S::VT; ++dt)
-                if (dt * 16 + g * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + g * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], 1.f);
+                if (dt * 16 + ge * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + ge * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], 1.f);
         }
         __syncthreads();
     }
@@ -771,15 +813,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
             for (int dt = 0; dt < S::DT; ++dt) dq[m][rt][dt] = ZERO4;
     if (tiles) {
         const Src<NI> src(lane, wave, a.d, a.km);
-        src.fetch(kp, a.kt, src.qk, 0, kl - 1, (XVA_LDS uint8_t*)even, wave);
-        src.fetch(vp, a.vt, src.v, 0, kl - 1, (XVA_LDS uint8_t*)even + NI * TILE, wave);
+        src.fetch_qk(kp, a.kt, a.km, a.d, kl, (XVA_LDS uint8_t*)even, wave);
+        src.fetch_v(vp, a.vt, a.d, kl, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
     auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         if (jb + 1 < tiles) {
             const Src<NI> src(again(lane), wave, a.d, a.km);
-            src.fetch(kp, a.kt, src.qk, (jb + 1) * 64, kl - 1, next, wave);
-            src.fetch(vp, a.vt, src.v, (jb + 1) * 64, kl - 1, next + NI * TILE, wave);
+            const int row0 = (jb + 1) * 64;
+            src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, next, wave);
+            src.fetch_v(vp + row0 * a.vt, a.vt, a.d, kl - row0, next + NI * TILE, wave);
         }
         if (jb * 64 < wave_keys) {
             const bool whole = (jb + 1) * 64 <= whole_keys && wrow + 32 <= ql;
@@ -889,7 +932,9 @@ int check(const xva_diff_attention_args* p, const char* who) {
     int64_t all = 0;
     for (int e = 0; e < 4; ++e) all |= p->q_stride[e] | p->k_stride[e];
     for (int e = 0; e < 3; ++e) all |= p->v_stride[e] | p->out_stride[e] | p->dout_stride[e];
-    XVA_CHECK_ARG(p->q_stride[3] < (1 << 30) && p->q_stride[3] > -(1 << 30) && p->k_stride[3] < (1 << 30) && p->k_stride[3] > -(1 << 30), "%s: maps further than 2^30 elements apart", who);
+    // 64 rows of a tile, and its maps, within 32-bit byte offsets
+    const int64_t near[] = {p->q_stride[1], p->q_stride[3], p->k_stride[1], p->k_stride[3], p->v_stride[1], p->dout_stride[1]};
+    for (int64_t e : near) XVA_CHECK_ARG(e >= 0 && e < (1 << 24), "%s: row and map strides are 0 .. 2^24 - 1", who);
     XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
     const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
     XVA_CHECK_ARG(wgs < (1ll << 31) && kwgs < (1ll << 31), "%s: too many blocks", who);
@@ -931,7 +976,7 @@ template <int D16, bool F16> int few(const Args& a, const Few& f, float* part, h
     else few_kernel<D16, F16, 2><<<grid, 256, 0, st>>>(a, part, f.chunk, f.nsplit);
     XVA_LAUNCH_CHECK();
     if (f.nsplit > 1) {
-        few_join_kernel<F16><<<(unsigned)(a.B * a.H * a.Tq), 128, 0, st>>>(a, part, f.nsplit);
+        few_join_kernel<F16><<<(unsigned)(a.B * a.H * a.Tq), 256, 0, st>>>(a, part, f.nsplit);
         XVA_LAUNCH_CHECK();
     }
     return XVA_OK;

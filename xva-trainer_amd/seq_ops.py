@@ -230,8 +230,9 @@ def rotary(plan, q, k=None, positions=None, inplace=False):
 
 # -------------------------------------------------------------------------------------------------------- differential attention ----
 def _wide(t):
-    """`t` as the attention kernels read it: 16-byte rows."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    """`t` as the attention kernels read it: 16-byte rows, 64 of them and their maps within 32-bit offsets."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in st[:-1]) and st[1] < 1 << 24 and st[3] < 1 << 24:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
