@@ -5,19 +5,22 @@
 //   dz = dy act'(z);  dw = sum dz xh, dbias = sum dz (over items and rows);  dx = r (w dz - mean(w dz) - xh mean(w dz xh))
 // Rows at or behind an item's length count for nothing: they are not read, and leave as zeros.
 //
-// Bound: HBM.  Two forms, by the size of one (item, group) slab of T x n values:
-//   * a slab that fits the registers of (part of) one wave — each head's norm behind an attention (T = 1), short items: `slab` kernels.  A slab lies over a
-//     power of two of lanes, so every reduction is a few shuffles; x is read once.  dw / dbias stay in the lanes' registers over all the items that a
-//     workgroup passes, leave as one partial row per workgroup and are added in a fixed order.
-//   * longer ones: `tile` kernels over chunks of rows (all channels of a row, so loads are whole lines whatever n is): statistics of each chunk, then one
-//     pass that joins them and writes.  The second read of x is as close behind the first as the size allows.
-// Statistics are two-pass inside a register tile and joined by the exact update of mean and squared deviations (Chan, Golub, LeVeque), so a mean that is
-// large against the deviation costs nothing.  Everything is held in fp32; sums over rows are made in a fixed order, so results repeat bit for bit.
+// Bound: HBM.  Three forms, by the size of one (item, group) slab of T x n values:
+//   * slab: it fits the registers of (part of) one wave — each head's norm behind an attention (T = 1), short items.  A slab lies over a power of two of lanes, so
+//     every reduction is a few shuffles; x is read once.  dw / dbias stay in the lanes' registers over all the items that a workgroup passes, leave as one partial
+//     row per workgroup and are added in a fixed order.
+//   * whole: some groups of an item fit the registers of a workgroup: read once, kept packed, normalised from there; one kernel forward, one and the sum of
+//     dw / dbias over items backward.
+//   * tile: chunks of rows (all channels of a row, so loads are whole lines whatever n is): statistics of each chunk, then one pass that joins them and writes.
+// Statistics are two-pass from registers and joined by the exact update of mean and squared deviations (Chan, Golub, LeVeque), so a mean that is large against the
+// deviation costs nothing.  Everything is held in fp32; sums over rows are made in a fixed order, so results repeat bit for bit.
 #include "xva_common.h"
 #include "../../include/xva_hip.h"
 #include "seq_vec.h"
 
 namespace {
+using xva_seq::Packed;
+using xva_seq::lanes_sum;
 using xva_seq::load_v;
 using xva_seq::store_v;
 
@@ -37,7 +40,9 @@ struct Args {
     int rows_per_chunk, chunks;
 };
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// (off by a few 2^-24 of 1, as z itself is)
+__device__ __forceinline__ float tanh_(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * z)); }
 template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act, float slope) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -45,8 +50,8 @@ template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act
         switch (act) {
             case RELU: z[e] = v > 0.f ? v : (v != v ? v : 0.f); break;
             case LRELU: z[e] = v > 0.f ? v : slope * v; break;
-            case TANH: z[e] = tanhf(v); break;
-            case SILU: z[e] = v / (1.f + __expf(-v)); break;
+            case TANH: z[e] = tanh_(v); break;
+            case SILU: z[e] = v * sigmoid(v); break;
             case GELU: z[e] = 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); break;
             default: break;
         }
@@ -56,7 +61,7 @@ __device__ __forceinline__ float slope_of(float v, int act, float slope) {
     switch (act) {
         case RELU: return v > 0.f ? 1.f : 0.f;
         case LRELU: return v > 0.f ? 1.f : slope;
-        case TANH: { const float t = tanhf(v); return 1.f - t * t; }
+        case TANH: { const float t = tanh_(v); return 1.f - t * t; }
         case SILU: { const float s = sigmoid(v); return s + s * v * (1.f - s); }
         case GELU: return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * __expf(-0.5f * v * v);
         default: return 1.f;
@@ -65,12 +70,6 @@ __device__ __forceinline__ float slope_of(float v, int act, float slope) {
 __device__ __forceinline__ int live_rows(const Args& a, int b) {
     return a.lens ? min(max(a.lens[b], 0), a.T) : a.T;
 }
-// sum over aligned runs of `width` (a power of two) lanes, in every lane
-__device__ __forceinline__ float lanes_sum(float v, int width) {
-    for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
 // ================================================================================ slab form ====
 // LPG lanes hold one slab, NV vectors of V values each: vector j = k * LPG + lane of the slab is row j / (n / V), channels (j % (n / V)) * V ...
 // A workgroup holds 256 / LPG slabs: GPB groups of 256 / (LPG * GPB) items, and walks over the items.
@@ -98,22 +97,37 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
             sw[k][e] = sb[k][e] = 0.f;
         }
     }
-    for (int64_t b0 = (int64_t)blockIdx.x * s.ipb; b0 < a.B; b0 += (int64_t)gridDim.x * s.ipb) {
+    // this item's values, and the next one's on their way
+    Packed<DT, V> nx[NV], ng[NV];
+    int nlen = 0;
+    auto fetch = [&](int64_t b) __attribute__((always_inline)) {
+        nlen = mine && b < a.B ? live_rows(a, (int)b) : 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            nx[k].clear();
+            if (BWD) ng[k].clear();
+            if (row[k] < nlen) {
+                nx[k].load(a.x, b * a.xb + (int64_t)row[k] * a.xt + ch[k]);
+                if (BWD) ng[k].load(a.dy, b * a.db_ + (int64_t)row[k] * a.dt_ + ch[k]);
+            }
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * s.ipb;
+    fetch((int64_t)blockIdx.x * s.ipb + il);
+    for (int64_t b0 = (int64_t)blockIdx.x * s.ipb; b0 < a.B; b0 += step) {
         const int64_t b = b0 + il;
         const bool on = mine && b < a.B;
-        const int len = on ? live_rows(a, (int)b) : 0;
-        float x[NV][V];
+        const int len = nlen;
+        float x[NV][V], dz[NV][V];
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (row[k] < len) load_v<DT, V>(a.x, b * a.xb + (int64_t)row[k] * a.xt + ch[k], x[k]);
-            else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[k][e] = 0.f;
-            }
+            nx[k].get(x[k]);
+            if (BWD) ng[k].get(dz[k]);
 #pragma unroll
             for (int e = 0; e < V; ++e) sum += x[k][e];
         }
+        if (b0 + step < a.B) fetch(b + step);
         const float inv_n = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
         float mean, rstd;
         if constexpr (!BWD) {
@@ -141,15 +155,9 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
         } else {
             mean = on ? a.mean[b * a.G + g] : 0.f;
             rstd = on ? a.rstd[b * a.G + g] : 0.f;
-            float dz[NV][V];
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (row[k] < len) load_v<DT, V>(a.dy, b * a.db_ + (int64_t)row[k] * a.dt_ + ch[k], dz[k]);
-                else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) dz[k][e] = 0.f;
-                }
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float xh = row[k] < len ? (x[k][e] - mean) * rstd : 0.f;
@@ -199,6 +207,159 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
     }
 }
 
+// ================================================================================ whole form ====
+// A workgroup holds all T rows of `gpw` groups of an item: lv vectors of a row side by side, threads / lv rows at once, NV vectors to a thread.  A vector lies in one
+// group (n is a multiple of V).
+struct WholePlan { int threads, gpw, lv, rows, blocks; };
+
+// sums over the workgroup of one value a thread, group by group: red[threads], result in out[gpw]
+__device__ __forceinline__ void whole_sums(float v, float* red, float* out, const WholePlan& q, int nv) {
+    red[threadIdx.x] = v;
+    __syncthreads();
+    const int lane = threadIdx.x & 63, waves = q.threads >> 6, count = q.rows * nv;
+    for (int g = threadIdx.x >> 6; g < q.gpw; g += waves) {
+        float t = 0.f;
+        for (int i = lane; i < count; i += 64) { const int r = i / nv; t += red[r * q.lv + g * nv + i - r * nv]; }
+        t = lanes_sum(t, 64);
+        if (lane == 0) out[g] = t;
+    }
+    __syncthreads();
+}
+
+template <int DT, int V, int NV, bool BWD>
+__global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
+    extern __shared__ float lds[];                 // threads | 2 gpw; backward: rows * channels instead of threads, and 2 x channels
+    // workgroups go to the eight XCDs by turns: those that share an item's lines get the same one
+    const int per = gridDim.x >> 3, id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const int b = id / q.blocks, blk = id - b * q.blocks;
+    if (b >= a.B) return;
+    const int r0 = threadIdx.x / q.lv, v = threadIdx.x - r0 * q.lv;
+    const int nv = a.n / V, g0 = blk * q.gpw, gn = min(q.gpw, a.G - g0), gl = v / nv, g = g0 + gl;
+    const bool on = r0 < q.rows && gl < gn;
+    const int len = live_rows(a, b), c = g0 * a.n + v * V;
+    const float inv_n = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
+    Packed<DT, V> x[NV], d[BWD ? NV : 1];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int r = r0 + k * q.rows;
+        x[k].clear();
+        if (BWD) d[k].clear();
+        if (on && r < len) {
+            x[k].load(a.x, b * a.xb + (int64_t)r * a.xt + c);
+            if (BWD) d[k].load(a.dy, b * a.db_ + (int64_t)r * a.dt_ + c);
+        }
+    }
+    float w[V], bias[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { w[e] = on && a.w ? a.w[c + e] : 1.f; bias[e] = on && a.bias ? a.bias[c + e] : 0.f; }
+    if constexpr (!BWD) {
+        float* sums = lds + q.threads;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float f[V];
+            x[k].get(f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += f[e];
+        }
+        whole_sums(s, lds, sums, q, nv);
+        const float mean = sums[min(gl, q.gpw - 1)] * inv_n;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float f[V];
+            x[k].get(f);
+            if (r0 + k * q.rows < len) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += (f[e] - mean) * (f[e] - mean);
+            }
+        }
+        whole_sums(on ? s : 0.f, lds, sums + q.gpw, q, nv);
+        const float rstd = rsqrtf(sums[q.gpw + min(gl, q.gpw - 1)] * inv_n + a.eps);
+        if (on && r0 == 0 && v == gl * nv) { a.mean[(int64_t)b * a.G + g] = mean; a.rstd[(int64_t)b * a.G + g] = rstd; }
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int r = r0 + k * q.rows;
+            if (!on || r >= a.T) continue;
+            float f[V];
+            x[k].get(f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = (f[e] - mean) * rstd * w[e] + bias[e];
+            activate<V>(f, a.act, a.slope);
+            if (r >= len) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] = 0.f;
+            }
+            store_v<DT, V>(a.out, b * a.ob + (int64_t)r * a.ot + c, f);
+        }
+    } else {
+        const int cw = q.lv * V;                   // channels of the workgroup
+        float* ch = lds + q.rows * cw;             // [2][channels]: sums of dz, dz xh
+        float* sums = ch + 2 * cw;                 // [2][gpw]
+        const float mean = on ? a.mean[(int64_t)b * a.G + g] : 0.f, rstd = on ? a.rstd[(int64_t)b * a.G + g] : 0.f;
+        float s1[V], s2[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (r0 + k * q.rows >= len) continue;
+            float f[V], h[V];
+            x[k].get(f); d[k].get(h);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (f[e] - mean) * rstd, dz = h[e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
+                s1[e] += dz; s2[e] += dz * xh;
+            }
+        }
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            if (r0 < q.rows) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) lds[r0 * cw + v * V + e] = which ? s2[e] : s1[e];
+            }
+            __syncthreads();
+            // a few threads to a channel, each a share of the rows; neighbours in a run of lanes add up
+            int run = 1;
+            while (run < 16 && run * 2 * cw <= q.threads) run *= 2;
+            for (int c0 = 0; c0 < cw; c0 += q.threads / run) {
+                const int cc = c0 + threadIdx.x / run;
+                float t = 0.f;
+                if (cc < cw)
+                    for (int r = threadIdx.x & (run - 1); r < q.rows; r += run) t += lds[r * cw + cc];
+                t = lanes_sum(t, run);
+                if (cc < cw && (threadIdx.x & (run - 1)) == 0) {
+                    ch[which * cw + cc] = t;
+                    if (cc < gn * a.n) a.part[((int64_t)b * 2 + which) * a.C + g0 * a.n + cc] = t;
+                }
+            }
+            __syncthreads();
+        }
+        const int lane = threadIdx.x & 63, waves = q.threads >> 6;
+        for (int i = threadIdx.x >> 6; i < 2 * gn; i += waves) {
+            const int which = i / gn, gg = i - which * gn;
+            float t = 0.f;
+            for (int cc = gg * a.n + lane; cc < (gg + 1) * a.n; cc += 64) t += (a.w ? a.w[g0 * a.n + cc] : 1.f) * ch[which * cw + cc];
+            t = lanes_sum(t, 64);
+            if (lane == 0) sums[which * q.gpw + gg] = t * inv_n;
+        }
+        __syncthreads();
+        const float k1 = sums[min(gl, q.gpw - 1)], k2 = sums[q.gpw + min(gl, q.gpw - 1)];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int r = r0 + k * q.rows;
+            if (!on || r >= a.T) continue;
+            float f[V], h[V];
+            x[k].get(f); d[k].get(h);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (f[e] - mean) * rstd, dz = h[e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
+                f[e] = r < len ? rstd * (w[e] * dz - k1 - xh * k2) : 0.f;
+            }
+            store_v<DT, V>(a.out, b * a.ob + (int64_t)r * a.ot + c, f);
+        }
+    }
+}
+
 // ================================================================================ tile form ====
 // A thread owns one vector of V channels and every `step`-th row of its chunk; lc = C / V vectors side by side, step = blockDim.x / lc rows at once.
 constexpr int NR = 8;      // rows of a thread in one register tile
@@ -234,8 +395,8 @@ __device__ __forceinline__ void group_sums(const float* red, float* out, const T
 __device__ __forceinline__ int run_of(int n) { int r = 1; while (r < n && r < 64) r <<= 1; return r; }
 
 // statistics of one chunk: part[(b * chunks + chunk) * G + g] = (mean, sum of squared deviations)
-template <int DT, int V>
-__global__ __launch_bounds__(1024) void tile_stats_kernel(Args a) {
+template <int DT, int V, int NT>
+__global__ __launch_bounds__(NT) void tile_stats_kernel(Args a) {
     extern __shared__ float lds[];
     const Tile t(a.C, V);
     float* red = lds;                          // step * C
@@ -303,8 +464,8 @@ __global__ __launch_bounds__(1024) void tile_stats_kernel(Args a) {
 }
 
 // joins the chunks' statistics (every workgroup for itself: a few hundred bytes), then normalises its chunk
-template <int DT, int V>
-__global__ __launch_bounds__(1024) void tile_apply_kernel(Args a) {
+template <int DT, int V, int NT>
+__global__ __launch_bounds__(NT) void tile_apply_kernel(Args a) {
     extern __shared__ float lds[];
     float* mean = lds;
     float* rstd = lds + a.G;
@@ -370,8 +531,8 @@ __global__ __launch_bounds__(1024) void tile_apply_kernel(Args a) {
 }
 
 // sums of dz and dz xh of one chunk: part[(b * chunks + chunk) * 2 C + which * C + c]
-template <int DT, int V>
-__global__ __launch_bounds__(1024) void tile_dsum_kernel(Args a) {
+template <int DT, int V, int NT>
+__global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
     extern __shared__ float red[];
     const Tile t(a.C, V);
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b);
@@ -429,11 +590,27 @@ __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ pa
     __shared__ float red[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), slot = threadIdx.x >> 5, which = blockIdx.y;
     float total = 0.f;
-    if (c < C)
+    if (c < C && !item) {
+        const float* at = part + (int64_t)which * C + c;
+        const int rows = items * per_item;
+        float t[4] = {};
+        int r = slot;
+        for (; r + 96 < rows; r += 128)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] += at[(int64_t)(r + 32 * k) * 2 * C];
+        for (; r < rows; r += 32) t[0] += at[(int64_t)r * 2 * C];
+        total = (t[0] + t[1]) + (t[2] + t[3]);
+    } else if (c < C)
         for (int b = slot; b < items; b += 32) {
-            float v = 0.f;
-            for (int k = 0; k < per_item; ++k) v += part[(((int64_t)b * per_item + k) * 2 + which) * C + c];
-            if (item) item[((int64_t)b * 2 + which) * C + c] = v;
+            const float* at = part + ((int64_t)b * per_item * 2 + which) * C + c;
+            float t[4] = {};
+            int k = 0;
+            for (; k + 3 < per_item; k += 4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[i] += at[(int64_t)(k + i) * 2 * C];
+            for (; k < per_item; ++k) t[0] += at[(int64_t)k * 2 * C];
+            const float v = (t[0] + t[1]) + (t[2] + t[3]);
+            item[((int64_t)b * 2 + which) * C + c] = v;
             total += v;
         }
     float* out = which ? dw : db;
@@ -446,8 +623,8 @@ __global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ pa
     }
 }
 
-template <int DT, int V>
-__global__ __launch_bounds__(1024) void tile_dx_kernel(Args a) {
+template <int DT, int V, int NT>
+__global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
     extern __shared__ float lds[];
     float* m1 = lds;                       // means of w dz and w dz xh of each group
     float* m2 = lds + a.G;
@@ -503,23 +680,26 @@ __global__ __launch_bounds__(1024) void tile_dx_kernel(Args a) {
 }
 
 // -------------------------------------------------------------------------------- plan ----
+enum { SLAB, WHOLE, TILE };
 struct Plan {
     int v;                                  // elements of a vector: 16 bytes, or one
-    bool slab; int nv; SlabPlan s; int slab_wgs;
+    int form, nv;                           // vectors of a thread: slab and whole forms
+    SlabPlan s; int slab_wgs;
+    WholePlan w; int whole_wgs;
     int threads, rows_per_chunk, chunks;
 };
 
 int pow2_at_least(int64_t x) { int r = 1; while (r < x) r <<= 1; return r; }
 
-bool make_plan(const xva_group_norm_args* p, bool vec, Plan* out) {
+bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
     Plan& q = *out;
     const int wide = p->dtype == 0 ? 4 : 8, n = p->C / p->G;
     q.v = vec && p->C % wide == 0 ? wide : 1;
     // slab form: a (item, group) slab of whole vectors (of one value, where 16 bytes would straddle groups) within 64 lanes x 4 vectors
     const int sv = n % q.v == 0 ? q.v : 1;
     const int64_t vecs = (int64_t)p->T * (n / sv);
-    q.slab = vecs <= 256;
-    if (q.slab) {
+    if (vecs <= 256) {
+        q.form = SLAB;
         q.v = sv;
         q.nv = vecs <= 64 ? 1 : (vecs <= 128 ? 2 : 4);
         q.s.lpg = pow2_at_least((vecs + q.nv - 1) / q.nv);
@@ -527,13 +707,38 @@ bool make_plan(const xva_group_norm_args* p, bool vec, Plan* out) {
         q.s.gpb = p->G < slots ? p->G : slots;
         q.s.ipb = slots / q.s.gpb;
         q.s.gy = (p->G + q.s.gpb - 1) / q.s.gpb;
-        // one workgroup for every `ipb` items up to eight to a CU; the backward's partial rows are as many
-        const int64_t want = (p->B + q.s.ipb - 1) / q.s.ipb;
-        int64_t most = 2048 / q.s.gy;
-        if (most < 64) most = 64;
+        // two turns of items to a workgroup, so that one's loads are under way while the other is computed; backward no more than four workgroups to a CU, since
+        // each leaves a partial row of dw / dbias
+        const int64_t want = ((int64_t)p->B + q.s.ipb - 1) / q.s.ipb;
+        int64_t most = bwd ? 1024 / q.s.gy : (want + 1) / 2;
+        if (bwd && most < 64) most = 64;
+        if (most < 256 / q.s.gy) most = 256 / q.s.gy;
+        if (most < 1) most = 1;
         q.slab_wgs = (int)(want < most ? want : most);
         return true;
     }
+    // whole form: groups of one item within the registers of 512 threads (16 packed vectors to a thread, 12 of x and 12 of dy backward).  As many groups as make
+    // 64 bytes of a row, more where workgroups abound.
+    if (sv == q.v && q.v > 1) {
+        const int nv = n / q.v, cap = 512 * (bwd ? 12 : 16);
+        int gpw = (4 + nv - 1) / nv;
+        if (gpw > p->G) gpw = p->G;
+        while (gpw > 1 && (int64_t)p->T * nv * gpw > cap) --gpw;
+        while (gpw * 2 <= p->G && gpw * 2 * nv <= 16 && (int64_t)p->T * nv * gpw * 2 <= cap && (int64_t)p->B * ((p->G + 2 * gpw - 1) / (2 * gpw)) >= 512) gpw *= 2;
+        const int lv = gpw * nv;
+        if (lv <= 512 && (int64_t)p->T * nv * gpw <= (int64_t)(512 / lv) * lv * (bwd ? 12 : 16)) {
+            q.form = WHOLE;
+            q.w.gpw = gpw; q.w.lv = lv;
+            q.w.threads = (int64_t)p->T * lv <= 4 * 256 && lv <= 256 ? 256 : 512;
+            q.w.rows = q.w.threads / lv;
+            q.w.blocks = (p->G + gpw - 1) / gpw;
+            const int each = (p->T + q.w.rows - 1) / q.w.rows;
+            q.nv = each <= 4 ? 4 : (each <= 8 ? 8 : (each <= 12 ? 12 : 16));
+            q.whole_wgs = (int)(((int64_t)p->B * q.w.blocks + 7) / 8 * 8);
+            if (each <= (bwd ? 12 : 16)) return true;
+        }
+    }
+    q.form = TILE;
     const int lc = p->C / q.v;
     if (lc > 1024 || p->G > 2048) return false;        // (a row in one workgroup, its groups in the LDS)
     q.threads = lc <= 256 ? 256 : (lc + 63) / 64 * 64;
@@ -583,9 +788,10 @@ int64_t workspace(const xva_group_norm_args* p, bool bwd) {
     int64_t most = 0;
     for (int vec = 0; vec < 2; ++vec) {
         Plan q = {};
-        if (!make_plan(p, vec != 0, &q)) continue;
+        if (!make_plan(p, vec != 0, bwd, &q)) continue;
         int64_t f;
-        if (q.slab) f = bwd ? (int64_t)q.slab_wgs * 2 * p->C : 0;
+        if (q.form == WHOLE) f = bwd ? (int64_t)p->B * 2 * p->C : 0;
+        else if (q.form == SLAB) f = bwd ? (int64_t)q.slab_wgs * 2 * p->C : 0;
         else f = bwd ? (int64_t)p->B * (q.chunks + 1) * 2 * p->C : (int64_t)p->B * q.chunks * 2 * p->G;
         if (f > most) most = f;
     }
@@ -602,13 +808,33 @@ template <int DT, int V, bool BWD> int slab_launch(const Args& a, const Plan& q,
     return XVA_OK;
 }
 
+template <int DT, int V, bool BWD> int whole_launch(const Args& a, const Plan& q, hipStream_t st) {
+    if constexpr (V == 1) { return XVA_ERR_ARG; }
+    else {
+        const int cw = q.w.lv * V;
+        const size_t lds = (BWD ? (size_t)q.w.rows * cw + 2 * cw : (size_t)q.w.threads) * 4 + 2 * q.w.gpw * 4;
+        const dim3 grid(q.whole_wgs);
+        switch (q.nv) {
+            case 4: whole_kernel<DT, V, 4, BWD><<<grid, q.w.threads, lds, st>>>(a, q.w); break;
+            case 8: whole_kernel<DT, V, 8, BWD><<<grid, q.w.threads, lds, st>>>(a, q.w); break;
+            case 12: whole_kernel<DT, V, 12, BWD><<<grid, q.w.threads, lds, st>>>(a, q.w); break;
+            default: if constexpr (!BWD) whole_kernel<DT, V, 16, BWD><<<grid, q.w.threads, lds, st>>>(a, q.w);
+        }
+        XVA_LAUNCH_CHECK();
+        return XVA_OK;
+    }
+}
+
 template <int DT, int V> int forward(Args& a, const Plan& q, hipStream_t st) {
-    if (q.slab) return slab_launch<DT, V, false>(a, q, st);
+    if (q.form == WHOLE) return whole_launch<DT, V, false>(a, q, st);
+    if (q.form == SLAB) return slab_launch<DT, V, false>(a, q, st);
     const dim3 grid((unsigned)(a.B * q.chunks));
     const int step = q.threads / (a.C / V);
-    tile_stats_kernel<DT, V><<<grid, q.threads, ((size_t)step * a.C + 3 * a.G) * 4, st>>>(a);
+    if (q.threads <= 256) tile_stats_kernel<DT, V, 256><<<grid, q.threads, ((size_t)step * a.C + 3 * a.G) * 4, st>>>(a);
+    else tile_stats_kernel<DT, V, 1024><<<grid, q.threads, ((size_t)step * a.C + 3 * a.G) * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
-    tile_apply_kernel<DT, V><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    if (q.threads <= 256) tile_apply_kernel<DT, V, 256><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    else tile_apply_kernel<DT, V, 1024><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
@@ -620,17 +846,23 @@ int join(const Args& a, int items, int per_item, hipStream_t st) {
 }
 
 template <int DT, int V> int backward(Args& a, const Plan& q, hipStream_t st) {
-    if (q.slab) {
+    if (q.form == WHOLE) {
+        XVA_TRY((whole_launch<DT, V, true>(a, q, st)));
+        return a.dw || a.db ? join(a, a.B, 1, st) : XVA_OK;
+    }
+    if (q.form == SLAB) {
         XVA_TRY((slab_launch<DT, V, true>(a, q, st)));
         return a.dw || a.db ? join(a, q.slab_wgs, 1, st) : XVA_OK;
     }
     const dim3 grid((unsigned)(a.B * q.chunks));
     const int step = q.threads / (a.C / V);
     a.item = a.part + (int64_t)a.B * q.chunks * 2 * a.C;
-    tile_dsum_kernel<DT, V><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
+    if (q.threads <= 256) tile_dsum_kernel<DT, V, 256><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
+    else tile_dsum_kernel<DT, V, 1024><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
     XVA_TRY(join(a, a.B, q.chunks, st));
-    tile_dx_kernel<DT, V><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    if (q.threads <= 256) tile_dx_kernel<DT, V, 256><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
+    else tile_dx_kernel<DT, V, 1024><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
@@ -640,8 +872,8 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     XVA_CHECK_ARG(!bwd || p->dy || p->B == 0 || p->T == 0, "%s: null gradient", who);
     hipStream_t st = (hipStream_t)stream;
     Plan q = {};
-    XVA_CHECK_ARG(make_plan(p, aligned(p, bwd), &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
-    XVA_CHECK_ARG(q.slab || (int64_t)p->B * q.chunks < (1ll << 31), "%s: %d items of %d rows", who, p->B, p->T);
+    XVA_CHECK_ARG(make_plan(p, aligned(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
+    XVA_CHECK_ARG(q.form != TILE || (int64_t)p->B * q.chunks < (1ll << 31), "%s: %d items of %d rows", who, p->B, p->T);
     if (ws_bytes < workspace(p, bwd)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)workspace(p, bwd)); return XVA_ERR_WS; }
     if (p->B == 0 || p->T == 0) {
         if (bwd) {

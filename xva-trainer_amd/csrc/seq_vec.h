@@ -55,7 +55,43 @@ template <int DT, int V> __device__ __forceinline__ void store_v(void* base, int
     }
 }
 
-// a launch over element type DT and vector width V, both known at run time
-template <int DT> struct Elem { static constexpr int size = DT == 0 ? 4 : 2, wide = 16 / size; };   // wide: elements of a 16-byte access
 inline int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// V elements as they lie in memory (1 element, or 16 bytes), kept packed until they are needed
+template <int DT, int V> struct Packed {
+    static_assert(V == 1 || V == (DT == 0 ? 4 : 8), "one element or 16 bytes");
+    typedef typename std::conditional<V != 1, u32x4, typename std::conditional<DT == 0, uint32_t, uint16_t>::type>::type T;
+    T v;
+    __device__ __forceinline__ void load(const void* base, int64_t off) {
+        v = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off * (DT == 0 ? 4 : 2));
+    }
+    __device__ __forceinline__ void clear() { if constexpr (V == 1) v = 0; else v = (u32x4){0, 0, 0, 0}; }
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+        if constexpr (V == 1) {
+            if constexpr (DT == 0) f[0] = __uint_as_float(v); else f[0] = xva_glds::ld16<DT == 2>(&v, 0);
+        } else if constexpr (DT == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) unpack2<DT == 2>(v[e], f[2 * e], f[2 * e + 1]);
+        }
+    }
+};
+
+// sum over aligned runs of `width` (a power of two, the same in the wave) lanes, in every lane; all lanes active.  Within 16 lanes by DPP: the partner is another
+// one of the other half, whose lanes all hold that half's sum by then.
+__device__ __forceinline__ float lanes_sum(float v, int width) {
+#define XVA_DPP_ADD(ctrl) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xf, 0xf, true))
+    if (width >= 2) XVA_DPP_ADD(0xB1);            // quad_perm 1 0 3 2
+    if (width >= 4) XVA_DPP_ADD(0x4E);            // quad_perm 2 3 0 1
+    if (width >= 8) XVA_DPP_ADD(0x141);           // row_half_mirror
+    if (width >= 16) XVA_DPP_ADD(0x140);          // row_mirror
+#undef XVA_DPP_ADD
+    if (width >= 32) v += __shfl_xor(v, 16, 64);
+    if (width >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
 }   // namespace xva_seq
