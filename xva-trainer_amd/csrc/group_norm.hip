@@ -43,28 +43,38 @@ struct Args {
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 // (off by a few 2^-24 of 1, as z itself is)
 __device__ __forceinline__ float tanh_(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * z)); }
-template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act, float slope) {
+// (one switch to V values: a branch of every value costs more than the activations)
+template <int V, class F> __device__ __forceinline__ void each(float (&z)[V], F f) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const float v = z[e];
-        switch (act) {
-            case RELU: z[e] = v > 0.f ? v : (v != v ? v : 0.f); break;
-            case LRELU: z[e] = v > 0.f ? v : slope * v; break;
-            case TANH: z[e] = tanh_(v); break;
-            case SILU: z[e] = v * sigmoid(v); break;
-            case GELU: z[e] = 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); break;
-            default: break;
-        }
+    for (int e = 0; e < V; ++e) z[e] = f(z[e]);
+}
+template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act, float slope) {
+    switch (act) {
+        case RELU: each<V>(z, [](float v) { return v > 0.f ? v : (v != v ? v : 0.f); }); break;
+        case LRELU: each<V>(z, [=](float v) { return v > 0.f ? v : slope * v; }); break;
+        case TANH: each<V>(z, [](float v) { return tanh_(v); }); break;
+        case SILU: each<V>(z, [](float v) { return v * sigmoid(v); }); break;
+        case GELU: each<V>(z, [](float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); }); break;
+        default: break;
     }
 }
-__device__ __forceinline__ float slope_of(float v, int act, float slope) {
+// z -> act'(z)
+template <int V> __device__ __forceinline__ void slopes(float (&z)[V], int act, float slope) {
     switch (act) {
-        case RELU: return v > 0.f ? 1.f : 0.f;
-        case LRELU: return v > 0.f ? 1.f : slope;
-        case TANH: { const float t = tanh_(v); return 1.f - t * t; }
-        case SILU: { const float s = sigmoid(v); return s + s * v * (1.f - s); }
-        case GELU: return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * __expf(-0.5f * v * v);
-        default: return 1.f;
+        case RELU: each<V>(z, [](float v) { return v > 0.f ? 1.f : 0.f; }); break;
+        case LRELU: each<V>(z, [=](float v) { return v > 0.f ? 1.f : slope; }); break;
+        case TANH: each<V>(z, [](float v) { const float t = tanh_(v); return 1.f - t * t; }); break;
+        case SILU: each<V>(z, [](float v) { const float s = sigmoid(v); return s + s * v * (1.f - s); }); break;
+        case GELU: each<V>(z, [](float v) { return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * __expf(-0.5f * v * v); }); break;
+        default: each<V>(z, [](float) { return 1.f; });
+    }
+}
+// V values of a weight vector (16-byte aligned where V > 1), `none` where there is none
+template <int V> __device__ __forceinline__ void load_w(const float* w, int c, float none, float (&f)[V]) {
+    if (w) load_v<0, V>(w, c, f);
+    else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = none;
     }
 }
 __device__ __forceinline__ int live_rows(const Args& a, int b) {
@@ -90,12 +100,10 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
         const int j = k * s.lpg + lane;
         row[k] = j < vecs ? j / nv : a.T;                  // a.T: no such row
         ch[k] = min(g, a.G - 1) * a.n + (j < vecs ? (j % nv) * V : 0);
+        load_w<V>(a.w, ch[k], 1.f, w[k]);
+        load_w<V>(a.bias, ch[k], 0.f, bias[k]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            w[k][e] = a.w ? a.w[ch[k] + e] : 1.f;
-            bias[k][e] = a.bias ? a.bias[ch[k] + e] : 0.f;
-            sw[k][e] = sb[k][e] = 0.f;
-        }
+        for (int e = 0; e < V; ++e) sw[k][e] = sb[k][e] = 0.f;
     }
     // this item's values, and the next one's on their way
     Packed<DT, V> nx[NV], ng[NV];
@@ -158,11 +166,16 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
             float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
+                float z[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float xh = row[k] < len ? (x[k][e] - mean) * rstd : 0.f;
-                    const float d = dz[k][e] * slope_of(xh * w[k][e] + bias[k][e], a.act, a.slope);
-                    x[k][e] = xh;
+                    x[k][e] = row[k] < len ? (x[k][e] - mean) * rstd : 0.f;
+                    z[e] = x[k][e] * w[k][e] + bias[k][e];
+                }
+                slopes<V>(z, a.act, a.slope);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = x[k][e], d = dz[k][e] * z[e];
                     sw[k][e] += d * xh; sb[k][e] += d;
                     dz[k][e] = d * w[k][e];
                     s1 += dz[k][e]; s2 += dz[k][e] * xh;
@@ -250,8 +263,8 @@ __global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
         }
     }
     float w[V], bias[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) { w[e] = on && a.w ? a.w[c + e] : 1.f; bias[e] = on && a.bias ? a.bias[c + e] : 0.f; }
+    load_w<V>(a.w, on ? c : 0, 1.f, w);
+    load_w<V>(a.bias, on ? c : 0, 0.f, bias);
     if constexpr (!BWD) {
         float* sums = lds + q.threads;
         float s = 0.f;
@@ -303,13 +316,13 @@ __global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             if (r0 + k * q.rows >= len) continue;
-            float f[V], h[V];
+            float f[V], h[V], z[V];
             x[k].get(f); d[k].get(h);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float xh = (f[e] - mean) * rstd, dz = h[e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
-                s1[e] += dz; s2[e] += dz * xh;
-            }
+            for (int e = 0; e < V; ++e) { f[e] = (f[e] - mean) * rstd; z[e] = f[e] * w[e] + bias[e]; }
+            slopes<V>(z, a.act, a.slope);
+#pragma unroll
+            for (int e = 0; e < V; ++e) { const float dz = h[e] * z[e]; s1[e] += dz; s2[e] += dz * f[e]; }
         }
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -348,13 +361,13 @@ __global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
         for (int k = 0; k < NV; ++k) {
             const int r = r0 + k * q.rows;
             if (!on || r >= a.T) continue;
-            float f[V], h[V];
+            float f[V], h[V], z[V];
             x[k].get(f); d[k].get(h);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float xh = (f[e] - mean) * rstd, dz = h[e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
-                f[e] = r < len ? rstd * (w[e] * dz - k1 - xh * k2) : 0.f;
-            }
+            for (int e = 0; e < V; ++e) { f[e] = (f[e] - mean) * rstd; z[e] = f[e] * w[e] + bias[e]; }
+            slopes<V>(z, a.act, a.slope);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = r < len ? rstd * (w[e] * (h[e] * z[e]) - k1 - f[e] * k2) : 0.f;
             store_v<DT, V>(a.out, b * a.ob + (int64_t)r * a.ot + c, f);
         }
     }
@@ -494,12 +507,13 @@ __global__ __launch_bounds__(NT) void tile_apply_kernel(Args a) {
     __syncthreads();
     if (!t.on) return;
     float mu[V], w[V], bias[V];
+    load_w<V>(a.w, t.v * V, 1.f, w);
+    load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int c = t.v * V + e, g = c / a.n;
         mu[e] = mean[g];
-        w[e] = rstd[g] * (a.w ? a.w[c] : 1.f);
-        bias[e] = a.bias ? a.bias[c] : 0.f;
+        w[e] *= rstd[g];
     }
     const int64_t xo = (int64_t)b * a.xb + t.v * V, oo = (int64_t)b * a.ob + t.v * V;
     int r = first + t.r;
@@ -542,11 +556,12 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
     for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
     if (t.on) {
         float mu[V], rs[V], w[V], bias[V];
+        load_w<V>(a.w, t.v * V, 1.f, w);
+        load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const int c = t.v * V + e, g = c / a.n;
             mu[e] = a.mean[(int64_t)b * a.G + g]; rs[e] = a.rstd[(int64_t)b * a.G + g];
-            w[e] = a.w ? a.w[c] : 1.f; bias[e] = a.bias ? a.bias[c] : 0.f;
         }
         const int64_t xo = (int64_t)b * a.xb + t.v * V, po = (int64_t)b * a.db_ + t.v * V;
         for (int r0 = first + t.r; r0 < end; r0 += 4 * t.step) {
@@ -561,12 +576,14 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k) {
+                float z[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float xh = (f[k][e] - mu[e]) * rs[e], dz = d[k][e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
-                    s1[e] += dz; s2[e] += r0 + k * t.step < end ? dz * xh : 0.f;
-                }
+                for (int e = 0; e < V; ++e) { f[k][e] = (f[k][e] - mu[e]) * rs[e]; z[e] = f[k][e] * w[e] + bias[e]; }
+                slopes<V>(z, a.act, a.slope);
+#pragma unroll
+                for (int e = 0; e < V; ++e) { const float dz = d[k][e] * z[e]; s1[e] += dz; s2[e] += r0 + k * t.step < end ? dz * f[k][e] : 0.f; }
+            }
         }
     }
     float* out = a.part + (int64_t)blockIdx.x * 2 * a.C;
@@ -648,11 +665,12 @@ __global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
     __syncthreads();
     if (!t.on) return;
     float mu[V], rs[V], w[V], bias[V], k1[V], k2[V];
+    load_w<V>(a.w, t.v * V, 1.f, w);
+    load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int c = t.v * V + e, g = c / a.n;
         mu[e] = a.mean[(int64_t)b * a.G + g]; rs[e] = a.rstd[(int64_t)b * a.G + g];
-        w[e] = a.w ? a.w[c] : 1.f; bias[e] = a.bias ? a.bias[c] : 0.f;
         k1[e] = m1[g]; k2[e] = m2[g];
     }
     const int64_t xo = (int64_t)b * a.xb + t.v * V, po = (int64_t)b * a.db_ + t.v * V, oo = (int64_t)b * a.ob + t.v * V;
@@ -667,12 +685,16 @@ __global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
         for (int k = 0; k < 2; ++k) {
             const int r = r0 + k * t.step;
             if (r >= end) continue;
+            if (r < len) {
+                float z[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (r < len) {
-                    const float xh = (f[k][e] - mu[e]) * rs[e], dz = d[k][e] * slope_of(xh * w[e] + bias[e], a.act, a.slope);
-                    f[k][e] = rs[e] * (w[e] * dz - k1[e] - xh * k2[e]);
-                } else f[k][e] = 0.f;
+                for (int e = 0; e < V; ++e) { f[k][e] = (f[k][e] - mu[e]) * rs[e]; z[e] = f[k][e] * w[e] + bias[e]; }
+                slopes<V>(z, a.act, a.slope);
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[k][e] = rs[e] * (w[e] * (d[k][e] * z[e]) - k1[e] - f[k][e] * k2[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[k][e] = 0.f;
             }
             store_v<DT, V>(a.out, oo + (int64_t)r * a.ot, f[k]);
         }
@@ -707,13 +729,11 @@ bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
         q.s.gpb = p->G < slots ? p->G : slots;
         q.s.ipb = slots / q.s.gpb;
         q.s.gy = (p->G + q.s.gpb - 1) / q.s.gpb;
-        // two turns of items to a workgroup, so that one's loads are under way while the other is computed; backward no more than four workgroups to a CU, since
-        // each leaves a partial row of dw / dbias
+        // several turns of items to a workgroup: its weights are loaded once, and one item's loads are under way while another is computed.  Eight workgroups to a
+        // CU, four backward, where each leaves a partial row of dw / dbias.
         const int64_t want = ((int64_t)p->B + q.s.ipb - 1) / q.s.ipb;
-        int64_t most = bwd ? 1024 / q.s.gy : (want + 1) / 2;
-        if (bwd && most < 64) most = 64;
-        if (most < 256 / q.s.gy) most = 256 / q.s.gy;
-        if (most < 1) most = 1;
+        int64_t most = (bwd ? 1024 : 2048) / q.s.gy;
+        if (most < 64) most = 64;
         q.slab_wgs = (int)(want < most ? want : most);
         return true;
     }
@@ -758,7 +778,7 @@ bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
 bool aligned(const xva_group_norm_args* p, bool bwd) {
     const int wide = p->dtype == 0 ? 4 : 8;
     int64_t all = p->x_stride[0] | p->x_stride[1] | p->out_stride[0] | p->out_stride[1];
-    uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->out;
+    uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->out | (uintptr_t)p->weight | (uintptr_t)p->bias;
     if (bwd) { all |= p->dy_stride[0] | p->dy_stride[1]; ptrs |= (uintptr_t)p->dy; }
     return all % wide == 0 && ptrs % 16 == 0;
 }
