@@ -7,6 +7,7 @@ import subprocess
 import pytest
 import torch
 
+from seq_util import DiffAttentionArgs, GroupNormArgs, RecurrenceArgs, RotaryArgs, entry, i64
 from xva_trainer_amd import _lib, seq_ops as S
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -41,8 +42,8 @@ def test_host_tensors_are_refused():
             call()
 
 
-STRUCTS = {"xva_rotary_args": S._RotaryArgs, "xva_group_norm_args": S._GroupNormArgs, "xva_recurrence_args": S._RecurrenceArgs,
-           "xva_diff_attention_args": S._DiffAttentionArgs}
+STRUCTS = {"xva_rotary_args": RotaryArgs, "xva_group_norm_args": GroupNormArgs, "xva_recurrence_args": RecurrenceArgs,
+           "xva_diff_attention_args": DiffAttentionArgs}
 
 
 def test_structs_match_the_header(tmp_path):
@@ -74,24 +75,24 @@ A = 1 << 20        # an address for arguments that are refused before anything r
 
 def _diff(**kw):
     base = dict(q=A, k=A, v=A, lam=A, out=A, dtype=1, B=1, Tq=4, Tk=4, H=2, Hk=1, d=16, causal=0, scale=0.25)
-    return S._DiffAttentionArgs(**{**base, **kw})
+    return DiffAttentionArgs(**{**base, **kw})
 
 
 @pytest.mark.parametrize("bad,says", [(dict(q=None), "null"), (dict(dtype=0), "dtype"), (dict(d=12), "head width"), (dict(d=72), "head width"), (dict(Hk=0), "Hk"),
                                       (dict(H=3, Hk=2), "Hk"), (dict(B=-1), "B -1"), (dict(scale=0.0), "scale"), (dict(q=A + 2), "aligned"),
                                       (dict(k_stride1=4), "strides"), (dict(out=None), "null"), (dict(lse=A), "null"), (dict(Tq=1 << 30), "Tq")])
 def test_diff_attention_refuses(bad, says):
-    assert _lib.lib.xva_diff_attention_fwd(C.byref(_diff(**bad)), None, 0, None) < 0
+    assert entry("xva_diff_attention_fwd")(C.byref(_diff(**bad)), None, 0, None) < 0
     assert says in _lib.lib.xva_last_error().decode()
 
 
 def test_diff_attention_backward_refuses_a_small_workspace():
     a = _diff(dout=A, maps=A, lse=A, dq=A, dk=A, dv=A, dlam=A)
-    need = _lib.lib.xva_diff_attention_workspace_bytes(C.byref(a), 1)
+    need = entry("xva_diff_attention_workspace_bytes", i64)(C.byref(a), 1)
     assert need > 0
-    assert _lib.lib.xva_diff_attention_bwd(C.byref(a), A, need - 1, None) == -3
-    assert _lib.lib.xva_diff_attention_bwd(C.byref(a), None, need, None) == -3
-    assert _lib.lib.xva_diff_attention_bwd(C.byref(_diff()), A, need, None) < 0
+    assert entry("xva_diff_attention_bwd")(C.byref(a), A, need - 1, None) == -3
+    assert entry("xva_diff_attention_bwd")(C.byref(a), None, need, None) == -3
+    assert entry("xva_diff_attention_bwd")(C.byref(_diff()), A, need, None) < 0
 
 
 @pytest.mark.parametrize("bad,says", [(dict(q=None), "null"), (dict(turns=None), "null"), (dict(dtype=3), "dtype"), (dict(rd=3), "rotary width"), (dict(rd=34), "rotary width"),
@@ -99,7 +100,7 @@ def test_diff_attention_backward_refuses_a_small_workspace():
                                       (dict(B=1 << 20, T=1 << 12), "tokens"), (dict(H=0), "H 0")])
 def test_rotary_refuses(bad, says):
     base = dict(q=A, k=A, q_out=2 * A, k_out=2 * A, turns=A, dtype=0, B=1, T=2, H=2, Hk=1, D=32, rd=32, gain=1.0, q_stride0=64)
-    assert _lib.lib.xva_rotary(C.byref(S._RotaryArgs(**{**base, **bad})), None) < 0
+    assert entry("xva_rotary")(C.byref(RotaryArgs(**{**base, **bad})), None) < 0
     assert says in _lib.lib.xva_last_error().decode()
 
 
@@ -108,14 +109,14 @@ def test_rotary_refuses(bad, says):
                                       (dict(T=500, C=1025, G=1), "vectors")])
 def test_group_norm_refuses(bad, says):
     base = dict(x=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3, C=32, G=4, act=0, eps=1e-5)
-    assert _lib.lib.xva_group_norm_act_fwd(C.byref(S._GroupNormArgs(**{**base, **bad})), None, 0, None) < 0
+    assert entry("xva_group_norm_act_fwd")(C.byref(GroupNormArgs(**{**base, **bad})), None, 0, None) < 0
     assert says in _lib.lib.xva_last_error().decode()
 
 
 def test_group_norm_refuses_a_small_workspace():
-    a = S._GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3000, C=32, G=4, act=0, eps=1e-5)
-    for bwd, call in ((0, _lib.lib.xva_group_norm_act_fwd), (1, _lib.lib.xva_group_norm_act_bwd)):
-        need = _lib.lib.xva_group_norm_workspace_bytes(C.byref(a), bwd)
+    a = GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3000, C=32, G=4, act=0, eps=1e-5)
+    for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
+        need = entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd)
         assert need > 0 and call(C.byref(a), A, need - 1, None) == -3
 
 
@@ -123,12 +124,12 @@ def test_group_norm_refuses_a_small_workspace():
                                       (dict(B=1 << 20, C=1 << 12), "B ")])
 def test_recurrence_refuses(bad, says):
     base = dict(x=A, gate=A, h=A, last=A, dtype=0, B=2, T=3, C=8)
-    assert _lib.lib.xva_recurrence_fwd(C.byref(S._RecurrenceArgs(**{**base, **bad})), None, 0, None) < 0
+    assert entry("xva_recurrence_fwd")(C.byref(RecurrenceArgs(**{**base, **bad})), None, 0, None) < 0
     assert says in _lib.lib.xva_last_error().decode()
 
 
 def test_recurrence_refuses_a_small_workspace():
-    need = _lib.lib.xva_recurrence_workspace_bytes(1, 30000, 64)
+    need = entry("xva_recurrence_workspace_bytes", i64)(1, 30000, 64)
     assert need > 0
-    assert _lib.lib.xva_recurrence_fwd(C.byref(S._RecurrenceArgs(x=A, gate=A, h=A, last=A, dtype=0, B=1, T=30000, C=64)), A, need - 1, None) == -3
-    assert _lib.lib.xva_recurrence_bwd(C.byref(S._RecurrenceArgs(x=A, gate=A, dtype=0, B=1, T=30000, C=64)), A, need, None) < 0
+    assert entry("xva_recurrence_fwd")(C.byref(RecurrenceArgs(x=A, gate=A, h=A, last=A, dtype=0, B=1, T=30000, C=64)), A, need - 1, None) == -3
+    assert entry("xva_recurrence_bwd")(C.byref(RecurrenceArgs(x=A, gate=A, dtype=0, B=1, T=30000, C=64)), A, need, None) < 0

@@ -53,13 +53,36 @@ def _compile(src, verbose, force=False):
     return obj, True
 
 
+def _build_torch_binding(verbose, force):
+    """_seq_torch.so: the sequence operators' torch side (autograd nodes, allocation), host code only."""
+    import sysconfig
+
+    import torch
+    src, out = os.path.join(CSRC, "seq_torch.cpp"), os.path.join(HERE, "_seq_torch.so")
+    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), _headers_mtime()):
+        return out
+    root = os.path.dirname(torch.__file__)
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_seq_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + os.path.join(root, "include"),
+           "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I/opt/rocm/include", "-I" + sysconfig.get_paths()["include"], src, "-o", out,
+           "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_hip", "-ltorch_hip"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
+    return out
+
+
 def build(verbose=True, force=False):
     """force: a from-source rebuild — every object is recompiled and the library relinked (`python xva-trainer_amd/build.py --force`)."""
     if force and os.path.exists(LIB):
         os.remove(LIB)
     srcs = _sources()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        binding = ex.submit(_build_torch_binding, verbose, force)
         res = list(ex.map(lambda s: _compile(s, verbose, force), srcs))
+        binding.result()
     objs = [o for o, _ in res]
     changed = any(c for _, c in res)
     if changed or not os.path.exists(LIB):
