@@ -32,39 +32,29 @@ struct Args {
     int B, T, D, rd, per_wg;
 };
 
-// 2 V neighbouring elements; element by element where V = 1 stands for any alignment
-template <int DT, int V> __device__ __forceinline__ void load_2v(const void* base, int64_t off, float (&f)[2 * V]) {
-    if constexpr (V == 1) {
-        float u[1];
-        load_v<DT, 1>(base, off, u); f[0] = u[0];
-        load_v<DT, 1>(base, off + 1, u); f[1] = u[0];
-    } else load_v<DT, 2 * V>(base, off, f);
-}
-template <int DT, int V> __device__ __forceinline__ void store_2v(void* base, int64_t off, const float (&f)[2 * V]) {
-    if constexpr (V == 1) {
-        const float u[1] = {f[0]}, w[1] = {f[1]};
-        store_v<DT, 1>(base, off, u); store_v<DT, 1>(base, off + 1, w);
-    } else store_v<DT, 2 * V>(base, off, f);
-}
-
-// A work item is V pairs of one (token, head), or 2 V elements (one, where V = 1) of its part that does not turn.  Items of a row lie side by side over the lanes.
+// A work item is V pairs of one (token, head), or 2 V elements of its part that does not turn.  Items of a row lie side by side over the lanes.
+// V = 0: one pair, element by element (any alignment), or one element of the still part; V = 1 in the half layout takes any alignment as it is.
 template <int DT, bool INTER, int V>
 __global__ __launch_bounds__(THREADS) void rotary_kernel(Args a) {
-    __shared__ float2 cs[LDS_PAIRS];
-    __shared__ int2 where[MAX_TOKENS];     // (item, row) of each token
+    extern __shared__ float2 cs[];         // (cos, sin) of the workgroup's tokens
+    __shared__ int64_t at[MAX_TOKENS][4];  // where each token's heads start: queries in and out, keys in and out
+    constexpr int P = V ? V : 1;           // pairs of an item
+    constexpr bool ONE = INTER ? V == 0 : V == 1;      // elements one by one
     const int np = a.rd >> 1;
-    const int64_t tokens = (int64_t)a.B * a.T;
-    const int64_t tok0 = (int64_t)blockIdx.x * a.per_wg;
-    const int ntok = (int)min((int64_t)a.per_wg, tokens - tok0);
+    const unsigned tok0 = blockIdx.x * (unsigned)a.per_wg;
+    const int ntok = (int)min((unsigned)a.per_wg, (unsigned)a.B * (unsigned)a.T - tok0);
     for (int e = threadIdx.x; e < ntok * np; e += THREADS) {
         const int tl = (unsigned)e / (unsigned)np, i = e - tl * np;
-        const unsigned tok = (unsigned)tok0 + tl;
+        const unsigned tok = tok0 + tl;
         const int b = (int)(tok / (unsigned)a.T), t = (int)(tok - (unsigned)b * (unsigned)a.T);
-        if (i == 0) where[tl] = make_int2(b, t);
+        if (i == 0) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) { at[tl][2 * k] = b * a.s[k].xb + t * a.s[k].xt; at[tl][2 * k + 1] = b * a.s[k].yb + t * a.s[k].yt; }
+        }
         int64_t p = t;
         if (a.pos) {
-            const int64_t at = b * a.pb + t * a.pt;
-            p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[at];
+            const int64_t where = b * a.pb + t * a.pt;
+            p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[where] : (int64_t)reinterpret_cast<const int32_t*>(a.pos)[where];
         }
         const float turn = (float)(int64_t)((uint64_t)p * a.turns[i]);      // in units of 2^-64 turns, -2^63 .. 2^63: within half a turn of zero
         float sn, c;
@@ -74,7 +64,7 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Args a) {
     __syncthreads();
     const int HT = a.s[0].heads + a.s[1].heads;
     // (in place the part that does not turn stays where it is)
-    const int turning = np / V, still = (a.s[0].x == a.s[0].y) ? 0 : (V == 1 ? a.D - a.rd : (a.D - a.rd) / (2 * V));
+    const int turning = np / P, still = (a.s[0].x == a.s[0].y) ? 0 : (ONE ? a.D - a.rd : (a.D - a.rd) / (2 * P));
     const int per_row = turning + still;
     const int lanes = min(per_row, THREADS), rows_at_once = THREADS / lanes;
     const int lane = threadIdx.x % lanes, first = threadIdx.x / lanes;
@@ -82,42 +72,49 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Args a) {
     const int step_t = rows_at_once / HT, step_h = rows_at_once - step_t * HT;
     int tl = first / HT, h = first - tl * HT;
     while (tl < ntok) {
-        const int b = where[tl].x, t = where[tl].y;
         const bool key = h >= a.s[0].heads;
-        const Side& s = a.s[key ? 1 : 0];
-        const int hh = key ? h - a.s[0].heads : h;
-        const int64_t xo = (int64_t)b * s.xb + (int64_t)t * s.xt + hh * s.xh, yo = (int64_t)b * s.yb + (int64_t)t * s.yt + hh * s.yh;
+        const uint32_t hh = key ? h - a.s[0].heads : h;
+        const void* x = key ? a.s[1].x : a.s[0].x;
+        void* y = key ? a.s[1].y : a.s[0].y;
+        const int64_t xo = at[tl][key ? 2 : 0] + (int64_t)((uint64_t)hh * (key ? a.s[1].xh : a.s[0].xh)), yo = at[tl][key ? 3 : 1] + (int64_t)((uint64_t)hh * (key ? a.s[1].yh : a.s[0].yh));
         for (int c = lane; c < per_row; c += lanes) {
             if (c < turning) {
-                const float2* w = cs + tl * np + c * V;
+                const float2* w = cs + tl * np + c * P;
                 if constexpr (INTER) {
-                    float f[2 * V];
-                    load_2v<DT, V>(s.x, xo + 2 * V * c, f);
+                    float f[2 * P];
+                    if constexpr (ONE) {
+                        float u[1];
+                        load_v<DT, 1>(x, xo + 2 * c, u); f[0] = u[0];
+                        load_v<DT, 1>(x, xo + 2 * c + 1, u); f[1] = u[0];
+                    } else load_v<DT, 2 * P>(x, xo + 2 * P * c, f);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
+                    for (int e = 0; e < P; ++e) {
                         const float2 k = w[e];
                         const float u = f[2 * e] * k.x - f[2 * e + 1] * k.y, v = f[2 * e + 1] * k.x + f[2 * e] * k.y;
                         f[2 * e] = u; f[2 * e + 1] = v;
                     }
-                    store_2v<DT, V>(s.y, yo + 2 * V * c, f);
+                    if constexpr (ONE) {
+                        const float u[1] = {f[0]}, v[1] = {f[1]};
+                        store_v<DT, 1>(y, yo + 2 * c, u); store_v<DT, 1>(y, yo + 2 * c + 1, v);
+                    } else store_v<DT, 2 * P>(y, yo + 2 * P * c, f);
                 } else {
-                    float f[V], g[V];
-                    load_v<DT, V>(s.x, xo + V * c, f);
-                    load_v<DT, V>(s.x, xo + np + V * c, g);
+                    float f[P], g[P];
+                    load_v<DT, P>(x, xo + P * c, f);
+                    load_v<DT, P>(x, xo + np + P * c, g);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) {
+                    for (int e = 0; e < P; ++e) {
                         const float2 k = w[e];
                         const float u = f[e] * k.x - g[e] * k.y, v = g[e] * k.x + f[e] * k.y;
                         f[e] = u; g[e] = v;
                     }
-                    store_v<DT, V>(s.y, yo + V * c, f);
-                    store_v<DT, V>(s.y, yo + np + V * c, g);
+                    store_v<DT, P>(y, yo + P * c, f);
+                    store_v<DT, P>(y, yo + np + P * c, g);
                 }
             } else {
-                constexpr int W = V == 1 ? 1 : 2 * V;
+                constexpr int W = ONE ? 1 : 2 * P;
                 float f[W];
-                load_v<DT, W>(s.x, xo + a.rd + W * (c - turning), f);
-                store_v<DT, W>(s.y, yo + a.rd + W * (c - turning), f);
+                load_v<DT, W>(x, xo + a.rd + W * (c - turning), f);
+                store_v<DT, W>(y, yo + a.rd + W * (c - turning), f);
             }
         }
         tl += step_t; h += step_h;
@@ -125,12 +122,13 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(Args a) {
     }
 }
 
-template <int DT, bool INTER> int launch(const Args& a, int v, dim3 grid, hipStream_t st) {
+template <int DT, bool INTER> int launch(const Args& a, int v, dim3 grid, size_t lds, hipStream_t st) {
     switch (v) {
-        case 8: if constexpr (DT != 0 && !INTER) { rotary_kernel<DT, INTER, 8><<<grid, THREADS, 0, st>>>(a); break; }
-        case 4: rotary_kernel<DT, INTER, 4><<<grid, THREADS, 0, st>>>(a); break;
-        case 2: rotary_kernel<DT, INTER, 2><<<grid, THREADS, 0, st>>>(a); break;
-        default: rotary_kernel<DT, INTER, 1><<<grid, THREADS, 0, st>>>(a);
+        case 8: if constexpr (DT != 0 && !INTER) { rotary_kernel<DT, INTER, 8><<<grid, THREADS, lds, st>>>(a); break; }
+        case 4: rotary_kernel<DT, INTER, 4><<<grid, THREADS, lds, st>>>(a); break;
+        case 2: rotary_kernel<DT, INTER, 2><<<grid, THREADS, lds, st>>>(a); break;
+        case 1: rotary_kernel<DT, INTER, 1><<<grid, THREADS, lds, st>>>(a); break;
+        default: rotary_kernel<DT, INTER, INTER ? 0 : 1><<<grid, THREADS, lds, st>>>(a);
     }
     XVA_LAUNCH_CHECK();
     return XVA_OK;
@@ -157,7 +155,7 @@ extern "C" int xva_rotary(const xva_rotary_args* p, void* stream) {
     // widest vector that divides both halves (half layout) / the pairs (interleaved), the still part and every stride and address
     const int es = p->dtype == 0 ? 4 : 2, np = p->rd / 2;
     int v = p->dtype != 0 && !p->interleaved ? 8 : 4;
-    for (; v > 1; v >>= 1) {
+    for (; v > (p->interleaved ? 0 : 1); v >>= 1) {
         const int el = p->interleaved ? 2 * v : v;                  // elements of one access, or 16 bytes where that is less
         const int al = el * es < 16 ? el : 16 / es;
         bool ok = np % v == 0 && (p->D - p->rd) % (2 * v) == 0;
@@ -182,10 +180,11 @@ extern "C" int xva_rotary(const xva_rotary_args* p, void* stream) {
     a.per_wg = (int)per;
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)wgs);
+    const size_t lds = (size_t)per * np * sizeof(float2);
     if (p->interleaved) {
-        if (p->dtype == 0) return launch<0, true>(a, v, grid, st);
-        return p->dtype == 1 ? launch<1, true>(a, v, grid, st) : launch<2, true>(a, v, grid, st);
+        if (p->dtype == 0) return launch<0, true>(a, v, grid, lds, st);
+        return p->dtype == 1 ? launch<1, true>(a, v, grid, lds, st) : launch<2, true>(a, v, grid, lds, st);
     }
-    if (p->dtype == 0) return launch<0, false>(a, v, grid, st);
-    return p->dtype == 1 ? launch<1, false>(a, v, grid, st) : launch<2, false>(a, v, grid, st);
+    if (p->dtype == 0) return launch<0, false>(a, v, grid, lds, st);
+    return p->dtype == 1 ? launch<1, false>(a, v, grid, lds, st) : launch<2, false>(a, v, grid, lds, st);
 }
