@@ -83,7 +83,10 @@ def _data(B, T, C, dt, seed=0, mean=0.3):
 
 
 SHAPES = [(1, 1, 16, 1), (300, 1, 512, 8), (5, 1, 1024, 2), (3, 2, 48, 3), (2, 860, 384, 16), (1, 1, 8, 2), (3, 65, 40, 5), (2, 33, 31, 1), (4, 300, 21, 3),
-          (1, 2000, 32, 4), (2, 9, 1023, 1), (1, 40, 2048, 32), (2, 700, 8, 8), (7, 3, 136, 8), (600, 5, 72, 8), (1, 5000, 16, 1), (2, 17, 2048, 2048), (1, 1, 1023, 3)]
+          (1, 2000, 32, 4), (2, 9, 1023, 1), (1, 40, 2048, 32), (2, 700, 8, 8), (7, 3, 136, 8), (600, 5, 72, 8), (1, 5000, 16, 1), (2, 17, 2048, 2048), (1, 1, 1023, 3),
+          # vectors of two, one to eight of them to a lane; groups of two values to the workgroup; many chunks, few channels; more items than one join takes
+          (5, 7, 432, 8), (3, 9, 432, 8), (2, 60, 432, 8), (3, 1, 150, 3), (2, 2500, 150, 3), (3, 388, 8, 8), (1, 20011, 16, 4), (1, 9000, 150, 3), (1100, 20, 32, 1),
+          (1100, 3, 2, 1), (1030, 21, 33, 1), (2, 70, 4088, 2)]
 
 
 @pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
@@ -154,7 +157,7 @@ def test_views_strides_and_flat_rows():
     from xva_trainer_amd import seq_ops as S
     store = torch.randn(3, 40, 100, device="cuda").bfloat16()
     for view in (store[:, 1:-1, :64], store[:, ::2, 8:72], store[:, :, 3:67], store.transpose(0, 1)[..., :32], store[1:2].expand(3, 40, 100)[..., :96],
-                 store.transpose(1, 2)[:, :64, :32]):
+                 store.transpose(1, 2)[:, :64, :32], store[:, :, 2:66], store[:, :1, 2:66], store[:, :, 6:14]):
         G = 4
         dy = torch.randn(view.shape, device="cuda").bfloat16()
         _run(view, None, None, dy, None, G)
@@ -225,6 +228,6 @@ def test_refusals():
                 lambda: S.group_norm_act(x, 4, lens=torch.tensor([1, 2, 3], device="cuda")), lambda: S.group_norm_act(x, 4, lens=torch.tensor([1, 2])),
                 lambda: S.group_norm_act(x, 4, lens=torch.tensor([1.0, 2.0], device="cuda")), lambda: S.group_norm_act(x[0], 4, lens=torch.tensor([1, 2], device="cuda")),
                 lambda: S.group_norm_act(x, 4, eps=-1.0), lambda: S.group_norm_act(x.cpu(), 4),
-                lambda: S.group_norm_act(torch.zeros(1, 300, 16384, device="cuda"), 2), lambda: S.group_norm_act(torch.zeros(1, 300, 4096, device="cuda"), 4096)):
+                lambda: S.group_norm_act(torch.zeros(1, 300, 16384, device="cuda"), 2), lambda: S.group_norm_act(torch.zeros(1, 600, 4096, device="cuda"), 4096)):
         with pytest.raises(S.XvaError):
             bad()

@@ -69,7 +69,7 @@ template <int V> __device__ __forceinline__ void slopes(float (&z)[V], int act, 
         default: each<V>(z, [](float) { return 1.f; });
     }
 }
-// V values of a weight vector (16-byte aligned where V > 1), `none` where there is none
+// V values of a weight vector (aligned to 16 bytes, 8 where V = 2), `none` where there is none
 template <int V> __device__ __forceinline__ void load_w(const float* w, int c, float none, float (&f)[V]) {
     if (w) load_v<0, V>(w, c, f);
     else {
@@ -376,6 +376,7 @@ __global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
 // ================================================================================ tile form ====
 // A thread owns one vector of V channels and every `step`-th row of its chunk; lc = C / V vectors side by side, step = blockDim.x / lc rows at once.
 constexpr int NR = 8;      // rows of a thread in one register tile
+constexpr int MAX_CHUNKS = 256;        // of an item
 
 struct Tile {
     int lc, step, v, r; bool on;
@@ -392,20 +393,29 @@ template <int V> __device__ __forceinline__ void put(float* red, const Tile& t, 
         for (int e = 0; e < V; ++e) red[t.r * C + t.v * V + e] = s[e];
     }
 }
-// group sums of red into out[g], by runs of `run` lanes (a power of two)
-__device__ __forceinline__ void group_sums(const float* red, float* out, const Tile& t, int C, int G, int n, int run) {
-    const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
+// Runs of lanes that share a sum: `chans` lanes over the n channels of a group (a power of two), times as many over the row slots as keep all groups within one turn
+// of the workgroup (few channels mean many slots).
+struct Run { int chans, lanes; };
+__device__ __forceinline__ Run run_of(int n, int G, int slots) {
+    Run r = {1, 1};
+    while (r.chans < n && r.chans < 64) r.chans <<= 1;
+    r.lanes = r.chans;
+    while (r.lanes < 64 && 2 * r.lanes * G <= (int)blockDim.x && r.lanes < r.chans * slots) r.lanes <<= 1;
+    return r;
+}
+// group sums of red into out[g]
+__device__ __forceinline__ void group_sums(const float* red, float* out, const Tile& t, int C, int G, int n, Run run) {
+    const int per = blockDim.x / run.lanes, lane = threadIdx.x & (run.lanes - 1), cl = lane & (run.chans - 1), s0 = lane / run.chans, ss = run.lanes / run.chans;
     for (int g0 = 0; g0 < G; g0 += per) {
-        const int g = g0 + threadIdx.x / run;
+        const int g = g0 + threadIdx.x / run.lanes;
         float v = 0.f;
         if (g < G)
-            for (int sl = 0; sl < t.step; ++sl)
-                for (int c = lane; c < n; c += run) v += red[sl * C + g * n + c];
-        v = lanes_sum(v, run);
+            for (int sl = s0; sl < t.step; sl += ss)
+                for (int c = cl; c < n; c += run.chans) v += red[sl * C + g * n + c];
+        v = lanes_sum(v, run.lanes);
         if (g < G && lane == 0) out[g] = v;
     }
 }
-__device__ __forceinline__ int run_of(int n) { int r = 1; while (r < n && r < 64) r <<= 1; return r; }
 
 // statistics of one chunk: part[(b * chunks + chunk) * G + g] = (mean, sum of squared deviations)
 template <int DT, int V, int NT>
@@ -416,7 +426,8 @@ __global__ __launch_bounds__(NT) void tile_stats_kernel(Args a) {
     float* mean = red + t.step * a.C;          // G: running mean, then squared deviations
     float* m2 = mean + a.G;
     float* now = m2 + a.G;                     // G: this tile's sums
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.n);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b);
+    const Run run = run_of(a.n, a.G, t.step);
     const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, len);
     for (int g = threadIdx.x; g < a.G; g += blockDim.x) mean[g] = m2[g] = 0.f;
     float before = 0.f;                        // rows joined so far
@@ -483,22 +494,27 @@ __global__ __launch_bounds__(NT) void tile_apply_kernel(Args a) {
     float* mean = lds;
     float* rstd = lds + a.G;
     const Tile t(a.C, V);
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.chunks);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.chunks, 1, 1).lanes;
     const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, a.T);
     const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
     const float2* part = reinterpret_cast<const float2*>(a.part) + (int64_t)b * a.chunks * a.G;
     const float inv = len > 0 ? 1.f / ((float)len * (float)a.n) : 0.f;
     for (int g0 = 0; g0 < a.G; g0 += per) {
         const int g = g0 + threadIdx.x / run;
-        float2 p = make_float2(0.f, 0.f);
-        float rows = 0.f;
-        if (g < a.G && lane < a.chunks) {
-            rows = (float)min(max(len - lane * a.rows_per_chunk, 0), a.rows_per_chunk);
-            if (rows > 0.f) p = part[lane * a.G + g];
+        float2 p[MAX_CHUNKS / 64];
+        float rows[MAX_CHUNKS / 64], mu = 0.f, var = 0.f;
+#pragma unroll
+        for (int i = 0; i < MAX_CHUNKS / 64; ++i) {
+            const int k = lane + 64 * i;                   // (more than one where there are more than 64 chunks, whose run is 64 lanes)
+            p[i] = make_float2(0.f, 0.f);
+            rows[i] = g < a.G && k < a.chunks ? (float)min(max(len - k * a.rows_per_chunk, 0), a.rows_per_chunk) : 0.f;
+            if (rows[i] > 0.f) p[i] = part[k * a.G + g];
+            mu += p[i].x * (rows[i] * (float)a.n);
         }
-        const float mu = lanes_sum(p.x * (rows * (float)a.n), run) * inv;
-        const float d = p.x - mu;
-        const float var = lanes_sum(p.y + d * d * (rows * (float)a.n), run) * inv;
+        mu = lanes_sum(mu, run) * inv;
+#pragma unroll
+        for (int i = 0; i < MAX_CHUNKS / 64; ++i) { const float d = p[i].x - mu; var += p[i].y + d * d * (rows[i] * (float)a.n); }
+        var = lanes_sum(var, run) * inv;
         if (g < a.G && lane == 0) {
             mean[g] = mu; rstd[g] = rsqrtf(var + a.eps);
             if (chunk == 0) { a.mean[(int64_t)b * a.G + g] = mean[g]; a.rstd[(int64_t)b * a.G + g] = rstd[g]; }
@@ -548,6 +564,7 @@ __global__ __launch_bounds__(NT) void tile_apply_kernel(Args a) {
 template <int DT, int V, int NT>
 __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
     extern __shared__ float red[];
+    constexpr int RU = NT > 256 && V > 4 ? 2 : 4;          // rows under way (four of them would not fit the registers that 1024 threads leave)
     const Tile t(a.C, V);
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b);
     const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, len);
@@ -564,10 +581,10 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
             mu[e] = a.mean[(int64_t)b * a.G + g]; rs[e] = a.rstd[(int64_t)b * a.G + g];
         }
         const int64_t xo = (int64_t)b * a.xb + t.v * V, po = (int64_t)b * a.db_ + t.v * V;
-        for (int r0 = first + t.r; r0 < end; r0 += 4 * t.step) {
-            float f[4][V], d[4][V];
+        for (int r0 = first + t.r; r0 < end; r0 += RU * t.step) {
+            float f[RU][V], d[RU][V];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < RU; ++k) {
                 const int r = r0 + k * t.step;
                 if (r < end) { load_v<DT, V>(a.x, xo + (int64_t)r * a.xt, f[k]); load_v<DT, V>(a.dy, po + (int64_t)r * a.dt_, d[k]); }
                 else {
@@ -576,7 +593,7 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < RU; ++k) {
                 float z[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) { f[k][e] = (f[k][e] - mu[e]) * rs[e]; z[e] = f[k][e] * w[e] + bias[e]; }
@@ -592,51 +609,50 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
         __syncthreads();
         put<V>(red, t, a.C, which ? s2 : s1);
         __syncthreads();
-        for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
-            float v = 0.f;
-            for (int sl = 0; sl < t.step; ++sl) v += red[sl * a.C + c];
-            out[which * a.C + c] = v;
-        }
+        const Run run = run_of(1, a.C, t.step);
+        group_sums(red, out + which * a.C, t, a.C, a.C, 1, run);
     }
 }
 
-// (rows, 2, C) partial sums -> per-item sums (items of `per_item` rows; null: not wanted) and the totals db = sum of [0], dw = sum of [1].
-// 32 channels x 32 item slots to a workgroup; the slots are added in order.
-__global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ part, int items, int per_item, int C, float* __restrict__ item, float* __restrict__ dw,
-                                                    float* __restrict__ db) {
+// (items of per_item rows, 2, C) partial sums -> sums of each item.  A workgroup: 32 channels of one of the two sums, 32 items.
+__global__ __launch_bounds__(1024) void item_kernel(const float* __restrict__ part, int items, int per_item, int C, float* __restrict__ item) {
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), which = blockIdx.y;
+    const int64_t b = (int64_t)blockIdx.z * 32 + (threadIdx.x >> 5);
+    if (c >= C || b >= items) return;
+    const float* at = part + (b * per_item * 2 + which) * C + c;
+    float t[4] = {};
+    int k = 0;
+    for (; k + 3 < per_item; k += 4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] += at[(int64_t)(k + i) * 2 * C];
+    for (; k < per_item; ++k) t[0] += at[(int64_t)k * 2 * C];
+    item[(b * 2 + which) * C + c] = (t[0] + t[1]) + (t[2] + t[3]);
+}
+
+// (rows, 2, C) -> sums over segments of `seg` rows, into out0 + segment * stride for [0] and out1 for [1] (null: not wanted).  A workgroup: 32 channels x 32 slots of
+// rows, added in order.
+__global__ __launch_bounds__(1024) void join_kernel(const float* __restrict__ part, int rows, int seg, int C, float* __restrict__ out0, float* __restrict__ out1, int64_t stride) {
     __shared__ float red[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), slot = threadIdx.x >> 5, which = blockIdx.y;
+    const int first = blockIdx.z * seg, end = min(rows, first + seg);
     float total = 0.f;
-    if (c < C && !item) {
+    if (c < C) {
         const float* at = part + (int64_t)which * C + c;
-        const int rows = items * per_item;
         float t[4] = {};
-        int r = slot;
-        for (; r + 96 < rows; r += 128)
+        int r = first + slot;
+        for (; r + 96 < end; r += 128)
 #pragma unroll
             for (int k = 0; k < 4; ++k) t[k] += at[(int64_t)(r + 32 * k) * 2 * C];
-        for (; r < rows; r += 32) t[0] += at[(int64_t)r * 2 * C];
+        for (; r < end; r += 32) t[0] += at[(int64_t)r * 2 * C];
         total = (t[0] + t[1]) + (t[2] + t[3]);
-    } else if (c < C)
-        for (int b = slot; b < items; b += 32) {
-            const float* at = part + ((int64_t)b * per_item * 2 + which) * C + c;
-            float t[4] = {};
-            int k = 0;
-            for (; k + 3 < per_item; k += 4)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) t[i] += at[(int64_t)(k + i) * 2 * C];
-            for (; k < per_item; ++k) t[0] += at[(int64_t)k * 2 * C];
-            const float v = (t[0] + t[1]) + (t[2] + t[3]);
-            item[((int64_t)b * 2 + which) * C + c] = v;
-            total += v;
-        }
-    float* out = which ? dw : db;
+    }
+    float* out = which ? out1 : out0;
     red[slot][threadIdx.x & 31] = total;
     __syncthreads();
     if (out && threadIdx.x < 32 && c < C) {
         float v = 0.f;
         for (int k = 0; k < 32; ++k) v += red[k][threadIdx.x];
-        out[c] = v;
+        out[blockIdx.z * stride + c] = v;
     }
 }
 
@@ -646,7 +662,7 @@ __global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
     float* m1 = lds;                       // means of w dz and w dz xh of each group
     float* m2 = lds + a.G;
     const Tile t(a.C, V);
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.n);
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, len = live_rows(a, b), run = run_of(a.n, 1, 1).lanes;
     const int first = chunk * a.rows_per_chunk, end = min(first + a.rows_per_chunk, a.T);
     const int per = blockDim.x / run, lane = threadIdx.x & (run - 1);
     const float* item = a.item + (int64_t)b * 2 * a.C;
@@ -704,7 +720,7 @@ __global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
 // -------------------------------------------------------------------------------- plan ----
 enum { SLAB, WHOLE, TILE };
 struct Plan {
-    int v;                                  // elements of a vector: 16 bytes, or one
+    int v;                                  // elements of a vector: 16 bytes, two or one
     int form, nv;                           // vectors of a thread: slab and whole forms
     SlabPlan s; int slab_wgs;
     WholePlan w; int whole_wgs;
@@ -713,17 +729,27 @@ struct Plan {
 
 int pow2_at_least(int64_t x) { int r = 1; while (r < x) r <<= 1; return r; }
 
-bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
+// widest of 16 bytes, two values and one that divides x and is allowed
+int widest(int dtype, int allowed, int x) {
+    const int wide = dtype == 0 ? 4 : 8;
+    return allowed >= wide && x % wide == 0 ? wide : (allowed >= 2 && x % 2 == 0 ? 2 : 1);
+}
+// rows of dw / dbias partial sums that one workgroup of the join adds: beyond it, segments first
+constexpr int JOIN_ROWS = 1024;
+int join_segment(int64_t rows) { return (int)(rows <= (int64_t)JOIN_ROWS * JOIN_ROWS ? JOIN_ROWS : (rows + JOIN_ROWS - 1) / JOIN_ROWS); }
+int join_segments(int64_t rows) { return (int)((rows + join_segment(rows) - 1) / join_segment(rows)); }
+
+bool make_plan(const xva_group_norm_args* p, int vec, bool bwd, Plan* out) {
     Plan& q = *out;
-    const int wide = p->dtype == 0 ? 4 : 8, n = p->C / p->G;
-    q.v = vec && p->C % wide == 0 ? wide : 1;
-    // slab form: a (item, group) slab of whole vectors (of one value, where 16 bytes would straddle groups) within 64 lanes x 4 vectors
-    const int sv = n % q.v == 0 ? q.v : 1;
+    const int n = p->C / p->G;
+    q.v = widest(p->dtype, vec, p->C);
+    // slab form: a (item, group) slab of whole vectors within 64 lanes x 4 vectors (8 where they are narrow)
+    const int sv = widest(p->dtype, vec, n);
     const int64_t vecs = (int64_t)p->T * (n / sv);
-    if (vecs <= 256) {
+    if (vecs <= (sv <= 2 ? 512 : 256)) {
         q.form = SLAB;
         q.v = sv;
-        q.nv = vecs <= 64 ? 1 : (vecs <= 128 ? 2 : 4);
+        q.nv = vecs <= 64 ? 1 : (vecs <= 128 ? 2 : (vecs <= 256 ? 4 : 8));
         q.s.lpg = pow2_at_least((vecs + q.nv - 1) / q.nv);
         const int slots = 256 / q.s.lpg;
         q.s.gpb = p->G < slots ? p->G : slots;
@@ -739,12 +765,12 @@ bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
     }
     // whole form: groups of one item within the registers of 512 threads (16 packed vectors to a thread, 12 of x and 12 of dy backward).  As many groups as make
     // 64 bytes of a row, more where workgroups abound.
-    if (sv == q.v && q.v > 1) {
-        const int nv = n / q.v, cap = 512 * (bwd ? 12 : 16);
-        int gpw = (4 + nv - 1) / nv;
+    if (sv > 1) {
+        const int nv = n / sv, cap = 512 * (bwd ? 12 : 16), line = 64 / (sv * xva_seq::elem_size(p->dtype));      // vectors of 64 bytes
+        int gpw = (line + nv - 1) / nv;
         if (gpw > p->G) gpw = p->G;
         while (gpw > 1 && (int64_t)p->T * nv * gpw > cap) --gpw;
-        while (gpw * 2 <= p->G && gpw * 2 * nv <= 16 && (int64_t)p->T * nv * gpw * 2 <= cap && (int64_t)p->B * ((p->G + 2 * gpw - 1) / (2 * gpw)) >= 512) gpw *= 2;
+        while (gpw * 2 <= p->G && gpw * 2 * nv <= 4 * line && (int64_t)p->T * nv * gpw * 2 <= cap && (int64_t)p->B * ((p->G + 2 * gpw - 1) / (2 * gpw)) >= 512) gpw *= 2;
         const int lv = gpw * nv;
         if (lv <= 512 && (int64_t)p->T * nv * gpw <= (int64_t)(512 / lv) * lv * (bwd ? 12 : 16)) {
             q.form = WHOLE;
@@ -755,7 +781,7 @@ bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
             const int each = (p->T + q.w.rows - 1) / q.w.rows;
             q.nv = each <= 4 ? 4 : (each <= 8 ? 8 : (each <= 12 ? 12 : 16));
             q.whole_wgs = (int)(((int64_t)p->B * q.w.blocks + 7) / 8 * 8);
-            if (each <= (bwd ? 12 : 16)) return true;
+            if (each <= (bwd ? 12 : 16)) { q.v = sv; return true; }
         }
     }
     q.form = TILE;
@@ -763,24 +789,26 @@ bool make_plan(const xva_group_norm_args* p, bool vec, bool bwd, Plan* out) {
     if (lc > 1024 || p->G > 2048) return false;        // (a row in one workgroup, its groups in the LDS)
     q.threads = lc <= 256 ? 256 : (lc + 63) / 64 * 64;
     const int step = q.threads / lc;
-    // chunks of whole register tiles: enough of them for four workgroups to a CU, at most 64 of an item (one lane each when they are joined)
-    const int tile = step * NR;
-    int64_t tiles = (p->T + tile - 1) / tile;
-    int64_t want = (1024 + p->B - 1) / p->B;
-    if (want > 64) want = 64;
-    if (want > tiles) want = tiles;
-    const int64_t each = (tiles + want - 1) / want;
-    q.rows_per_chunk = (int)(each * tile);
+    // chunks of whole register tiles where there are rows for four workgroups to a CU, of fewer rows where there are not; at most 256 of an item (four to a
+    // lane when they are joined)
+    int64_t turns = (p->T + step - 1) / step, want = (1024 + p->B - 1) / p->B;
+    if (want > MAX_CHUNKS) want = MAX_CHUNKS;
+    if (want > turns) want = turns;
+    int64_t each = (turns + want - 1) / want;
+    if (each > NR) each = (each + NR - 1) / NR * NR;
+    q.rows_per_chunk = (int)(each * step);
     q.chunks = (int)((p->T + q.rows_per_chunk - 1) / q.rows_per_chunk);
     return true;
 }
 
-bool aligned(const xva_group_norm_args* p, bool bwd) {
+// the widest vector that strides and addresses allow
+int allowed(const xva_group_norm_args* p, bool bwd) {
     const int wide = p->dtype == 0 ? 4 : 8;
     int64_t all = p->x_stride[0] | p->x_stride[1] | p->out_stride[0] | p->out_stride[1];
-    uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->out | (uintptr_t)p->weight | (uintptr_t)p->bias;
+    uintptr_t ptrs = (uintptr_t)p->x | (uintptr_t)p->out, weights = (uintptr_t)p->weight | (uintptr_t)p->bias;
     if (bwd) { all |= p->dy_stride[0] | p->dy_stride[1]; ptrs |= (uintptr_t)p->dy; }
-    return all % wide == 0 && ptrs % 16 == 0;
+    if (all % wide == 0 && (ptrs | weights) % 16 == 0) return wide;
+    return all % 2 == 0 && ptrs % (2 * xva_seq::elem_size(p->dtype)) == 0 && weights % 8 == 0 ? 2 : 1;
 }
 
 int check(const xva_group_norm_args* p, const char* who) {
@@ -804,15 +832,15 @@ Args args_of(const xva_group_norm_args* p, const Plan& q) {
 }
 
 int64_t workspace(const xva_group_norm_args* p, bool bwd) {
-    // (over both vector widths: which one runs depends on addresses and strides)
+    // (over the vector widths: which one runs depends on addresses and strides)
     int64_t most = 0;
-    for (int vec = 0; vec < 2; ++vec) {
+    for (int vec = 8; vec > 0; vec = vec == 8 ? 2 : vec - 1) {
         Plan q = {};
-        if (!make_plan(p, vec != 0, bwd, &q)) continue;
+        if (!make_plan(p, vec, bwd, &q)) continue;
         int64_t f;
-        if (q.form == WHOLE) f = bwd ? (int64_t)p->B * 2 * p->C : 0;
-        else if (q.form == SLAB) f = bwd ? (int64_t)q.slab_wgs * 2 * p->C : 0;
-        else f = bwd ? (int64_t)p->B * (q.chunks + 1) * 2 * p->C : (int64_t)p->B * q.chunks * 2 * p->G;
+        if (q.form == TILE) f = bwd ? (int64_t)p->B * (q.chunks + (q.chunks > 1)) * 2 * p->C : (int64_t)p->B * q.chunks * 2 * p->G;
+        else f = bwd ? (q.form == SLAB ? (int64_t)q.slab_wgs : (int64_t)p->B) * 2 * p->C : 0;
+        if (bwd) f += (int64_t)join_segments(q.form == SLAB ? q.slab_wgs : p->B) * 2 * p->C;
         if (f > most) most = f;
     }
     return most * 4;
@@ -823,7 +851,8 @@ template <int DT, int V, bool BWD> int slab_launch(const Args& a, const Plan& q,
     const size_t lds = BWD ? (size_t)256 * q.nv * 2 * V * 4 : 0;
     if (q.nv == 1) slab_kernel<DT, V, 1, BWD><<<grid, 256, lds, st>>>(a, q.s);
     else if (q.nv == 2) slab_kernel<DT, V, 2, BWD><<<grid, 256, lds, st>>>(a, q.s);
-    else slab_kernel<DT, V, 4, BWD><<<grid, 256, lds, st>>>(a, q.s);
+    else if (q.nv == 4) slab_kernel<DT, V, 4, BWD><<<grid, 256, lds, st>>>(a, q.s);
+    else if constexpr (V <= 2) slab_kernel<DT, V, 8, BWD><<<grid, 256, lds, st>>>(a, q.s);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
@@ -859,32 +888,42 @@ template <int DT, int V> int forward(Args& a, const Plan& q, hipStream_t st) {
     return XVA_OK;
 }
 
-int join(const Args& a, int items, int per_item, hipStream_t st) {
-    join_kernel<<<dim3((a.C + 31) / 32, 2), 1024, 0, st>>>(a.part, items, per_item, a.C, a.item, a.dw, a.db);
+// dw, dbias from (rows, 2, C) partial sums; `spare` holds the segments' sums where there are several
+int join(const Args& a, const float* part, int rows, float* spare, hipStream_t st) {
+    if (!a.dw && !a.db) return XVA_OK;
+    const int segs = join_segments(rows);
+    if (segs > 1) {
+        join_kernel<<<dim3((a.C + 31) / 32, 2, segs), 1024, 0, st>>>(part, rows, join_segment(rows), a.C, spare, spare + a.C, 2 * (int64_t)a.C);
+        XVA_LAUNCH_CHECK();
+        part = spare; rows = segs;
+    }
+    join_kernel<<<dim3((a.C + 31) / 32, 2), 1024, 0, st>>>(part, rows, rows, a.C, a.db, a.dw, 0);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
 
 template <int DT, int V> int backward(Args& a, const Plan& q, hipStream_t st) {
-    if (q.form == WHOLE) {
-        XVA_TRY((whole_launch<DT, V, true>(a, q, st)));
-        return a.dw || a.db ? join(a, a.B, 1, st) : XVA_OK;
-    }
-    if (q.form == SLAB) {
-        XVA_TRY((slab_launch<DT, V, true>(a, q, st)));
-        return a.dw || a.db ? join(a, q.slab_wgs, 1, st) : XVA_OK;
+    if (q.form != TILE) {
+        const int rows = q.form == SLAB ? q.slab_wgs : a.B;
+        if (q.form == WHOLE) XVA_TRY((whole_launch<DT, V, true>(a, q, st)));
+        else XVA_TRY((slab_launch<DT, V, true>(a, q, st)));
+        return join(a, a.part, rows, a.part + (int64_t)rows * 2 * a.C, st);
     }
     const dim3 grid((unsigned)(a.B * q.chunks));
     const int step = q.threads / (a.C / V);
-    a.item = a.part + (int64_t)a.B * q.chunks * 2 * a.C;
+    const int64_t parts = (int64_t)a.B * q.chunks * 2 * a.C;
+    a.item = q.chunks > 1 ? a.part + parts : a.part;
     if (q.threads <= 256) tile_dsum_kernel<DT, V, 256><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
     else tile_dsum_kernel<DT, V, 1024><<<grid, q.threads, (size_t)step * a.C * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
-    XVA_TRY(join(a, a.B, q.chunks, st));
+    if (q.chunks > 1) {
+        item_kernel<<<dim3((a.C + 31) / 32, 2, (a.B + 31) / 32), 1024, 0, st>>>(a.part, a.B, q.chunks, a.C, a.item);
+        XVA_LAUNCH_CHECK();
+    }
     if (q.threads <= 256) tile_dx_kernel<DT, V, 256><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
     else tile_dx_kernel<DT, V, 1024><<<grid, q.threads, (size_t)2 * a.G * 4, st>>>(a);
     XVA_LAUNCH_CHECK();
-    return XVA_OK;
+    return join(a, a.item, a.B, a.item + (int64_t)a.B * 2 * a.C, st);
 }
 
 int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void* stream, const char* who) {
@@ -892,7 +931,7 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     XVA_CHECK_ARG(!bwd || p->dy || p->B == 0 || p->T == 0, "%s: null gradient", who);
     hipStream_t st = (hipStream_t)stream;
     Plan q = {};
-    XVA_CHECK_ARG(make_plan(p, aligned(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
+    XVA_CHECK_ARG(make_plan(p, allowed(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
     XVA_CHECK_ARG(q.form != TILE || (int64_t)p->B * q.chunks < (1ll << 31), "%s: %d items of %d rows", who, p->B, p->T);
     if (ws_bytes < workspace(p, bwd)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)workspace(p, bwd)); return XVA_ERR_WS; }
     if (p->B == 0 || p->T == 0) {
@@ -904,11 +943,12 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     }
     Args a = args_of(p, q);
     a.part = (float*)ws;
-    const bool v1 = q.v == 1;
 #define GN(DT, V) (bwd ? backward<DT, V>(a, q, st) : forward<DT, V>(a, q, st))
-    if (p->dtype == 0) return v1 ? GN(0, 1) : GN(0, 4);
-    if (p->dtype == 1) return v1 ? GN(1, 1) : GN(1, 8);
-    return v1 ? GN(2, 1) : GN(2, 8);
+#define GNV(DT, WIDE) return q.v == WIDE ? GN(DT, WIDE) : (q.v == 2 ? GN(DT, 2) : GN(DT, 1))
+    if (p->dtype == 0) GNV(0, 4);
+    if (p->dtype == 1) GNV(1, 8);
+    GNV(2, 8);
+#undef GNV
 #undef GN
 }
 }   // namespace

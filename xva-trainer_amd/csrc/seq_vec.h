@@ -59,22 +59,28 @@ inline int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-// V elements as they lie in memory (1 element, or 16 bytes), kept packed until they are needed
+// V elements as they lie in memory (1 or 2 elements, or 16 bytes), kept packed until they are needed
 template <int DT, int V> struct Packed {
-    static_assert(V == 1 || V == (DT == 0 ? 4 : 8), "one element or 16 bytes");
-    typedef typename std::conditional<V != 1, u32x4, typename std::conditional<DT == 0, uint32_t, uint16_t>::type>::type T;
+    static_assert(V == 1 || V == 2 || V == (DT == 0 ? 4 : 8), "one or two elements, or 16 bytes");
+    static constexpr int BYTES = V * (DT == 0 ? 4 : 2);
+    typedef typename std::conditional<BYTES == 16, u32x4, typename std::conditional<BYTES == 8, u32x2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type T;
     T v;
     __device__ __forceinline__ void load(const void* base, int64_t off) {
         v = *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off * (DT == 0 ? 4 : 2));
     }
-    __device__ __forceinline__ void clear() { if constexpr (V == 1) v = 0; else v = (u32x4){0, 0, 0, 0}; }
+    __device__ __forceinline__ void clear() {
+        if constexpr (BYTES == 16) v = (u32x4){0, 0, 0, 0};
+        else if constexpr (BYTES == 8) v = (u32x2){0, 0};
+        else v = 0;
+    }
     __device__ __forceinline__ void get(float (&f)[V]) const {
         if constexpr (V == 1) {
             if constexpr (DT == 0) f[0] = __uint_as_float(v); else f[0] = xva_glds::ld16<DT == 2>(&v, 0);
         } else if constexpr (DT == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
-        } else {
+            for (int e = 0; e < V; ++e) f[e] = __uint_as_float(v[e]);
+        } else if constexpr (V == 2) unpack2<DT == 2>(v, f[0], f[1]);
+        else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) unpack2<DT == 2>(v[e], f[2 * e], f[2 * e + 1]);
         }
