@@ -106,6 +106,21 @@ def test_long_rows(causal, Tq, Tk):
     _run(*_data(2, Tq, Tk, 4, 2, 64, "bf16", seed=1), causal=causal, kl=torch.tensor([Tk, Tk // 3], dtype=torch.int32))
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ragged", [None, "some", "empty"])
+@pytest.mark.parametrize("B,Tq,Tk,H,Hk,d", [(2, 700, 300, 4, 2, 40), (1, 1300, 130, 2, 1, 64), (3, 400, 700, 1, 1, 8), (1, 2050, 64, 3, 1, 24), (2, 90, 1000, 8, 2, 48)])
+def test_key_blocks_in_pieces(causal, ragged, B, Tq, Tk, H, Hk, d):
+    """Few key blocks, many query tiles: dK and dV are summed over several workgroups."""
+    _run(*_data(B, Tq, Tk, H, Hk, d, "bf16", seed=5), ql=lengths(B, Tq, ragged), kl=lengths(B, Tk, ragged), causal=causal)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_numbers_of_a_head_of_any_sign(dt):
+    q, k, v, lam, dout = _data(2, 200, 200, 6, 3, 32, dt, seed=6)
+    lam.copy_(torch.tensor([0.0, -0.7, 1.5, -0.0, 1e-3, -3.0]))
+    _run(q, k, v, lam, dout, causal=True)
+
+
 @pytest.mark.parametrize("size,scale", [(4.0, None), (1.0, 2.0), (0.05, None)])
 def test_sharp_and_flat_rows(size, scale):
     """Scores of hundreds (one key takes all), and of nothing (all keys alike)."""

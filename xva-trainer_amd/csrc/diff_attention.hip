@@ -35,6 +35,7 @@ struct Args {
     int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
     int B, Tq, Tk, H, Hk, share, d, causal;
     float scale, c;                               // c = scale log2 e
+    float* part; int pieces, piece;               // dkv: workgroups of a key block, and the tiles that one of them takes (see there)
 };
 // contiguous results: out-of-line maps (2, B, Tq, H, 2 d), dq (B, Tq, H, 2, d), dk (B, Tk, Hk, 2, d), dv (B, Tk, Hk, 2 d)
 // lse (2, B, H, Tq): minus the row's logarithm of sums, in units of unscaled scores (-inf: the row sees nothing), so P = exp2(c (S + lse)); D (2, B, H, Tq): -D_1
@@ -587,9 +588,22 @@ __global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
     if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
 }
 
+// A key block's 64-query tiles: of each query head that shares the keys, `per_head` from tile `t0` on
+struct KeyBlock {
+    int t0, per_head, all;
+    __device__ __forceinline__ KeyBlock(const Args& a, int k0, int ql, int kl) {
+        const int first = a.causal ? max(k0 - (kl - ql), 0) : 0;       // queries that see a key of the block: from here on
+        t0 = first / 64;
+        per_head = k0 < kl && first < ql ? (ql + 63) / 64 - t0 : 0;
+        all = per_head * a.share;
+    }
+};
+
 // dK, dV of 64 keys of a key head over the query heads that share it and their 64-query tiles.  Waves: two halves of the keys x two halves of a tile's
 // queries; the queries' halves are added at the end through LDS.  (128 keys to a workgroup, 32 to a wave over all rows: half as many workgroups, which
 // leaves long causal sequences waiting for the first keys' ones.)
+// Where key blocks are few, or causal ones of very different length, the tiles of a key block are cut into pieces of equal length, one to a workgroup; a second
+// kernel adds the pieces' fp32 sums in order (rows of [2][d] of dK and [2 d] of dV).
 template <int D16, bool F16>
 __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     using S = Shape<D16>;
@@ -599,21 +613,20 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     constexpr int STAT = 2 * NI * TILE;                                                        // {Q dO | lse1 lse2 D1 D2} of the even and of the odd tiles
     __shared__ __attribute__((aligned(1024))) uint8_t even[STAT + 1024], odd[STAT + 1024];
     __shared__ __attribute__((aligned(16))) uint8_t away_raw[AWAY ? AWAY * 4096 : 16];
-    // Under `causal` the first keys are seen by most queries: they start first.  Where all workgroups are on the card at once, two to a CU, the second of a CU
-    // is one from the other end, so that each CU has as much to do as another.
-    unsigned id = blockIdx.x;
-    if (a.causal && gridDim.x <= 512 && id >= 256) id = gridDim.x - 1 - (id - 256);
-    const int kblk = id / (unsigned)(a.B * a.Hk), bh = id % (unsigned)(a.B * a.Hk);
+    // (under `causal` the first keys are seen by most queries: they start first)
+    const unsigned heads = a.B * a.Hk, bh = blockIdx.x % heads, rest = blockIdx.x / heads;
+    const unsigned kblks = (a.Tk + 63) / 64;
+    const int piece = rest / kblks, kblk = rest - piece * kblks;
     const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15, t = wave >> 1;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql;
     const int wkey = k0 + (wave & 1) * 32, w = 2 * a.d;
     Lane fr(lane, t * 4096);
-    // queries that see a key of the workgroup: from `first` on
-    const int first = a.causal ? max(k0 - off, 0) : 0;
-    const bool any = k0 < kl && first < ql;
-    const int t0 = first / 64, per_head = any ? (ql + 63) / 64 - t0 : 0, total = per_head * a.share;
+    const KeyBlock kb(a, k0, ql, kl);
+    const bool any = kb.all > 0;
+    const int begin = piece * a.piece, total = min(kb.all - begin, a.piece);
+    if (piece > 0 && total <= 0) return;
     bf16x8 kf[2][2][S::KH], vf[2][S::VH];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -648,13 +661,14 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)min(ql - row0, 64) * 4u, 0x00027000),
                                                  (XVA_LDS void*)(to + STAT + wave * 256), 4, min(lane_, ql - row0 - 1) * 4, 0, 0, 0);
     };
-    if (total) fetch(0, t0 * 64, (XVA_LDS uint8_t*)even);
+    // from the last rows on, which all key blocks see, and by turns over the heads: workgroups that start together read the same tiles at about the same time
+    int qtile = kb.t0 + kb.per_head - 1 - begin / a.share, hs = begin % a.share;
+    if (any) fetch(hs, qtile * 64, (XVA_LDS uint8_t*)even);
     __syncthreads();
-    int hs = 0, qtile = t0;
     auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         const int row0 = qtile * 64;
-        const float lam = uniform(a.lam, hk * a.share + hs);
-        if (++qtile == t0 + per_head) { qtile = t0; ++hs; }
+        const float lam = uniform(a.lam, hk * a.share + hs), loglam = __log2f(fabsf(lam)), minus = lam < 0.f ? 1.f : -1.f;
+        if (++hs == a.share) { hs = 0; --qtile; }
         if (it + 1 < total) fetch(hs, qtile * 64, next);
         const int wrow = row0 + t * 32;                       // this wave's 32 rows
         const bool whole = wrow + 32 <= ql && wkey + 32 <= kl && (!a.causal || wkey + 31 <= wrow + off);      // every row sees every key
@@ -695,15 +709,16 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
                             s[1][kt][r] = ok ? s[1][kt][r] : -INFINITY;
                         }
                 }
-                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768);
+                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768) * minus;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = -lam * exp2_(s[1][kt][r] * a.c), x = dp[kt][r];
+                        // (|lam| in the exponent, its sign in the sums: no product more than without it)
+                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = exp2_(__builtin_fmaf(s[1][kt][r], a.c, loglam)), x = dp[kt][r];
                         s[0][kt][r] = p1 * x;
-                        s[1][kt][r] = p2 * (x + dD[r]);
-                        dp[kt][r] = p1 + p2;
+                        s[1][kt][r] = p2 * __builtin_fmaf(x, minus, dD[r]);
+                        dp[kt][r] = __builtin_fmaf(p2, minus, p1);
                     }
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -748,7 +763,17 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
         }
         __syncthreads();
         const int key = wkey + kt * 16 + ie;
-        if (t == 0 && key < a.Tk) {
+        if (t == 0 && key < a.Tk && kb.all > a.piece) {
+            float* row = a.part + (((int64_t)piece * a.B + b) * a.Tk + key) * a.Hk * 4 * a.d + hk * 4 * a.d;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int dt = 0; dt < S::DT; ++dt)
+                    if (dt * 16 + ge * 4 < a.d) *reinterpret_cast<f32x4*>(row + m * a.d + dt * 16 + ge * 4) = dk[m][kt][dt] + xch[(m * S::DT + dt) * 64];
+#pragma unroll
+            for (int dt = 0; dt < S::VT; ++dt)
+                if (dt * 16 + ge * 4 < w) *reinterpret_cast<f32x4*>(row + w + dt * 16 + ge * 4) = dv[kt][dt] + xch[(2 * S::DT + dt) * 64];
+        } else if (t == 0 && key < a.Tk) {
             const int64_t row = ((int64_t)b * a.Tk + key) * a.Hk + hk;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
@@ -761,6 +786,21 @@ __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
         }
         __syncthreads();
     }
+}
+
+// the pieces of a key's dK and dV, four columns to a thread
+template <bool F16>
+__global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.Tk * a.Hk, row = id / a.d;
+    if (row >= rows) return;
+    const int col = (int)(id - row * a.d) * 4, w = 2 * a.d;
+    const int b = (int)(row / ((int64_t)a.Tk * a.Hk)), key = (int)(row / a.Hk - (int64_t)b * a.Tk);
+    const KeyBlock kb(a, key & ~63, len_of(a.ql, b, a.Tq), len_of(a.kl, b, a.Tk));
+    if (kb.all <= a.piece) return;
+    f32x4 v = ZERO4;
+    for (int p = 0; p * a.piece < kb.all; ++p) v += *reinterpret_cast<const f32x4*>(a.part + (p * rows + row) * 2 * w + col);
+    if (col < w) xva_attn::st4<F16>(a.dk + row * w + col, v, a.scale);
+    else xva_attn::st4<F16>(a.dv + row * w + col - w, v, 1.f);
 }
 
 // dq of 128 queries of a head, 32 to a wave, and their part of dlam
@@ -981,6 +1021,24 @@ template <int D16, bool F16> int few(const Args& a, const Few& f, float* part, h
     }
     return XVA_OK;
 }
+// Pieces of dkv's key blocks.  512 workgroups are on the card at once: key blocks fewer than that, and fewer than twice that where `causal` makes their lengths differ,
+// are cut so that the pieces make 512 equal ones in all, four tiles long at least (a piece's sums are written and read once more).  Uncut | cut, us, heads of 64
+// (16 heads on 4 keys', 8192 positions, causal: 865 | 690 + 11; 4 heads, 4096, all pairs: 125 | 91 + 8; 5 items of 2635 on 391, one head: 90 | 21 + 6; pieces of
+// half that length: 751 + 16, 97 + 13, 21 + 6).
+struct Pieces { int pieces, piece; };
+Pieces dkv_plan(const xva_diff_attention_args* p) {
+    const int64_t wgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64), most = (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64);
+    Pieces s = {1, (int)(most < 1 ? 1 : most)};
+    if (wgs == 0 || wgs >= (p->causal ? 1024 : 512)) return s;
+    int64_t piece = ((p->causal ? most * wgs / 2 : most * wgs) + 511) / 512;
+    if (piece < 4) piece = 4;
+    if (piece < most) { s.piece = (int)piece; s.pieces = (int)((most + piece - 1) / piece); }
+    return s;
+}
+int64_t dkv_floats(const xva_diff_attention_args* p) {
+    const Pieces s = dkv_plan(p);
+    return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tk * p->Hk * 4 * p->d : 0;
+}
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
     const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128));
     if (train) fwd_kernel<D16, F16, true><<<grid, 256, 0, st>>>(a);
@@ -994,8 +1052,12 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
     rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
     if (a.Tk > 0) {
-        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64)), 256, 0, st>>>(a);
+        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64) * a.pieces), 256, 0, st>>>(a);
         XVA_LAUNCH_CHECK();
+        if (a.pieces > 1) {
+            dkv_join_kernel<F16><<<(unsigned)(((int64_t)a.B * a.Tk * a.Hk * a.d + 255) / 256), 256, 0, st>>>(a);
+            XVA_LAUNCH_CHECK();
+        }
     }
     dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb), 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
@@ -1005,12 +1067,12 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
 }
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
     if (!bwd) return few_floats(p, few_plan(p)) * 4;
-    return ((int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128)) * 4;
+    return (dkv_floats(p) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128)) * 4;
 }
 }   // namespace
 
 extern "C" int64_t xva_diff_attention_workspace_bytes(const xva_diff_attention_args* p, int backward_pass) {
-    return p && p->B >= 0 && p->Tq >= 0 && p->H >= 1 ? workspace(p, backward_pass != 0) : -1;
+    return p && p->B >= 0 && p->Tq >= 0 && p->Tk >= 0 && p->H >= 1 && p->Hk >= 1 && p->H % p->Hk == 0 ? workspace(p, backward_pass != 0) : -1;
 }
 
 #define XVA_DIFF_BY_SHAPE(call)                                                          \
@@ -1046,7 +1108,10 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
         return XVA_ERR_WS;
     }
     Args a = args_of(p);
-    a.D = (float*)ws;
+    const Pieces s = dkv_plan(p);
+    a.pieces = s.pieces; a.piece = s.piece;
+    a.part = (float*)ws;
+    a.D = a.part + dkv_floats(p);
     a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
 #define CALL(D16, F16) backward<D16, F16>(a, p->dlam, (hipStream_t)stream)
     XVA_DIFF_BY_SHAPE(CALL)
