@@ -114,6 +114,20 @@ def test_key_blocks_in_pieces(causal, ragged, B, Tq, Tk, H, Hk, d):
     _run(*_data(B, Tq, Tk, H, Hk, d, "bf16", seed=5), ql=lengths(B, Tq, ragged), kl=lengths(B, Tk, ragged), causal=causal)
 
 
+@pytest.mark.parametrize("Tq,Tk", [(200, 900), (300, 100), (4, 900), (1, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_a_query_that_is_no_number_stays_one(Tq, Tk, causal):
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(1, Tq, Tk, 2, 1, 32, "bf16", seed=7)
+    with torch.no_grad():
+        clean = S.differential_attention(q, k, v, lam, causal=causal)
+        q[0, Tq - 1, 1] = float("nan")
+        out = S.differential_attention(q, k, v, lam, causal=causal)
+    assert out[0, Tq - 1, 1].isnan().all()
+    out[0, Tq - 1, 1] = clean[0, Tq - 1, 1]
+    assert torch.equal(out, clean)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_numbers_of_a_head_of_any_sign(dt):
     q, k, v, lam, dout = _data(2, 200, 200, 6, 3, 32, dt, seed=6)

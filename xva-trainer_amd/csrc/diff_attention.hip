@@ -35,7 +35,9 @@ struct Args {
     int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
     int B, Tq, Tk, H, Hk, share, d, causal;
     float scale, c;                               // c = scale log2 e
-    float* part; int pieces, piece;               // dkv: workgroups of a key block, and the tiles that one of them takes (see there)
+    // dkv: workgroups of a key block, and the tiles that one of them takes; forward and dq: the same of a query block (see dkv_kernel)
+    float* part; int pieces, piece;
+    float* qpart; int qpieces, qpiece;
 };
 // contiguous results: out-of-line maps (2, B, Tq, H, 2 d), dq (B, Tq, H, 2, d), dk (B, Tk, Hk, 2, d), dv (B, Tk, Hk, 2 d)
 // lse (2, B, H, Tq): minus the row's logarithm of sums, in units of unscaled scores (-inf: the row sees nothing), so P = exp2(c (S + lse)); D (2, B, H, Tq): -D_1
@@ -128,16 +130,31 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float uniform(const float* p, int i) { return reinterpret_cast<const __attribute__((address_space(4))) float*>((uintptr_t)p)[i]; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A workgroup's query block of a (item, head), and its piece of the keys.  The last blocks see most keys under `causal`: they start first.
+struct QueryBlock {
+    int bh, blk, piece, blocks;
+    __device__ __forceinline__ QueryBlock(const Args& a) {
+        const unsigned heads = a.B * a.H, rest = blockIdx.x / heads;
+        bh = blockIdx.x - rest * heads;
+        blocks = (a.Tq + 127) / 128;
+        piece = rest / (unsigned)blocks;
+        blk = blocks - 1 - (rest - piece * blocks);
+    }
+};
+// 64-key tiles that some query of the block from q0 on sees
+__device__ __forceinline__ int key_tiles(const Args& a, int q0, int ql, int kl) {
+    if (q0 >= ql) return 0;
+    return ((a.causal ? max(min(kl, min(q0 + 127, ql - 1) + kl - ql + 1), 0) : kl) + 63) / 64;
+}
+
 // ================================================================================ forward ====
 template <int D16, bool F16, bool TRAIN>
 __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
     __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];       // {K V} of the even and of the odd tiles (see XVA_TWO_BUFFERS)
-    // the last query blocks see most keys under `causal`: they start first
-    const int nqb = gridDim.x / (a.B * a.H);
-    const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
-    const int h = bh % a.H, b = bh / a.H, q0 = qblk * 128;
+    const QueryBlock qb(a);
+    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
@@ -145,12 +162,12 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
     const uint16_t* qp = a.q + b * a.qb + h * a.qh;
     const int wrow = q0 + wave * 32;
-    // keys that some query of the workgroup / of the wave sees, and that every query of the wave sees
+    // keys that some query of the wave sees, and that every query of the wave sees
     auto seen_by = [&](int row) { return a.causal ? max(min(kl, row + off + 1), 0) : kl; };
-    const int wg_keys = q0 < ql ? seen_by(min(q0 + 127, ql - 1)) : 0;
     const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
     const int whole_keys = seen_by(wrow);
-    const int tiles = (wg_keys + 63) / 64;
+    const int all = key_tiles(a, q0, ql, kl), first = qb.piece * a.qpiece, tiles = min(all - first, a.qpiece);
+    if (qb.piece > 0 && tiles <= 0) return;
     Lane fr(lane, 0);
     bf16x8 qf[2][2][S::KH];
     // keys that row tile rt's row of this lane sees
@@ -162,7 +179,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = tiles ? ld_edge(qr + m * a.qm, kh * 32 + g * 8, a.d) : ld_edge(qr, 1, 0);
+            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = tiles > 0 ? ld_edge(qr + m * a.qm, kh * 32 + g * 8, a.d) : ld_edge(qr, 1, 0);
     }
     f32x4 o[2][2][S::VT];
     float mx[2][2], sum[2][2];
@@ -174,14 +191,16 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
 #pragma unroll
             for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] = ZERO4;
         }
-    if (tiles) {
+    if (tiles > 0) {
         const Src<NI> src(lane, wave, a.d, a.km);
-        src.fetch_qk(kp, a.kt, a.km, a.d, kl, (XVA_LDS uint8_t*)even, wave);
-        src.fetch_v(vp, a.vt, a.d, kl, (XVA_LDS uint8_t*)even + NI * TILE, wave);
+        const int row0 = first * 64;
+        src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, (XVA_LDS uint8_t*)even, wave);
+        src.fetch_v(vp + row0 * a.vt, a.vt, a.d, kl - row0, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
-    auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
-        if (jb + 1 < tiles) {
+    auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
+        const int jb = first + it;
+        if (it + 1 < tiles) {
             const Src<NI> src(again(lane), wave, a.d, a.km);
             const int row0 = (jb + 1) * 64;
             src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, next, wave);
@@ -266,14 +285,26 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
         const bool seen = limit(rt) > 0;
-        float inv[2];
+        float inv[2], total[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             float l = sum[m][rt];
             l += __shfl_xor(l, 16, 64);
             l += __shfl_xor(l, 32, 64);
+            total[m] = l;
             inv[m] = seen ? 1.f / l : 0.f;
-            if (TRAIN && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m][rt] + __log2f(l) / a.c) : -INFINITY;
+            if (TRAIN && all <= a.qpiece && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m][rt] + __log2f(l) / a.c) : -INFINITY;
+        }
+        if (all > a.qpiece) {                                  // a piece: (max, sum) of both maps and the sums as they are, for fwd_join_kernel
+            if (row >= a.Tq) continue;
+            float* to = a.qpart + ((((int64_t)qb.piece * a.B + b) * a.Tq + row) * a.H + h) * (2 * w + 4);
+            if (g == 0) *reinterpret_cast<f32x4*>(to) = (f32x4){mx[0][rt], total[0], mx[1][rt], total[1]};
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int dt = 0; dt < S::VT; ++dt)
+                    if (dt * 16 + g * 4 < w) *reinterpret_cast<f32x4*>(to + 4 + m * w + dt * 16 + g * 4) = o[m][rt][dt];
+            continue;
         }
         if (row >= a.Tq) continue;
         uint16_t* out = a.out + b * a.ob + row * a.ot + h * a.oh;
@@ -295,6 +326,50 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
                 *reinterpret_cast<uint2*>(m0 + col) = make_uint2(pack2<F16>(u[0], u[1]), pack2<F16>(u[2], u[3]));
                 *reinterpret_cast<uint2*>(m0 + plane + col) = make_uint2(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]));
             }
+        }
+    }
+}
+
+// joins the pieces of a row: four columns to a thread
+template <bool F16>
+__global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.Tq * a.H;
+    const int w = 2 * a.d, quads = w / 4;
+    const int64_t R = id / quads;
+    if (R >= rows) return;
+    const int col = (int)(id - R * quads) * 4, h = (int)(R % a.H), b = (int)(R / ((int64_t)a.Tq * a.H)), row = (int)(R / a.H - (int64_t)b * a.Tq);
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), all = key_tiles(a, row & ~127, ql, kl);
+    if (all <= a.qpiece) return;
+    const float* from = a.qpart + R * (2 * w + 4);
+    const int64_t step = rows * (2 * w + 4);
+    const int n = (all + a.qpiece - 1) / a.qpiece;
+    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    f32x4 o[2] = {ZERO4, ZERO4};
+#pragma unroll 4
+    for (int p = 0; p < n; ++p)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) mx[m] = fmaxf(mx[m], from[p * step + 2 * m]);
+#pragma unroll 4
+    for (int p = 0; p < n; ++p) {
+        const f32x4 st = *reinterpret_cast<const f32x4*>(from + p * step);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            // (a piece of which nothing is seen: its sums are zero, or no numbers where its scores are none)
+            const float by = st[2 * m] == -INFINITY ? 0.f : exp2_((st[2 * m] - mx[m]) * a.c);
+            sum[m] += st[2 * m + 1] * by;
+            o[m] += *reinterpret_cast<const f32x4*>(from + p * step + 4 + m * w + col) * by;
+        }
+    }
+    const bool seen = row < ql && (!a.causal || row + kl - ql >= 0);
+    const float lam = a.lam[h];
+    const f32x4 u = seen ? o[0] * (1.f / sum[0]) : ZERO4, v = seen ? o[1] * (1.f / sum[1]) : ZERO4;
+    xva_attn::st4<F16>(a.out + b * a.ob + row * a.ot + h * a.oh + col, seen ? u - v * lam : ZERO4, 1.f);
+    if (a.maps) {
+        xva_attn::st4<F16>(a.maps + R * w + col, u, 1.f);
+        xva_attn::st4<F16>(a.maps + (rows + R) * w + col, v, 1.f);
+        if (col < 8) {
+            const int m = col >> 2;
+            a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m] + __log2f(sum[m]) / a.c) : -INFINITY;
         }
     }
 }
@@ -472,7 +547,7 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
 #pragma unroll
             for (int v = 0; v < 4; ++v) rtop = fmaxf(rtop, stat[v][m][r][0]);
 #pragma unroll
-            for (int v = 0; v < 4; ++v) l += stat[v][m][r][0] == -INFINITY ? 0.f : stat[v][m][r][1] * exp2_((stat[v][m][r][0] - rtop) * a.c);
+            for (int v = 0; v < 4; ++v) l += stat[v][m][r][1] * (stat[v][m][r][0] == -INFINITY ? 0.f : exp2_((stat[v][m][r][0] - rtop) * a.c));
 #pragma unroll
             for (int e = 0; e < W / 16; ++e) acc[e] = x[row * W + col + e] + x[(16 + row) * W + col + e] + x[(32 + row) * W + col + e] + x[(48 + row) * W + col + e];
             if (r < R && col < w) {
@@ -483,10 +558,10 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
                     for (int e = 0; e < W / 16; ++e)
                         if (col + e < w) to[4 * R + (int64_t)(m * R + r) * w + col + e] = acc[e];
                 } else {
-                    const float inv = rtop == -INFINITY ? 0.f : 1.f / l;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;                // (nothing seen; scores that are no numbers have a sum, which is none)
                     if (m == 0) {
 #pragma unroll
-                        for (int e = 0; e < W / 16; ++e) first[e] = rtop == -INFINITY ? 0.f : acc[e] * inv;
+                        for (int e = 0; e < W / 16; ++e) first[e] = acc[e] * inv;
                     } else {
                         const int hs = r / a.Tq, h = hk * a.share + hs;
                         const float by = a.lam[h];
@@ -494,8 +569,8 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
 #pragma unroll
                         for (int e = 0; e < W / 16; e += 2)
                             if (col + e < w)
-                                *reinterpret_cast<uint32_t*>(out + col + e) = pack2<F16>(first[e] - by * (rtop == -INFINITY ? 0.f : acc[e] * inv),
-                                                                                         first[e + 1] - by * (rtop == -INFINITY ? 0.f : acc[e + 1] * inv));
+                                *reinterpret_cast<uint32_t*>(out + col + e) = pack2<F16>(first[e] - by * acc[e] * inv,
+                                                                                         first[e + 1] - by * acc[e + 1] * inv);
                     }
                 }
             }
@@ -602,8 +677,8 @@ struct KeyBlock {
 // dK, dV of 64 keys of a key head over the query heads that share it and their 64-query tiles.  Waves: two halves of the keys x two halves of a tile's
 // queries; the queries' halves are added at the end through LDS.  (128 keys to a workgroup, 32 to a wave over all rows: half as many workgroups, which
 // leaves long causal sequences waiting for the first keys' ones.)
-// Where key blocks are few, or causal ones of very different length, the tiles of a key block are cut into pieces of equal length, one to a workgroup; a second
-// kernel adds the pieces' fp32 sums in order (rows of [2][d] of dK and [2 d] of dV).
+// Where key blocks are few, or causal ones of very different length, the tiles of a key block are cut into pieces, one to a workgroup; a second kernel adds the pieces'
+// fp32 sums in order (rows of [2][d] of dK and [2 d] of dV).  Query blocks' keys are cut the same way in the forward pass and in dq.
 template <int D16, bool F16>
 __global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
     using S = Shape<D16>;
@@ -809,9 +884,8 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
     __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];
-    const int nqb = gridDim.x / (a.B * a.H);
-    const int qblk = nqb - 1 - blockIdx.x / (a.B * a.H), bh = blockIdx.x % (a.B * a.H);
-    const int h = bh % a.H, b = bh / a.H, q0 = qblk * 128;
+    const QueryBlock qb(a);
+    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
@@ -819,10 +893,13 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
     const int wrow = q0 + wave * 32, w = 2 * a.d;
     auto seen_by = [&](int row) { return a.causal ? max(min(kl, row + off + 1), 0) : kl; };
-    const int wg_keys = q0 < ql ? seen_by(min(q0 + 127, ql - 1)) : 0;
     const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
     const int whole_keys = seen_by(wrow);
-    const int tiles = (wg_keys + 63) / 64;
+    const int all = key_tiles(a, q0, ql, kl), first = qb.piece * a.qpiece, tiles = min(all - first, a.qpiece);
+    if (qb.piece > 0 && tiles <= 0) {
+        if (threadIdx.x == 0) a.dlam_part[(((int64_t)h * a.B + b) * qb.blocks + qb.blk) * a.qpieces + qb.piece] = 0.f;
+        return;
+    }
     Lane fr(lane, 0);
     bf16x8 qf[2][2][S::KH], of[2][S::VH];
     int limit[2];
@@ -834,14 +911,14 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
-            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = ld_edge(a.q + b * a.qb + h * a.qh + m * a.qm + safe * a.qt, kh * 32 + g * 8, tiles ? a.d : 0);
+            for (int kh = 0; kh < S::KH; ++kh) qf[m][rt][kh] = ld_edge(a.q + b * a.qb + h * a.qh + m * a.qm + safe * a.qt, kh * 32 + g * 8, tiles > 0 ? a.d : 0);
             const int64_t at = (((int64_t)m * a.B + b) * a.H + h) * a.Tq + safe;
             L[m][rt] = -a.lse[at] * a.c; Dr[m][rt] = a.D[at];
         }
         Dr[0][rt] = -Dr[0][rt];
         Dr[1][rt] = Dr[0][rt] - Dr[1][rt];
 #pragma unroll
-        for (int kh = 0; kh < S::VH; ++kh) of[rt][kh] = ld_edge(a.dout + b * a.gb + h * a.gh + safe * a.gt, kh * 32 + g * 8, tiles ? w : 0);
+        for (int kh = 0; kh < S::VH; ++kh) of[rt][kh] = ld_edge(a.dout + b * a.gb + h * a.gh + safe * a.gt, kh * 32 + g * 8, tiles > 0 ? w : 0);
     }
     f32x4 dq[2][2][S::DT];
     float dl = 0.f;
@@ -851,14 +928,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
         for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
             for (int dt = 0; dt < S::DT; ++dt) dq[m][rt][dt] = ZERO4;
-    if (tiles) {
+    if (tiles > 0) {
         const Src<NI> src(lane, wave, a.d, a.km);
-        src.fetch_qk(kp, a.kt, a.km, a.d, kl, (XVA_LDS uint8_t*)even, wave);
-        src.fetch_v(vp, a.vt, a.d, kl, (XVA_LDS uint8_t*)even + NI * TILE, wave);
+        const int row0 = first * 64;
+        src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, (XVA_LDS uint8_t*)even, wave);
+        src.fetch_v(vp + row0 * a.vt, a.vt, a.d, kl - row0, (XVA_LDS uint8_t*)even + NI * TILE, wave);
     }
     __syncthreads();
-    auto tile = [&](const int jb, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
-        if (jb + 1 < tiles) {
+    auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
+        const int jb = first + it;
+        if (it + 1 < tiles) {
             const Src<NI> src(again(lane), wave, a.d, a.km);
             const int row0 = (jb + 1) * 64;
             src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, next, wave);
@@ -932,6 +1011,15 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
         if (row >= a.Tq) continue;
+        if (all > a.qpiece) {                                  // a piece, for dq_join_kernel
+            float* to = a.qpart + ((((int64_t)qb.piece * a.B + b) * a.Tq + row) * a.H + h) * w;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int dt = 0; dt < S::DT; ++dt)
+                    if (dt * 16 + g * 4 < a.d) *reinterpret_cast<f32x4*>(to + m * a.d + dt * 16 + g * 4) = dq[m][rt][dt];
+            continue;
+        }
         uint16_t* dst = a.dq + (((int64_t)b * a.Tq + row) * a.H + h) * w;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
@@ -945,7 +1033,22 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     for (int o = 32; o > 0; o >>= 1) dl += __shfl_xor(dl, o, 64);
     if (lane == 0) red[wave] = dl;
     __syncthreads();
-    if (threadIdx.x == 0) a.dlam_part[((int64_t)h * a.B + b) * nqb + qblk] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) a.dlam_part[(((int64_t)h * a.B + b) * qb.blocks + qb.blk) * a.qpieces + qb.piece] = red[0] + red[1] + red[2] + red[3];
+}
+
+// the pieces of a row's dq, four columns to a thread
+template <bool F16>
+__global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.B * a.Tq * a.H;
+    const int w = 2 * a.d, quads = w / 4;
+    const int64_t R = id / quads;
+    if (R >= rows) return;
+    const int col = (int)(id - R * quads) * 4, h = (int)(R % a.H), b = (int)(R / ((int64_t)a.Tq * a.H)), row = (int)(R / a.H - (int64_t)b * a.Tq);
+    const int all = key_tiles(a, row & ~127, len_of(a.ql, b, a.Tq), len_of(a.kl, b, a.Tk));
+    if (all <= a.qpiece) return;
+    f32x4 v = ZERO4;
+    for (int p = 0; p * a.qpiece < all; ++p) v += *reinterpret_cast<const f32x4*>(a.qpart + (p * rows + R) * w + col);
+    xva_attn::st4<F16>(a.dq + R * w + col, v, col < a.d ? a.scale : -a.lam[h] * a.scale);
 }
 
 // dlam[h] = - sum of the head's parts, in a fixed order
@@ -1021,29 +1124,47 @@ template <int D16, bool F16> int few(const Args& a, const Few& f, float* part, h
     }
     return XVA_OK;
 }
-// Pieces of dkv's key blocks.  512 workgroups are on the card at once: key blocks fewer than that, and fewer than twice that where `causal` makes their lengths differ,
-// are cut so that the pieces make 512 equal ones in all, four tiles long at least (a piece's sums are written and read once more).  Uncut | cut, us, heads of 64
-// (16 heads on 4 keys', 8192 positions, causal: 865 | 690 + 11; 4 heads, 4096, all pairs: 125 | 91 + 8; 5 items of 2635 on 391, one head: 90 | 21 + 6; pieces of
-// half that length: 751 + 16, 97 + 13, 21 + 6).
+// Pieces of the tiles that a workgroup would walk over: 512 workgroups are on the card at once, and `wgs` are fewer than that, or `causal` makes their lengths (up to
+// `most` tiles) differ.  All pairs: as many pieces as fill the card.  `causal`: pieces of one length, 512 in all.  Four tiles long at least; a piece's sums are written
+// and read once more, so the cut pays where workgroups are at most `few`, or `causal` ones long and less than `uneven`.
+// Uncut | cut, us, with the joining kernel:
+//   dkv, heads of 64: 16 heads on 4 keys', 8192 positions, causal (512 workgroups) 865 | 701 (pieces of half that length 767); 4 heads, 4096, all pairs (256) 125 | 99
+//   (half that length 110); 5 items of 2635 on 391, one head (35) 90 | 27
+//   forward + dq: one item of 860, 4 heads of 64 (28) 77 | 46; 10 items of 232 on 3397, 3 heads of 48 (60) 228 | 85; 6 items of 860, 4 heads of 32 (168) 64 | 62; 8 of
+//   them (224) 65 | 72; 8 heads of 64, 4096, causal (256) 286 | 227; 12 items of 860, 4 heads of 32, causal (336, of 14 tiles) 66 | 76
 struct Pieces { int pieces, piece; };
-Pieces dkv_plan(const xva_diff_attention_args* p) {
-    const int64_t wgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64), most = (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64);
+Pieces pieces_of(int64_t wgs, int64_t most, bool causal, int few, int uneven) {
     Pieces s = {1, (int)(most < 1 ? 1 : most)};
-    if (wgs == 0 || wgs >= (p->causal ? 1024 : 512)) return s;
-    int64_t piece = ((p->causal ? most * wgs / 2 : most * wgs) + 511) / 512;
+    if (wgs == 0 || wgs > (causal && most >= 32 ? uneven : few)) return s;
+    int64_t piece = causal ? (most * wgs + 1023) / 1024 : (most + 512 / wgs - 1) / (512 / wgs);
     if (piece < 4) piece = 4;
     if (piece < most) { s.piece = (int)piece; s.pieces = (int)((most + piece - 1) / piece); }
     return s;
+}
+Pieces dkv_plan(const xva_diff_attention_args* p) {
+    return pieces_of((int64_t)p->B * p->Hk * ((p->Tk + 63) / 64), (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64), p->causal, 256, 768);
+}
+Pieces query_plan(const xva_diff_attention_args* p) {
+    return pieces_of((int64_t)p->B * p->H * ((p->Tq + 127) / 128), (p->Tk + 63) / 64, p->causal, 192, 512);
 }
 int64_t dkv_floats(const xva_diff_attention_args* p) {
     const Pieces s = dkv_plan(p);
     return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tk * p->Hk * 4 * p->d : 0;
 }
+int64_t query_floats(const xva_diff_attention_args* p, bool bwd) {
+    const Pieces s = query_plan(p);
+    return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tq * p->H * (bwd ? 2 * p->d : 4 * p->d + 4) : 0;
+}
+unsigned join_grid(const Args& a) { return (unsigned)(((int64_t)a.B * a.Tq * a.H * (a.d / 2) + 255) / 256); }
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
-    const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128));
+    const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128) * a.qpieces);
     if (train) fwd_kernel<D16, F16, true><<<grid, 256, 0, st>>>(a);
     else fwd_kernel<D16, F16, false><<<grid, 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
+    if (a.qpieces > 1) {
+        fwd_join_kernel<F16><<<join_grid(a), 256, 0, st>>>(a);
+        XVA_LAUNCH_CHECK();
+    }
     return XVA_OK;
 }
 template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_t st) {
@@ -1059,15 +1180,20 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
             XVA_LAUNCH_CHECK();
         }
     }
-    dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb), 256, 0, st>>>(a);
+    dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb * a.qpieces), 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
-    dlam_kernel<<<a.H, 256, 0, st>>>(a.dlam_part, dlam, a.B * nqb);
+    if (a.qpieces > 1) {
+        dq_join_kernel<F16><<<join_grid(a), 256, 0, st>>>(a);
+        XVA_LAUNCH_CHECK();
+    }
+    dlam_kernel<<<a.H, 256, 0, st>>>(a.dlam_part, dlam, a.B * nqb * a.qpieces);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
-    if (!bwd) return few_floats(p, few_plan(p)) * 4;
-    return (dkv_floats(p) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128)) * 4;
+    const Few f = few_plan(p);
+    if (!bwd) return (f.on ? few_floats(p, f) : query_floats(p, false)) * 4;
+    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p).pieces) * 4;
 }
 }   // namespace
 
@@ -1087,9 +1213,11 @@ extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws
     XVA_TRY(check(p, "xva_diff_attention_fwd"));
     if (p->B == 0 || p->Tq == 0) return XVA_OK;
     XVA_CHECK_ARG(p->out && (p->maps == nullptr) == (p->lse == nullptr), "xva_diff_attention_fwd: null argument");
-    const Args a = args_of(p);
+    Args a = args_of(p);
     const Few f = few_plan(p);
-    const int64_t need = few_floats(p, f) * 4;
+    const Pieces s = query_plan(p);
+    a.qpieces = s.pieces; a.qpiece = s.piece; a.qpart = (float*)ws;
+    const int64_t need = workspace(p, false);
     if (ws_bytes < need || (need && !ws)) {
         xva_set_error("xva_diff_attention_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
         return XVA_ERR_WS;
@@ -1109,9 +1237,11 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     }
     Args a = args_of(p);
     const Pieces s = dkv_plan(p);
-    a.pieces = s.pieces; a.piece = s.piece;
+    const Pieces sq = query_plan(p);
+    a.pieces = s.pieces; a.piece = s.piece; a.qpieces = sq.pieces; a.qpiece = sq.piece;
     a.part = (float*)ws;
-    a.D = a.part + dkv_floats(p);
+    a.qpart = a.part + dkv_floats(p);
+    a.D = a.qpart + query_floats(p, true);
     a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
 #define CALL(D16, F16) backward<D16, F16>(a, p->dlam, (hipStream_t)stream)
     XVA_DIFF_BY_SHAPE(CALL)
