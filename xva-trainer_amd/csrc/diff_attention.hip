@@ -148,6 +148,14 @@ __device__ __forceinline__ int key_tiles(const Args& a, int q0, int ql, int kl) 
 }
 
 // ================================================================================ forward ====
+// Running maxima are of c S (base 2).  Before a row's first key: so low that any score moves it, and finite, so that differences need no special case.
+constexpr float UNSEEN = -3e38f;
+// the largest of eight scores: the IEEE maximum, since fmaxf would first quiet each matrix product's result, an instruction apiece
+__device__ __forceinline__ float top8(f32x4 a, f32x4 b) {
+#define MAXIMUM __builtin_elementwise_maximum
+    return MAXIMUM(MAXIMUM(MAXIMUM(MAXIMUM(a[0], a[1]), a[2]), MAXIMUM(MAXIMUM(a[3], b[0]), b[1])), MAXIMUM(b[2], b[3]));
+#undef MAXIMUM
+}
 template <int D16, bool F16, bool TRAIN>
 __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     using S = Shape<D16>;
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-            mx[m][rt] = -INFINITY; sum[m][rt] = 0.f;
+            mx[m][rt] = UNSEEN; sum[m][rt] = 0.f;
 #pragma unroll
             for (int dt = 0; dt < S::VT; ++dt) o[m][rt][dt] = ZERO4;
         }
@@ -236,16 +244,13 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
                     }
                     float top[2];                             // of this lane's keys
 #pragma unroll
-                    for (int rt = 0; rt < 2; ++rt)
-                        top[rt] = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
-                                        fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
-                    // (a first key: the difference is +inf; nothing seen yet: it is NaN)
-                    if (__any((top[0] - mx[m][0]) * a.c > 8.f || (top[1] - mx[m][1]) * a.c > 8.f)) {
+                    for (int rt = 0; rt < 2; ++rt) top[rt] = top8(s[rt][0], s[rt][1]);
+                    if (__any(__builtin_fmaf(top[0], a.c, -mx[m][0]) > 8.f || __builtin_fmaf(top[1], a.c, -mx[m][1]) > 8.f)) {
 #pragma unroll
                         for (int rt = 0; rt < 2; ++rt) {
                             float now = fmaxf(top[rt], __shfl_xor(top[rt], 16, 64));
-                            now = fmaxf(fmaxf(now, __shfl_xor(now, 32, 64)), mx[m][rt]);
-                            const float alpha = mx[m][rt] == now ? 1.f : exp2_((mx[m][rt] - now) * a.c);
+                            now = fmaxf(fmaxf(now, __shfl_xor(now, 32, 64)) * a.c, mx[m][rt]);
+                            const float alpha = exp2_(mx[m][rt] - now);
                             mx[m][rt] = now;
                             sum[m][rt] *= alpha;
 #pragma unroll
@@ -254,12 +259,11 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
                     }
 #pragma unroll
                     for (int rt = 0; rt < 2; ++rt) {
-                        const float base = mx[m][rt] == -INFINITY ? 0.f : mx[m][rt] * a.c;
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const float p = exp2_(s[rt][u][r] * a.c - base);
+                                const float p = exp2_(__builtin_fmaf(s[rt][u][r], a.c, -mx[m][rt]));
                                 sum[m][rt] += p;
                                 s[rt][u][r] = p;
                             }
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
             l += __shfl_xor(l, 32, 64);
             total[m] = l;
             inv[m] = seen ? 1.f / l : 0.f;
-            if (TRAIN && all <= a.qpiece && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m][rt] + __log2f(l) / a.c) : -INFINITY;
+            if (TRAIN && all <= a.qpiece && g == 0 && row < a.Tq) a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m][rt] + __log2f(l)) / a.c : -INFINITY;
         }
         if (all > a.qpiece) {                                  // a piece: (max, sum) of both maps and the sums as they are, for fwd_join_kernel
             if (row >= a.Tq) continue;
@@ -343,7 +347,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
     const float* from = a.qpart + R * (2 * w + 4);
     const int64_t step = rows * (2 * w + 4);
     const int n = (all + a.qpiece - 1) / a.qpiece;
-    float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    float mx[2] = {UNSEEN, UNSEEN}, sum[2] = {0.f, 0.f};
     f32x4 o[2] = {ZERO4, ZERO4};
 #pragma unroll 4
     for (int p = 0; p < n; ++p)
@@ -354,8 +358,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
         const f32x4 st = *reinterpret_cast<const f32x4*>(from + p * step);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            // (a piece of which nothing is seen: its sums are zero, or no numbers where its scores are none)
-            const float by = st[2 * m] == -INFINITY ? 0.f : exp2_((st[2 * m] - mx[m]) * a.c);
+            const float by = exp2_(st[2 * m] - mx[m]);         // (a piece of which nothing is seen: its sums are zero, or no numbers where its scores are none)
             sum[m] += st[2 * m + 1] * by;
             o[m] += *reinterpret_cast<const f32x4*>(from + p * step + 4 + m * w + col) * by;
         }
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
         xva_attn::st4<F16>(a.maps + (rows + R) * w + col, v, 1.f);
         if (col < 8) {
             const int m = col >> 2;
-            a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m] + __log2f(sum[m]) / a.c) : -INFINITY;
+            a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + row] = seen ? -(mx[m] + __log2f(sum[m])) / a.c : -INFINITY;
         }
     }
 }
