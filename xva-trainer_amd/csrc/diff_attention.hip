@@ -135,9 +135,9 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // A workgroup's query block of a (item, head), and its piece of the keys.  The last blocks see most keys under `causal`: they start first.
 struct QueryBlock {
     int bh, blk, piece, blocks;
-    __device__ __forceinline__ QueryBlock(const Args& a) {
-        const unsigned heads = a.B * a.H, rest = blockIdx.x / heads;
-        bh = blockIdx.x - rest * heads;
+    __device__ __forceinline__ QueryBlock(const Args& a, unsigned id) {
+        const unsigned heads = a.B * a.H, rest = id / heads;
+        bh = id - rest * heads;
         blocks = (a.Tq + 127) / 128;
         piece = rest / (unsigned)blocks;
         blk = blocks - 1 - (rest - piece * blocks);
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
     __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];       // {K V} of the even and of the odd tiles (see XVA_TWO_BUFFERS)
-    const QueryBlock qb(a);
+    const QueryBlock qb(a, blockIdx.x);
     const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
@@ -686,17 +686,19 @@ struct KeyBlock {
 // leaves long causal sequences waiting for the first keys' ones.)
 // Where key blocks are few, or causal ones of very different length, the tiles of a key block are cut into pieces, one to a workgroup; a second kernel adds the pieces'
 // fp32 sums in order (rows of [2][d] of dK and [2 d] of dV).  Query blocks' keys are cut the same way in the forward pass and in dq.
-template <int D16, bool F16>
-__global__ __launch_bounds__(256, 2) void dkv_kernel(Args a) {
-    using S = Shape<D16>;
-    constexpr int NI = S::NI;
+template <int D16> struct BwdLds {
     // (the widest heads' accumulators leave too few registers for all of V's fragments: a spilled one would be waited for together with the tiles in flight)
-    constexpr int AWAY = D16 == 4 ? 3 : 0;                                                    // V fragments of the second key tile kept in LDS
-    constexpr int STAT = 2 * NI * TILE;                                                        // {Q dO | lse1 lse2 D1 D2} of the even and of the odd tiles
-    __shared__ __attribute__((aligned(1024))) uint8_t even[STAT + 1024], odd[STAT + 1024];
-    __shared__ __attribute__((aligned(16))) uint8_t away_raw[AWAY ? AWAY * 4096 : 16];
+    static constexpr int AWAY = D16 == 4 ? 3 : 0;                                             // V fragments of the second key tile kept in LDS
+    static constexpr int STAT = 2 * Shape<D16>::NI * TILE;                                     // {Q dO | lse1 lse2 D1 D2} of the even and of the odd tiles
+    typedef uint8_t Buffer[STAT + 1024];
+    typedef uint8_t Away[AWAY ? AWAY * 4096 : 16];
+};
+template <int D16, bool F16>
+__device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typename BwdLds<D16>::Buffer& even, typename BwdLds<D16>::Buffer& odd, typename BwdLds<D16>::Away& away_raw) {
+    using S = Shape<D16>;
+    constexpr int NI = S::NI, AWAY = BwdLds<D16>::AWAY, STAT = BwdLds<D16>::STAT;
     // (under `causal` the first keys are seen by most queries: they start first)
-    const unsigned heads = a.B * a.Hk, bh = blockIdx.x % heads, rest = blockIdx.x / heads;
+    const unsigned heads = a.B * a.Hk, bh = id % heads, rest = id / heads;
     const unsigned kblks = (a.Tk + 63) / 64;
     const int piece = rest / kblks, kblk = rest - piece * kblks;
     const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 64;
@@ -889,11 +891,10 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
 
 // dq of 128 queries of a head, 32 to a wave, and their part of dlam
 template <int D16, bool F16>
-__global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
+__device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typename BwdLds<D16>::Buffer& even, typename BwdLds<D16>::Buffer& odd) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
-    __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];
-    const QueryBlock qb(a);
+    const QueryBlock qb(a, id);
     const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
@@ -1047,6 +1048,16 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(Args a) {
     if (threadIdx.x == 0) a.dlam_part[(((int64_t)h * a.B + b) * qb.blocks + qb.blk) * a.qpieces + qb.piece] = red[0] + red[1] + red[2] + red[3];
 }
 
+// One launch for both: the first `dkv` workgroups take key blocks, the others query blocks, which fill the chip where the last key blocks leave it empty (32 x 860
+// frames, heads of 48: 128 + 84 us in two launches, 178 in one; 8192 causal positions, heads of 64: 1095 | 1073).
+template <int D16, bool F16>
+__global__ __launch_bounds__(256, 2) void grad_kernel(Args a, unsigned dkv) {
+    __shared__ __attribute__((aligned(1024))) typename BwdLds<D16>::Buffer even, odd;
+    __shared__ __attribute__((aligned(16))) typename BwdLds<D16>::Away away;
+    if (blockIdx.x < dkv) dkv_part<D16, F16>(a, blockIdx.x, even, odd, away);
+    else dq_part<D16, F16>(a, blockIdx.x - dkv, even, odd);
+}
+
 // the pieces of a row's dq, four columns to a thread
 template <bool F16>
 __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
@@ -1091,7 +1102,7 @@ int check(const xva_diff_attention_args* p, const char* who) {
     for (int64_t e : near) XVA_CHECK_ARG(e >= 0 && e < (1 << 24), "%s: row and map strides are 0 .. 2^24 - 1", who);
     XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
     const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
-    XVA_CHECK_ARG(wgs < (1ll << 31) && kwgs < (1ll << 31), "%s: too many blocks", who);
+    XVA_CHECK_ARG(wgs + kwgs < (1ll << 31), "%s: too many blocks", who);
     return XVA_OK;
 }
 Args args_of(const xva_diff_attention_args* p) {
@@ -1183,16 +1194,13 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
     const int64_t rows = (int64_t)a.B * a.Tq * a.H;
     rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
-    if (a.Tk > 0) {
-        dkv_kernel<D16, F16><<<(unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64) * a.pieces), 256, 0, st>>>(a);
-        XVA_LAUNCH_CHECK();
-        if (a.pieces > 1) {
-            dkv_join_kernel<F16><<<(unsigned)(((int64_t)a.B * a.Tk * a.Hk * a.d + 255) / 256), 256, 0, st>>>(a);
-            XVA_LAUNCH_CHECK();
-        }
-    }
-    dq_kernel<D16, F16><<<(unsigned)(a.B * a.H * nqb * a.qpieces), 256, 0, st>>>(a);
+    const unsigned dkv = (unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64) * a.pieces);
+    grad_kernel<D16, F16><<<dkv + (unsigned)(a.B * a.H * nqb * a.qpieces), 256, 0, st>>>(a, dkv);
     XVA_LAUNCH_CHECK();
+    if (a.pieces > 1) {
+        dkv_join_kernel<F16><<<(unsigned)(((int64_t)a.B * a.Tk * a.Hk * a.d + 255) / 256), 256, 0, st>>>(a);
+        XVA_LAUNCH_CHECK();
+    }
     if (a.qpieces > 1) {
         dq_join_kernel<F16><<<join_grid(a), 256, 0, st>>>(a);
         XVA_LAUNCH_CHECK();
