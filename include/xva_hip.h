@@ -716,7 +716,7 @@ int xva_sdp_dequant_bwd(const float* z_u, const float* dr, const float* d_z0_log
 /* ----------------------------------------------------------------- sequence operators ---- */
 /* Blocks of a sequence model on time-major tensors, beside the reference's own (no call site of the reference: attention with positions inside it, group
  * normalisation and recurrences are what a changed acoustic model asks for next).  dtype: 0 fp32, 1 bf16, 2 fp16; strides in elements, the last dimension
- * contiguous; rows at or behind an item's length are not read and leave as zeros.  Every call only enqueues; buffers of one call in flight (workspace
+ * contiguous; rows at or behind an item's length are not read and leave as zeros; workspaces are 16-byte aligned.  Every call only enqueues; buffers of one call in flight (workspace
  * included) are not shared with another on a different stream, nor with another captured graph that may run beside it. */
 
 /* Rotary positions.  q (B, T, H, D), k (B, T, Hk, D) (null with Hk = 0); pair i of the first rd elements of a head turns by position * turns[i]:
@@ -739,8 +739,9 @@ int xva_rotary(const xva_rotary_args* p, void* stream);
 /* Group normalisation + activation, channels last.  x (B, T, C) in G groups of channels; statistics over an item's live rows and a group's channels;
  * y = act(weight * xh + bias) (weight / bias fp32 (C), null: 1 / 0).  act: 0 none, 1 relu, 2 leaky relu (slope), 3 tanh, 4 silu, 5 gelu (erf).
  * mean / rstd (B, G) are written by the forward and read by the backward.  Backward: x, dy -> out = dx, and dweight / dbias (overwritten; null: not wanted).
- * At most 2048 groups, and 1024 vectors of 16 bytes in a row (1024 channels, where C, a stride or an address rules 16-byte accesses out), unless one
- * group of an item fits a wave (T * C / G of at most 256 vectors). */
+ * At most 2048 groups, and 1024 vectors in a row (of 16 bytes, of two elements or of one: the widest that C, strides and addresses allow), unless one group
+ * of an item fits the registers of a wave (T * C / G of at most 256 vectors of 16 bytes, 512 narrower ones) or, in vectors of 16 bytes or two elements, of a
+ * workgroup (some 6000 vectors). */
 typedef struct {
     const void *x, *dy;
     void* out;

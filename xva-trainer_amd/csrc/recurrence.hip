@@ -12,6 +12,9 @@
 //   * A workgroup walks over the tiles of its item and channels with the state in registers, the next tile's loads in flight under the present one: one read,
 //     one write.  Where items x channels leave too few workgroups for that (few long sequences), the tiles are also spread over workgroups: a first kernel leaves
 //     each chunk's (A, U), the second starts each chunk from the maps before it; gates and inputs are read twice.
+// 2 x 32768 x 1024 fp32 (8 chunks): maps 134 us (4.0 TB/s), forward 154 (5.2), gradient maps 126, backward 273 (4.9); one read of everything would take 430 us in all.
+// Cutting the launches along time so that the second read meets the Infinity Cache does not shorten it (two halves: 80 + 71 us each, four quarters 43 + 35).
+// 32 x 860 x 384 bf16 (no chunks): 21 + 36 us.
 // The backward pass needs h_{t-1} in fp32 at every step: the forward leaves the state at every STATE_STEPS-th step, the backward rebuilds a tile from there
 // (x and gate it reads anyway) and runs the gradient's recurrence, the same composition from the end.
 #include "xva_common.h"

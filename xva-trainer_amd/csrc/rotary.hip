@@ -5,7 +5,8 @@
 //
 // Bound: HBM — one read and one write of q and k.  The angles are not read from a table over positions (at 128 of head width that is a fp32 table row of
 // 512 bytes per token) but made on the spot, once per (token, pair), and shared by all heads through LDS: a workgroup owns a few tokens, first fills
-// (cos, sin) of its tokens, then streams the tokens' heads in memory order.
+// (cos, sin) of its tokens, then streams the tokens' heads in memory order.  bf16, 2 x 16384 tokens of 16 + 4 heads of 128: 336 MB in 65 - 70 us (5 TB/s, what a large
+// copy reaches); 64 tokens of 16 + 4 heads of 96 (interleaved): 3.7 us, a launch.
 //
 // Angles of far positions: p w in fp32 is off by p w 2^-24 radians (half a radian at a position of 8 million).  The plan holds w / 2 pi as a 64-bit
 // fixed-point fraction of a turn, so that p * w modulo one turn is the low half of an integer product: exact for every 64-bit position but for the table's
