@@ -165,6 +165,25 @@ def test_views_strides_and_flat_rows():
     assert torch.equal(S.group_norm_act(rows, 6), S.group_norm_act(rows[:, None], 6)[:, 0])
 
 
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_many_channels_at_any_address(dt):
+    """2048 channels need vectors: an input or a gradient that lies between two of them is taken all the same."""
+    from xva_trainer_amd import seq_ops as S
+    x, w, b, dy = _data(2, 300, 2048, dt, seed=8)
+    odd = lambda t: torch.cat([t[..., :1], t, t[..., :2]], -1)[..., 1:2049]
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = S.group_norm_act(x, 4, w, b, act="silu")
+    want = torch.autograd.grad(y, (x, w), dy)
+    x2 = odd(x.detach()).requires_grad_(True)
+    y2 = S.group_norm_act(x2, 4, w, b, act="silu")
+    assert torch.equal(y, y2)
+    for got in (torch.autograd.grad(y2, (x2, w), odd(dy), retain_graph=True), torch.autograd.grad(y2, (x2, w), dy)):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    flat = torch.zeros(x.numel() + 1, device="cuda", dtype=x.dtype)[1:].view(x.shape).copy_(x.detach())      # contiguous, at an odd address
+    with torch.no_grad():
+        assert torch.equal(S.group_norm_act(flat, 4, w, b, act="silu"), y)
+
+
 def test_repeats_bit_for_bit():
     x, w, b, dy = _data(3, 1500, 96, "bf16", seed=5)
     y1, g1 = _run(x, w, b, dy, None, 8, act="gelu")

@@ -130,6 +130,24 @@ def test_empty_and_graph_and_stream():
         assert torch.equal(qo, eager[0]) and torch.equal(ko, eager[1]), turn
 
 
+def test_in_place_refuses_shared_memory_and_tells_autograd():
+    from xva_trainer_amd import seq_ops as S
+    plan = S.RotaryPlan(32)
+    q = torch.randn(2, 3, 4, 32, device="cuda")
+    for bad in (lambda: S.rotary(plan, q, q, inplace=True), lambda: S.rotary(plan, q[:1].expand(2, 3, 4, 32), inplace=True),
+                lambda: S.rotary(plan, q, q[:, :, :1].expand(2, 3, 2, 32), inplace=True)):
+        with pytest.raises(S.XvaError):
+            bad()
+    with torch.no_grad():
+        one, two = S.rotary(plan, q, q)                                  # read only, the same tensor may come twice
+    assert torch.equal(one, two)
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    y = (q * w).sum()                                                    # saves q
+    S.rotary(plan, q, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_refusals():
     from xva_trainer_amd import seq_ops as S
     plan = S.RotaryPlan(32)

@@ -106,6 +106,7 @@ def test_rotary_refuses(bad, says):
 
 @pytest.mark.parametrize("bad,says", [(dict(x=None), "null"), (dict(mean=None), "null"), (dict(dtype=-1), "dtype"), (dict(G=5), "groups"), (dict(G=0), "groups"),
                                       (dict(act=9), "activation"), (dict(eps=-1.0), "eps"), (dict(T=500, C=16384, G=2), "vectors"), (dict(T=600, C=4096, G=4096), "2048 groups"),
+                                      (dict(T=3500, C=16384, G=4096, dtype=2), "2048 groups"),     # (the forward alone could: its backward could not)
                                       (dict(T=500, C=1025, G=1), "vectors")])
 def test_group_norm_refuses(bad, says):
     base = dict(x=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=3, C=32, G=4, act=0, eps=1e-5)

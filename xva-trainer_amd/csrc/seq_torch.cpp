@@ -8,6 +8,7 @@
 // The kernel library is not linked: seq_ops.py hands over the addresses of its entry points (`bind`), so that both sides use the one that _lib.py has loaded.
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <cmath>
@@ -63,6 +64,7 @@ Tensor lengths(const Tensor& lens, int64_t B, const char* what) {
 Tensor fp32(const Tensor& t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
 // with a contiguous last dimension
 Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor aligned(const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
 bool wants_grad(std::initializer_list<Tensor> ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor& t : ts)
@@ -155,7 +157,14 @@ variable_list rotary(const Tensor& turns, int64_t rd, bool interleaved, double g
         REFUSE(inplace, "inplace: no gradient");
         return Rotary::apply(q, maybe(k), turns, maybe(pos), rd, interleaved, gain);
     }
-    REFUSE(inplace && (q.stride(3) != 1 || (k.defined() && k.stride(3) != 1)), "inplace: a contiguous last dimension");
+    if (inplace) {
+        REFUSE(q.stride(3) != 1 || (k.defined() && k.stride(3) != 1), "inplace: a contiguous last dimension");
+        REFUSE(at::has_internal_overlap(q) == at::MemOverlap::Yes || (k.defined() && at::has_internal_overlap(k) == at::MemOverlap::Yes), "inplace: an expanded tensor");
+        REFUSE(k.defined() && k.numel() > 0 && (q.data_ptr() == k.data_ptr() || at::get_overlap_status(q, k) == at::MemOverlapStatus::Full || at::get_overlap_status(q, k) == at::MemOverlapStatus::Partial),
+               "inplace: q and k share memory");
+        for (const Tensor& t : {q, k})
+            if (t.defined()) t.unsafeGetTensorImpl()->bump_version();       // (a graph that saved it says so when it is run)
+    }
     const auto out = rotary_launch(q, k, {turns, pos, rd, interleaved, gain}, false, inplace);
     if (k.defined()) return {out.first, out.second};
     return {out.first};
@@ -168,8 +177,7 @@ Tensor wide(const Tensor& t) {
     bool ok = st.back() == 1 && (uintptr_t)t.data_ptr() % 16 == 0 && st[1] < (1 << 24) && (st.size() < 5 || st[3] < (1 << 24));
     for (size_t e = 0; e + 1 < st.size(); ++e) ok = ok && st[e] % 8 == 0;
     if (ok) return t;
-    const Tensor c = t.contiguous();
-    return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
+    return aligned(t.contiguous());
 }
 xva_diff_attention_args diff_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& ql, const Tensor& kl, bool causal, double scale) {
     xva_diff_attention_args a = {};
@@ -326,6 +334,14 @@ xva_group_norm_args norm_args(const Tensor& x, const Tensor& weight, const Tenso
     a.eps = (float)how.eps; a.slope = (float)how.slope;
     return a;
 }
+// as the kernels read it: one whose strides or address rule out vectors that its many channels, or groups, need is copied
+Tensor norm_rows(const Tensor& t_, int64_t groups) {
+    const Tensor t = rows(t_);
+    const int64_t C = t.size(2), all = t.stride(0) | t.stride(1), wide = t.scalar_type() == at::kFloat ? 4 : 8, bytes = t.element_size();
+    const auto at_address = [&](int64_t v) { return all % v == 0 && (uintptr_t)t.data_ptr() % (v * bytes) == 0; };
+    const int64_t v = C % wide == 0 && at_address(wide) ? wide : (C % 2 == 0 && at_address(2) ? 2 : 1);
+    return C / v <= 1024 && groups <= 2048 ? t : aligned(t.contiguous());
+}
 // (y, stats)
 variable_list norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& lens, const NormHow& how) {
     const c10::DeviceGuard guard(x.device());
@@ -354,7 +370,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const c10::DeviceGuard guard(x.device());
         auto& d = ctx->saved_data;
         xva_group_norm_args a = norm_args(x, weight, bias, s[3], s[4], {d["groups"].toInt(), (int)d["act"].toInt(), d["eps"].toDouble(), d["slope"].toDouble()});
-        const Tensor dy = rows(grads[0].to(x.scalar_type())), dx = at::empty(x.sizes(), x.options());
+        const Tensor dy = norm_rows(grads[0].to(x.scalar_type()), a.G), dx = at::empty(x.sizes(), x.options());
         // (needs_input_grad counts the inputs that were there)
         const Tensor dw = weight.defined() && ctx->needs_input_grad(1) ? at::empty(weight.sizes(), weight.options()) : Tensor();
         const Tensor db = bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1) ? at::empty(bias.sizes(), bias.options()) : Tensor();
@@ -383,7 +399,7 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const MaybeTensor& weigh
     REFUSE(!(eps >= 0.0 && std::isfinite(eps)), "eps ", eps);
     for (const Tensor& t : {weight, bias}) REFUSE(t.defined() && (t.dim() != 1 || t.size(0) != C || !t.is_floating_point()), "weight / bias ", t.sizes(), ": (", C, ",), a float type");
     const c10::DeviceGuard guard(x_.device());
-    const Tensor x = rows(flat ? x_.unsqueeze(1) : x_);
+    const Tensor x = norm_rows(flat ? x_.unsqueeze(1) : x_, groups);
     lens = lengths(lens, x.size(0), "lens");
     weight = fp32(weight); bias = fp32(bias);
     const NormHow how = {groups, which, eps, slope};
