@@ -7,7 +7,7 @@
 //   j <= i + kl - ql.  A row that sees nothing leaves as zeros and gives no gradient.
 //
 // Bound: MFMA and the exponentials beside it.  Flash-style: no score leaves the chip.
-//   forward : a workgroup takes 128 queries of a head, 32 to a wave; the two maps run their own online softmax over 64-key tiles and share every fragment of
+//   forward : a workgroup takes 128 queries of a head (64 of the narrower ones), 32 to a wave; the two maps run their own online softmax over 64-key tiles and share every fragment of
 //             V (one LDS read feeds both maps' products).  Base-2 exponentials, the scale folded in; the running maximum is only moved when a tile exceeds it
 //             by 2^8, so the accumulators are rescaled in the first tiles and hardly ever after.
 //   backward: dK / dV by key block and dq by query block, each rebuilding the maps from the saved logsumexp; no atomics, so results repeat bit for bit.
@@ -138,18 +138,18 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // A workgroup's query block of a (item, head), and its piece of the keys.  The last blocks see most keys under `causal`: they start first.
 struct QueryBlock {
     int bh, blk, piece, blocks;
-    __device__ __forceinline__ QueryBlock(const Args& a, unsigned id) {
+    __device__ __forceinline__ QueryBlock(const Args& a, unsigned id, int size = 128) {
         const unsigned heads = a.B * a.H, rest = id / heads;
         bh = id - rest * heads;
-        blocks = (a.Tq + 127) / 128;
+        blocks = (a.Tq + size - 1) / size;
         piece = rest / (unsigned)blocks;
         blk = blocks - 1 - (rest - piece * blocks);
     }
 };
 // 64-key tiles that some query of the block from q0 on sees
-__device__ __forceinline__ int key_tiles(const Args& a, int q0, int ql, int kl) {
+__device__ __forceinline__ int key_tiles(const Args& a, int q0, int ql, int kl, int size = 128) {
     if (q0 >= ql) return 0;
-    return ((a.causal ? max(min(kl, min(q0 + 127, ql - 1) + kl - ql + 1), 0) : kl) + 63) / 64;
+    return ((a.causal ? max(min(kl, min(q0 + size - 1, ql - 1) + kl - ql + 1), 0) : kl) + 63) / 64;
 }
 
 // ================================================================================ forward ====
@@ -161,27 +161,34 @@ __device__ __forceinline__ float top8(f32x4 a, f32x4 b) {
     return MAXIMUM(MAXIMUM(MAXIMUM(MAXIMUM(a[0], a[1]), a[2]), MAXIMUM(MAXIMUM(a[3], b[0]), b[1])), MAXIMUM(b[2], b[3]));
 #undef MAXIMUM
 }
+// HALF: 64 queries to a workgroup, two waves to 32 of them, each with the first or the second 32 keys of a tile; their softmaxes join through LDS.  For heads of 24 and
+// 32, where its 145 registers let a third wave onto each SIMD (forward kernel, us, 128 | 64 queries: 12 items of 860, 4 heads of 32 45 | 38, causal 35 | 27; 16 heads, 8192
+// 622 | 583; of 48: 32 items 108 | 116; of 16: 64 items of 1000 147 | 167, 8 heads, 2 x 8192 causal 277 | 258).
+__host__ __device__ constexpr int forward_rows(int d16) { return d16 == 2 ? 64 : 128; }       // queries of a workgroup
 template <int D16, bool F16, bool TRAIN>
 __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
     __shared__ __attribute__((aligned(1024))) uint8_t even[2 * NI * TILE], odd[2 * NI * TILE];       // {K V} of the even and of the odd tiles (see XVA_TWO_BUFFERS)
-    const QueryBlock qb(a, blockIdx.x);
-    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
+    constexpr int SIZE = forward_rows(D16);
+    constexpr bool HALF = SIZE == 64;
+    constexpr int STEPS = HALF ? 1 : 2;                                       // 32-key steps of a wave in a tile
+    const QueryBlock qb(a, blockIdx.x, SIZE);
+    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * SIZE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
     const uint16_t* kp = a.k + b * a.kb + hk * a.kh;
     const uint16_t* vp = a.v + b * a.vb + hk * a.vh;
     const uint16_t* qp = a.q + b * a.qb + h * a.qh;
-    const int wrow = q0 + wave * 32;
+    const int wrow = q0 + (HALF ? wave & 1 : wave) * 32, t0 = HALF ? wave >> 1 : 0;
     // keys that some query of the wave sees, and that every query of the wave sees
     auto seen_by = [&](int row) { return a.causal ? max(min(kl, row + off + 1), 0) : kl; };
     const int wave_keys = wrow < ql ? seen_by(min(wrow + 31, ql - 1)) : 0;
     const int whole_keys = seen_by(wrow);
-    const int all = key_tiles(a, q0, ql, kl), first = qb.piece * a.qpiece, tiles = min(all - first, a.qpiece);
+    const int all = key_tiles(a, q0, ql, kl, SIZE), first = qb.piece * a.qpiece, tiles = min(all - first, a.qpiece);
     if (qb.piece > 0 && tiles <= 0) return;
-    Lane fr(lane, 0);
+    Lane fr(lane, t0 * 4096);
     bf16x8 qf[2][2][S::KH];
     // keys that row tile rt's row of this lane sees
     auto limit = [&](int rt) { const int row = wrow + rt * 16 + (again(lane) & 15); return row < ql ? seen_by(row) : 0; };
@@ -219,10 +226,10 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
             src.fetch_qk(kp + row0 * a.kt, a.kt, a.km, a.d, kl - row0, next, wave);
             src.fetch_v(vp + row0 * a.vt, a.vt, a.d, kl - row0, next + NI * TILE, wave);
         }
-        if (jb * 64 < wave_keys) {
+        if (jb * 64 + t0 * 32 < wave_keys) {
             const bool whole = (jb + 1) * 64 <= whole_keys;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {                     // 32 keys at a time
+            for (int t = 0; t < STEPS; ++t) {                 // 32 keys at a time
                 bf16x8 pf[2][2];
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
@@ -240,7 +247,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
                     if (!whole) {
 #pragma unroll
                         for (int rt = 0; rt < 2; ++rt) {
-                            const int left = limit(rt) - (jb * 64 + t * 32 + g * 4);
+                            const int left = limit(rt) - (jb * 64 + (t0 + t) * 32 + g * 4);
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -290,6 +297,35 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
         __syncthreads();
     };
     XVA_TWO_BUFFERS(tiles, tile)
+    if constexpr (HALF) {                                     // (the tile loop has ended with a barrier)
+        XVA_LDS float* x = (XVA_LDS float*)((wave & 1) ? odd : even) + again(lane);       // [map][max, sum, 4 VT sums] of each lane, a row tile at a time
+        constexpr int EACH = 2 + 4 * S::VT;
+        static_assert(2 * EACH * 256 <= (int)sizeof even, "half of a wave's state in one buffer");
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            if (wave >> 1) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    x[m * EACH * 64] = mx[m][rt]; x[(m * EACH + 1) * 64] = sum[m][rt];
+#pragma unroll
+                    for (int e = 0; e < 4 * S::VT; ++e) x[(m * EACH + 2 + e) * 64] = o[m][rt][e >> 2][e & 3];
+                }
+            }
+            __syncthreads();
+            if (!(wave >> 1)) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const float other = x[m * EACH * 64], now = fmaxf(mx[m][rt], other), mine = exp2_(mx[m][rt] - now), its = exp2_(other - now);
+                    mx[m][rt] = now;
+                    sum[m][rt] = sum[m][rt] * mine + x[(m * EACH + 1) * 64] * its;
+#pragma unroll
+                    for (int e = 0; e < 4 * S::VT; ++e) o[m][rt][e >> 2][e & 3] = o[m][rt][e >> 2][e & 3] * mine + x[(m * EACH + 2 + e) * 64] * its;
+                }
+            }
+            __syncthreads();
+        }
+        if (wave >> 1) return;
+    }
     const float lam = uniform(a.lam, h);
     const int w = 2 * a.d;
 #pragma unroll
@@ -349,7 +385,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
     const int64_t R = id / quads;
     if (R >= rows) return;
     const int col = (int)(id - R * quads) * 4, h = (int)(R % a.H), b = (int)(R / ((int64_t)a.Tq * a.H)), row = (int)(R / a.H - (int64_t)b * a.Tq);
-    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), all = key_tiles(a, row & ~127, ql, kl);
+    const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), size = forward_rows((a.d + 15) / 16), all = key_tiles(a, row & -size, ql, kl, size);
     if (all <= a.qpiece) return;
     const float* from = a.qpart + R * (2 * w + 4);
     const int64_t step = rows * (2 * w + 4);
@@ -1104,7 +1140,7 @@ int check(const xva_diff_attention_args* p, const char* who) {
     const int64_t near[] = {p->q_stride[1], p->q_stride[3], p->k_stride[1], p->k_stride[3], p->v_stride[1], p->dout_stride[1]};
     for (int64_t e : near) XVA_CHECK_ARG(e >= 0 && e < (1 << 24), "%s: row and map strides are 0 .. 2^24 - 1", who);
     XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
-    const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 127) / 128), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
+    const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 63) / 64), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
     XVA_CHECK_ARG(wgs + kwgs < (1ll << 31), "%s: too many blocks", who);
     return XVA_OK;
 }
@@ -1169,20 +1205,21 @@ Pieces pieces_of(int64_t wgs, int64_t most, bool causal, int few, int uneven) {
 Pieces dkv_plan(const xva_diff_attention_args* p) {
     return pieces_of((int64_t)p->B * p->Hk * ((p->Tk + 63) / 64), (int64_t)(p->H / p->Hk) * ((p->Tq + 63) / 64), p->causal, 256, 768);
 }
-Pieces query_plan(const xva_diff_attention_args* p) {
-    return pieces_of((int64_t)p->B * p->H * ((p->Tq + 127) / 128), (p->Tk + 63) / 64, p->causal, 192, 512);
+Pieces query_plan(const xva_diff_attention_args* p, bool bwd) {
+    const int rows = bwd ? 128 : forward_rows((p->d + 15) / 16);
+    return pieces_of((int64_t)p->B * p->H * ((p->Tq + rows - 1) / rows), (p->Tk + 63) / 64, p->causal, 192, 512);
 }
 int64_t dkv_floats(const xva_diff_attention_args* p) {
     const Pieces s = dkv_plan(p);
     return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tk * p->Hk * 4 * p->d : 0;
 }
 int64_t query_floats(const xva_diff_attention_args* p, bool bwd) {
-    const Pieces s = query_plan(p);
+    const Pieces s = query_plan(p, bwd);
     return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tq * p->H * (bwd ? 2 * p->d : 4 * p->d + 4) : 0;
 }
 unsigned join_grid(const Args& a) { return (unsigned)(((int64_t)a.B * a.Tq * a.H * (a.d / 2) + 255) / 256); }
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
-    const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + 127) / 128) * a.qpieces);
+    const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + forward_rows(D16) - 1) / forward_rows(D16)) * a.qpieces);
     if (train) fwd_kernel<D16, F16, true><<<grid, 256, 0, st>>>(a);
     else fwd_kernel<D16, F16, false><<<grid, 256, 0, st>>>(a);
     XVA_LAUNCH_CHECK();
@@ -1215,7 +1252,7 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
     const Few f = few_plan(p);
     if (!bwd) return (f.on ? few_floats(p, f) : query_floats(p, false)) * 4;
-    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p).pieces) * 4;
+    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces) * 4;
 }
 }   // namespace
 
@@ -1237,7 +1274,7 @@ extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws
     XVA_CHECK_ARG(p->out && (p->maps == nullptr) == (p->lse == nullptr), "xva_diff_attention_fwd: null argument");
     Args a = args_of(p);
     const Few f = few_plan(p);
-    const Pieces s = query_plan(p);
+    const Pieces s = query_plan(p, false);
     a.qpieces = s.pieces; a.qpiece = s.piece; a.qpart = (float*)ws;
     const int64_t need = workspace(p, false);
     if (ws_bytes < need || (need && !ws)) {
@@ -1259,7 +1296,7 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     }
     Args a = args_of(p);
     const Pieces s = dkv_plan(p);
-    const Pieces sq = query_plan(p);
+    const Pieces sq = query_plan(p, true);
     a.pieces = s.pieces; a.piece = s.piece; a.qpieces = sq.pieces; a.qpiece = sq.piece;
     a.part = (float*)ws;
     a.qpart = a.part + dkv_floats(p);
