@@ -67,7 +67,9 @@ def _data(B, T, C, dt, seed=0):
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("ragged", [None, "some", "empty"])
 @pytest.mark.parametrize("B,T,C", [(1, 1, 1), (64, 1, 128), (3, 7, 5), (2, 8, 64), (2, 9, 130), (4, 127, 33), (3, 128, 2), (2, 129, 256), (3, 860, 48), (1, 3000, 7),
-                                   (2, 2500, 128), (5, 1, 2048)])
+                                   (2, 2500, 128), (5, 1, 2048),
+                                   # rows of 32 bytes: one tile, several, an odd width
+                                   (16, 200, 128), (32, 1300, 65), (9, 1100, 448)])
 def test_shapes(dt, reverse, ragged, B, T, C):
     lens = lengths(B, T, ragged)
     got = _run(*_data(B, T, C, dt), lens=lens.cuda() if lens is not None else None, reverse=reverse, gain="unit" if C % 2 else "convex")

@@ -449,6 +449,11 @@ Plan make_plan(int dtype, int B, int T, int C, int v, bool bwd) {
     int lc = 64;
     while (lc > 1 && lc / 2 >= lanes) lc /= 2;
     while (lc > 16 && (int64_t)B * ((lanes + lc - 1) / lc) < 256) lc /= 2;
+    // Still few: rows of 32 bytes, where that fills the CUs and time need not be cut, so that inputs are read once.  Kernels' time, us, cut | narrow: 32 x 3000 x 64 fp32
+    // forward 36 | 20, backward 43 | 31; 2 x 3000 x 1024 37 | 22, 44 | 32; 1 x 8192 x 4096 bf16 74 | 57, 118 | 113; longer than that the cut wins or draws (4 x 16384 x 512
+    // fp32 131 | 141, 190 | 207).
+    const int narrow = 32 / (v * (dtype == 0 ? 4 : 2));
+    if (T <= 8192 && (int64_t)B * ((lanes + lc - 1) / lc) < 160 && narrow < lc && (int64_t)B * ((lanes + narrow - 1) / narrow) >= 256) lc = narrow;
     p.lc = lc;
     p.lc_log = __builtin_ctz(lc);
     p.cblocks = (lanes + lc - 1) / lc;
