@@ -128,6 +128,15 @@ def test_a_query_that_is_no_number_stays_one(Tq, Tk, causal):
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens", [[600, 0, 17, 600, 300], [1] * 4 + [530] * 3, [520] * 66, list(range(64))])
+def test_items_of_any_lengths_in_any_order(causal, lens):
+    """Long ragged batches start their longest items first: ties, empty items, more items than are ranked."""
+    T, kl = max(max(lens), 513), torch.tensor(lens, dtype=torch.int32)
+    _run(*_data(len(lens), T, T, 1, 1, 8, "bf16", seed=8), ql=kl, kl=kl, causal=causal)
+    _run(*_data(len(lens), 70, T, 2, 1, 16, "bf16", seed=9), kl=kl, causal=causal)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_numbers_of_a_head_of_any_sign(dt):
     q, k, v, lam, dout = _data(2, 200, 200, 6, 3, 32, dt, seed=6)

@@ -135,15 +135,35 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float uniform(const float* p, int i) { return reinterpret_cast<const __attribute__((address_space(4))) float*>((uintptr_t)p)[i]; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A workgroup's query block of a (item, head), and its piece of the keys.  The last blocks see most keys under `causal`: they start first.
-struct QueryBlock {
-    int bh, blk, piece, blocks;
-    __device__ __forceinline__ QueryBlock(const Args& a, unsigned id, int size = 128) {
-        const unsigned heads = a.B * a.H, rest = id / heads;
-        bh = id - rest * heads;
-        blocks = (a.Tq + size - 1) / size;
-        piece = rest / (unsigned)blocks;
-        blk = blocks - 1 - (rest - piece * blocks);
+// Workgroups that walk over more than this start by their length: ranking the items takes a microsecond or two (32 x 150, heads of 32: 16 -> 22 us of dK / dV / dq)
+constexpr int LONG = 512;
+// The r-th longest item of a ragged batch, by `lens` (the same in every lane): workgroups start in this order, so that the last ones to start are short (32 x 860 ragged
+// frames, 4 heads of 48: forward 90 -> 81 us, dK / dV / dq 183 -> 156).  Each lane ranks one item; larger batches, whose workgroups are many, keep their order.
+__device__ __forceinline__ int item_by_length(const int32_t* lens, int B, int T, int r) {
+    if (!lens || B > 64 || T <= LONG) return r;
+    const int lane = threadIdx.x & 63, mine = lane < B ? len_of(lens, lane, T) : -1;
+    int rank = 0;
+    for (int j = 0; j < B; ++j) {
+        const int other = __builtin_amdgcn_readlane(mine, j);
+        rank += other > mine || (other == mine && j < lane);
+    }
+    return __builtin_ctzll(__ballot(lane < B && rank == r));
+}
+// A workgroup's block of a (item, head) and its piece.  All pairs over LT long rows: the items by length, with all their blocks; otherwise block by block, under `causal` by
+// their length (`last_first`: the last ones see most keys), the items by length within.
+struct Block {
+    int b, h, blk, piece, blocks;
+    __device__ __forceinline__ Block(const Args& a, unsigned id, int heads, int T, int size, const int32_t* lens, int LT, bool last_first) {
+        const bool by_block = a.causal || LT <= LONG;
+        blocks = (T + size - 1) / size;
+        const unsigned all = (unsigned)blocks * a.B * heads;
+        piece = id / all;
+        const unsigned at = id - piece * all, inner = by_block ? (unsigned)a.B * heads : (unsigned)blocks * heads;
+        const int outer = at / inner, in = at - outer * inner, mid = in / heads;
+        h = in - mid * heads;
+        blk = by_block ? outer : mid;
+        b = item_by_length(lens, a.B, LT, by_block ? mid : outer);
+        if (last_first) blk = blocks - 1 - blk;
     }
 };
 // 64-key tiles that some query of the block from q0 on sees
@@ -173,8 +193,8 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
     constexpr int SIZE = forward_rows(D16);
     constexpr bool HALF = SIZE == 64;
     constexpr int STEPS = HALF ? 1 : 2;                                       // 32-key steps of a wave in a tile
-    const QueryBlock qb(a, blockIdx.x, SIZE);
-    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * SIZE;
+    const Block qb(a, blockIdx.x, a.H, a.Tq, SIZE, a.kl, a.Tk, true);
+    const int h = qb.h, b = qb.b, q0 = qb.blk * SIZE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
@@ -736,11 +756,8 @@ template <int D16, bool F16>
 __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typename BwdLds<D16>::Buffer& even, typename BwdLds<D16>::Buffer& odd, typename BwdLds<D16>::Away& away_raw) {
     using S = Shape<D16>;
     constexpr int NI = S::NI, AWAY = BwdLds<D16>::AWAY, STAT = BwdLds<D16>::STAT;
-    // (under `causal` the first keys are seen by most queries: they start first)
-    const unsigned heads = a.B * a.Hk, bh = id % heads, rest = id / heads;
-    const unsigned kblks = (a.Tk + 63) / 64;
-    const int piece = rest / kblks, kblk = rest - piece * kblks;
-    const int hk = bh % a.Hk, b = bh / a.Hk, k0 = kblk * 64;
+    const Block at(a, id, a.Hk, a.Tk, 64, a.ql, a.Tq, false);             // (under `causal` the first keys are seen by most queries: they start first)
+    const int kblk = at.blk, piece = at.piece, hk = at.h, b = at.b, k0 = kblk * 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15, t = wave >> 1;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql;
@@ -933,8 +950,8 @@ template <int D16, bool F16>
 __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typename BwdLds<D16>::Buffer& even, typename BwdLds<D16>::Buffer& odd) {
     using S = Shape<D16>;
     constexpr int NI = S::NI;
-    const QueryBlock qb(a, id);
-    const int h = qb.bh % a.H, b = qb.bh / a.H, q0 = qb.blk * 128;
+    const Block qb(a, id, a.H, a.Tq, 128, a.kl, a.Tk, true);
+    const int h = qb.h, b = qb.b, q0 = qb.blk * 128;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i = lane & 15;
     const int ql = len_of(a.ql, b, a.Tq), kl = len_of(a.kl, b, a.Tk), off = kl - ql, hk = h / a.share;
