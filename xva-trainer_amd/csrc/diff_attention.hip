@@ -16,8 +16,9 @@
 // Waves raise their priority over the products that follow a softmax (s_setprio): the other wave of a SIMD then does its exponentials meanwhile (8192 causal positions,
 // heads of 64: dq 463 -> 429 us, dK/dV 692 -> 673, forward 484 -> 476; over the score products as well: 481, 699, 474).
 // Reached (kernels' time, dense operations of the formulas): 8192 causal positions, 16 heads of 64 on 4 keys' 472 us forward (870 TFLOP/s), 1073 us dK / dV / dq (640);
-// matrix units 47 - 49 % busy, vector units 59 - 66 %, two waves to a SIMD.  32 x 860 ragged frames, 4 heads of 48: 91 + 178 us: 704 query blocks on 512 places, and
-// scores of 48 columns take matrix steps of 64.  32 x 150: 14 + 16 us.
+// matrix units 47 - 49 % busy, vector units 59 - 66 %, two waves to a SIMD.  32 x 860 ragged frames, 4 heads of 48: 81 + 155 us: 688 query blocks on 512 places, and
+// scores of 48 columns take matrix steps of 64.  32 x 150, heads of 32: 13 + 16 us.  One query on each of 16 ragged caches of up to 8192 keys, 16 heads of 64 on 4 keys':
+// 41 us (4.7 TB/s) and 7 for the join.
 // Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands (the accumulators are fp32; sums, maxima and logsumexp stay fp32).
 //
 // Tiles: 64 rows x 64 columns of 16-bit values (attn_tile.h).  d <= 32: one image holds both maps' 32 columns side by side; d <= 64: one image for each map.
