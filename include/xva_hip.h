@@ -716,7 +716,8 @@ int xva_sdp_dequant_bwd(const float* z_u, const float* dr, const float* d_z0_log
 /* ----------------------------------------------------------------- sequence operators ---- */
 /* Blocks of a sequence model on time-major tensors, beside the reference's own (no call site of the reference: attention with positions inside it, group
  * normalisation and recurrences are what a changed acoustic model asks for next).  dtype: 0 fp32, 1 bf16, 2 fp16; strides in elements, the last dimension
- * contiguous; rows at or behind an item's length are not read and leave as zeros; workspaces are 16-byte aligned.  Every call only enqueues; buffers of one call in flight (workspace
+ * contiguous; rows at or behind an item's length are not read and leave as zeros; workspaces are 16-byte aligned, their size asked
+ * for with the arguments of the call.  Every call only enqueues; buffers of one call in flight (workspace
  * included) are not shared with another on a different stream, nor with another captured graph that may run beside it. */
 
 /* Rotary positions.  q (B, T, H, D), k (B, T, Hk, D) (null with Hk = 0); pair i of the first rd elements of a head turns by position * turns[i]:

@@ -6,7 +6,7 @@
 //   Key heads may be fewer than query heads (their gradients add up); a query of an item with ql queries and kl keys sees keys j < kl, and with `causal`
 //   j <= i + kl - ql.  A row that sees nothing leaves as zeros and gives no gradient.
 //
-// Bound: MFMA and the exponentials beside it.  Flash-style: no score leaves the chip.
+// Bound: MFMA and the exponentials beside it.  No score leaves the chip.
 //   forward : a workgroup takes 128 queries of a head (64 of the narrower ones), 32 to a wave; the two maps run their own online softmax over 64-key tiles and share every fragment of
 //             V (one LDS read feeds both maps' products).  Base-2 exponentials, the scale folded in; the running maximum is only moved when a tile exceeds it
 //             by 2^8, so the accumulators are rescaled in the first tiles and hardly ever after.
