@@ -779,25 +779,23 @@ int64_t xva_recurrence_state_floats(int B, int T, int C);
 int xva_recurrence_fwd(const xva_recurrence_args* p, void* workspace, int64_t workspace_bytes, void* stream);
 int xva_recurrence_bwd(const xva_recurrence_args* p, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Differential attention (bf16 / fp16).  q (B, Tq, H, 2, d), k (B, Tk, Hk, 2, d), v (B, Tk, Hk, 2 d), lam (H) fp32; d a multiple of 8 up to 64, H a multiple
+/* Differential attention (bf16 / fp16).  q (B, Tq, H, 2, d), k (B, Tk, Hk, 2, d), v (B, Tk, Hk, 2 d), lam (H) of lam_dtype; d a multiple of 8 up to 64, H a multiple
  * of Hk (query head h reads key head h / (H / Hk)); addresses 16-byte aligned, strides multiples of 8, those of rows and maps
  * under 2^24.  out (B, Tq, H, 2 d) =
  * (softmax(scale q_1 k_1^T) - lam softmax(scale q_2 k_2^T)) v.  q_lens / k_lens (B): live queries and keys (null: all); causal: query i sees keys
  * j <= i + k_len - q_len.  Rows that see nothing, and rows behind q_len, leave as zeros.
  * For a backward pass the forward also writes maps (2, B, Tq, H, 2 d), each softmax's own output, and lse (2, B, H, Tq) fp32 (both null: no backward).
- * Backward: dout -> dq, dk, dv (contiguous, the inputs' shapes) and dlam (H) fp32, all overwritten (B = 0 or Tq = 0: nothing is). */
+ * Backward: dout -> dq, dk, dv (contiguous, the inputs' shapes) and dlam (H) of lam_dtype, all overwritten (B = 0 or Tq = 0: nothing is). */
 typedef struct {
-    const void *q, *k, *v;
-    const float* lam;
+    const void *q, *k, *v, *lam;
     void *out, *maps;
     float* lse;
     const void* dout;
-    void *dq, *dk, *dv;
-    float* dlam;
+    void *dq, *dk, *dv, *dlam;
     const int32_t *q_lens, *k_lens;
     int64_t q_stride[4], k_stride[4];                                      /* items, rows, heads, maps */
     int64_t v_stride[3], out_stride[3], dout_stride[3];                    /* items, rows, heads */
-    int32_t dtype, B, Tq, Tk, H, Hk, d, causal;
+    int32_t dtype, B, Tq, Tk, H, Hk, d, causal, lam_dtype;
     float scale;
 } xva_diff_attention_args;
 int64_t xva_diff_attention_workspace_bytes(const xva_diff_attention_args* p, int backward_pass);

@@ -67,7 +67,7 @@ class RecurrenceArgs(C.Structure):
 
 class DiffAttentionArgs(C.Structure):
     _fields_ = _fields(("q k v lam out maps lse dout dq dk dv dlam q_lens k_lens", vp), ("q_stride[4] k_stride[4] v_stride[3] out_stride[3] dout_stride[3]", i64),
-                       ("dtype B Tq Tk H Hk d causal", i32), ("scale", f32))
+                       ("dtype B Tq Tk H Hk d causal lam_dtype", i32), ("scale", f32))
 
 
 def entry(name, restype=i32):

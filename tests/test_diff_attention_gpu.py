@@ -137,6 +137,24 @@ def test_items_of_any_lengths_in_any_order(causal, lens):
     _run(*_data(len(lens), 70, T, 2, 1, 16, "bf16", seed=9), kl=kl, causal=causal)
 
 
+@pytest.mark.parametrize("Tq,Tk,causal", [(200, 200, True), (1, 90, False), (4, 900, True), (700, 130, False), (90, 2000, False)])
+@pytest.mark.parametrize("lam_type", [torch.bfloat16, torch.float16, torch.float64])
+def test_numbers_of_any_type(Tq, Tk, causal, lam_type):
+    """lam and its gradient in their own type: the results are those of the same numbers in fp32, the gradient is that one rounded once."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(2, Tq, Tk, 4, 2, 32, "bf16", seed=10)
+    lam = lam.to(lam_type)
+    out = {}
+    for number in (lam, lam.float()):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, number)]
+        y = S.differential_attention(*leaves, causal=causal)
+        with torch.no_grad():
+            out[number.dtype] = (y, S.differential_attention(*leaves, causal=causal)) + torch.autograd.grad(y, leaves, dout)
+    mine, want = out[lam_type], out[torch.float32]
+    assert mine[-1].dtype == lam_type and torch.equal(mine[-1], want[-1].to(lam_type))
+    assert all(torch.equal(p, r) for p, r in zip(mine[:-1], want[:-1]))
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_numbers_of_a_head_of_any_sign(dt):
     q, k, v, lam, dout = _data(2, 200, 200, 6, 3, 32, dt, seed=6)

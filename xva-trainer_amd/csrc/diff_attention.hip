@@ -35,7 +35,9 @@ using xva_attn::pack_rows;
 struct Args {
     const uint16_t *q, *k, *v, *dout;
     uint16_t *out, *maps, *dq, *dk, *dv;
-    const float* lam;
+    const void* lam;                              // (H) of type lam_type: 0 fp32, 1 bf16, 2 fp16
+    int lam_type;
+    float* lam32;                                 // backward: the same in fp32, for the scalar unit (rowdot_kernel leaves it)
     float *lse, *D, *dlam_part;
     const int32_t *ql, *kl;
     int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
@@ -134,6 +136,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define ZERO4 ((f32x4){0.f, 0.f, 0.f, 0.f})
 // p[i] of an input that is the same in every lane, by a scalar load (a vector load would be waited for together with the tiles in flight)
 __device__ __forceinline__ float uniform(const float* p, int i) { return reinterpret_cast<const __attribute__((address_space(4))) float*>((uintptr_t)p)[i]; }
+__device__ __forceinline__ float lam_of(const Args& a, int h) {
+    return a.lam_type == 0 ? static_cast<const float*>(a.lam)[h] : (a.lam_type == 1 ? ld16<false>(a.lam, h) : ld16<true>(a.lam, h));
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Workgroups that walk over more than this start by their length: ranking the items takes a microsecond or two (32 x 150, heads of 32: 16 -> 22 us of dK / dV / dq)
@@ -347,7 +352,7 @@ __global__ __launch_bounds__(256, 2) void fwd_kernel(Args a) {
         }
         if (wave >> 1) return;
     }
-    const float lam = uniform(a.lam, h);
+    const float lam = lam_of(a, h);
     const int w = 2 * a.d;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(256) void fwd_join_kernel(Args a) {
         }
     }
     const bool seen = row < ql && (!a.causal || row + kl - ql >= 0);
-    const float lam = a.lam[h];
+    const float lam = lam_of(a, h);
     const f32x4 u = seen ? o[0] * (1.f / sum[0]) : ZERO4, v = seen ? o[1] * (1.f / sum[1]) : ZERO4;
     xva_attn::st4<F16>(a.out + b * a.ob + row * a.ot + h * a.oh + col, seen ? u - v * lam : ZERO4, 1.f);
     if (a.maps) {
@@ -631,7 +636,7 @@ __global__ __launch_bounds__(256, RT == 2 && D16 >= 3 ? 1 : 2) void few_kernel(A
                         for (int e = 0; e < W / 16; ++e) first[e] = acc[e] * inv;
                     } else {
                         const int hs = r / a.Tq, h = hk * a.share + hs;
-                        const float by = a.lam[h];
+                        const float by = lam_of(a, h);
                         uint16_t* out = a.out + b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh;
 #pragma unroll
                         for (int e = 0; e < W / 16; e += 2)
@@ -695,7 +700,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a, const float* __re
             t[m] *= inv[m];
         }
         const int hs = r / a.Tq, h = hk * a.share + hs;
-        xva_attn::st4<F16>(a.out + b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh + col, t[0] - a.lam[h] * t[1], 1.f);
+        xva_attn::st4<F16>(a.out + b * a.ob + (int64_t)(r - hs * a.Tq) * a.ot + h * a.oh + col, t[0] - lam_of(a, h) * t[1], 1.f);
     }
 }
 
@@ -728,6 +733,7 @@ __global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
         s[m] += __shfl_xor(s[m], 1, 64); s[m] += __shfl_xor(s[m], 2, 64); s[m] += __shfl_xor(s[m], 4, 64); s[m] += __shfl_xor(s[m], 8, 64);
     }
     if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
+    if (id < a.H && (threadIdx.x & 15) == 0) a.lam32[id] = lam_of(a, (int)id);
 }
 
 // A key block's 64-query tiles: of each query head that shares the keys, `per_head` from tile `t0` on
@@ -808,7 +814,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
     __syncthreads();
     auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         const int row0 = qtile * 64;
-        const float lam = uniform(a.lam, hk * a.share + hs), loglam = __log2f(fabsf(lam)), minus = lam < 0.f ? 1.f : -1.f;
+        const float lam = uniform(a.lam32, hk * a.share + hs), loglam = __log2f(fabsf(lam)), minus = lam < 0.f ? 1.f : -1.f;
         if (++hs == a.share) { hs = 0; --qtile; }
         if (it + 1 < total) fetch(hs, qtile * 64, next);
         const int wrow = row0 + t * 32;                       // this wave's 32 rows
@@ -1075,7 +1081,7 @@ __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typena
         __syncthreads();
     };
     XVA_TWO_BUFFERS(tiles, tile)
-    const float lam = uniform(a.lam, h);
+    const float lam = uniform(a.lam32, h);
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const int row = wrow + rt * 16 + i;
@@ -1127,16 +1133,18 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
     if (all <= a.qpiece) return;
     f32x4 v = ZERO4;
     for (int p = 0; p * a.qpiece < all; ++p) v += *reinterpret_cast<const f32x4*>(a.qpart + (p * rows + R) * w + col);
-    xva_attn::st4<F16>(a.dq + R * w + col, v, col < a.d ? a.scale : -a.lam[h] * a.scale);
+    xva_attn::st4<F16>(a.dq + R * w + col, v, col < a.d ? a.scale : -a.lam32[h] * a.scale);
 }
 
-// dlam[h] = - sum of the head's parts, in a fixed order
-__global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ part, float* __restrict__ dlam, int n) {
+// dlam[h] = - sum of the head's parts, in a fixed order, rounded once to lam's type
+__global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ part, void* __restrict__ dlam, int type, int n) {
     __shared__ float sh[16];
     float v = 0.f;
     for (int k = threadIdx.x; k < n; k += 256) v += part[(int64_t)blockIdx.x * n + k];
     v = xva_block_sum(v, sh);
-    if (threadIdx.x == 0) dlam[blockIdx.x] = -v;
+    if (threadIdx.x != 0) return;
+    if (type == 0) static_cast<float*>(dlam)[blockIdx.x] = -v;
+    else static_cast<uint16_t*>(dlam)[blockIdx.x] = type == 1 ? cvt16<false>(-v) : cvt16<true>(-v);
 }
 #undef MFMA
 
@@ -1148,6 +1156,7 @@ int check(const xva_diff_attention_args* p, const char* who) {
                   "%s: B %d Tq %d Tk %d H %d Hk %d", who, p->B, p->Tq, p->Tk, p->H, p->Hk);
     XVA_CHECK_ARG(p->d >= 8 && p->d <= 64 && p->d % 8 == 0, "%s: head width %d (a multiple of 8 up to 64)", who, p->d);
     XVA_CHECK_ARG(p->scale > 0.f, "%s: scale %g", who, p->scale);
+    XVA_CHECK_ARG(p->lam_dtype >= 0 && p->lam_dtype <= 2, "%s: lam of dtype %d", who, p->lam_dtype);
     if (p->B == 0 || p->Tq == 0) return XVA_OK;
     XVA_CHECK_ARG(p->q && p->lam && (p->Tk == 0 || (p->k && p->v)), "%s: null argument", who);
     uintptr_t ptrs = (uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->out | (uintptr_t)p->dout;
@@ -1166,7 +1175,7 @@ Args args_of(const xva_diff_attention_args* p) {
     Args a = {};
     a.q = (const uint16_t*)p->q; a.k = (const uint16_t*)p->k; a.v = (const uint16_t*)p->v; a.dout = (const uint16_t*)p->dout;
     a.out = (uint16_t*)p->out; a.maps = (uint16_t*)p->maps; a.dq = (uint16_t*)p->dq; a.dk = (uint16_t*)p->dk; a.dv = (uint16_t*)p->dv;
-    a.lam = p->lam; a.lse = p->lse; a.ql = p->q_lens; a.kl = p->k_lens;
+    a.lam = p->lam; a.lam_type = p->lam_dtype; a.lse = p->lse; a.ql = p->q_lens; a.kl = p->k_lens;
     a.qb = p->q_stride[0]; a.qt = p->q_stride[1]; a.qh = p->q_stride[2]; a.qm = p->q_stride[3];
     a.kb = p->k_stride[0]; a.kt = p->k_stride[1]; a.kh = p->k_stride[2]; a.km = p->k_stride[3];
     a.vb = p->v_stride[0]; a.vt = p->v_stride[1]; a.vh = p->v_stride[2];
@@ -1247,7 +1256,7 @@ template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t 
     }
     return XVA_OK;
 }
-template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_t st) {
+template <int D16, bool F16> int backward(const Args& a, void* dlam, hipStream_t st) {
     const int nqb = (a.Tq + 127) / 128;
     const int64_t rows = (int64_t)a.B * a.Tq * a.H;
     rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
@@ -1263,14 +1272,14 @@ template <int D16, bool F16> int backward(const Args& a, float* dlam, hipStream_
         dq_join_kernel<F16><<<join_grid(a), 256, 0, st>>>(a);
         XVA_LAUNCH_CHECK();
     }
-    dlam_kernel<<<a.H, 256, 0, st>>>(a.dlam_part, dlam, a.B * nqb * a.qpieces);
+    dlam_kernel<<<a.H, 256, 0, st>>>(a.dlam_part, dlam, a.lam_type, a.B * nqb * a.qpieces);
     XVA_LAUNCH_CHECK();
     return XVA_OK;
 }
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
     const Few f = few_plan(p);
     if (!bwd) return (f.on ? few_floats(p, f) : query_floats(p, false)) * 4;
-    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces) * 4;
+    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces + p->H) * 4;
 }
 }   // namespace
 
@@ -1320,6 +1329,7 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     a.qpart = a.part + dkv_floats(p);
     a.D = a.qpart + query_floats(p, true);
     a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
+    a.lam32 = a.dlam_part + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * a.qpieces;
 #define CALL(D16, F16) backward<D16, F16>(a, p->dlam, (hipStream_t)stream)
     XVA_DIFF_BY_SHAPE(CALL)
 #undef CALL

@@ -181,7 +181,7 @@ Tensor wide(const Tensor& t) {
 }
 xva_diff_attention_args diff_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& ql, const Tensor& kl, bool causal, double scale) {
     xva_diff_attention_args a = {};
-    a.q = ptr(q); a.k = ptr(k); a.v = ptr(v); a.lam = (const float*)ptr(lam); a.q_lens = (const int32_t*)ptr(ql); a.k_lens = (const int32_t*)ptr(kl);
+    a.q = ptr(q); a.k = ptr(k); a.v = ptr(v); a.lam = ptr(lam); a.lam_dtype = dtype_of(lam); a.q_lens = (const int32_t*)ptr(ql); a.k_lens = (const int32_t*)ptr(kl);
     for (int e = 0; e < 4; ++e) { a.q_stride[e] = q.stride(e); a.k_stride[e] = k.stride(e); }
     for (int e = 0; e < 3; ++e) a.v_stride[e] = v.stride(e);
     a.dtype = dtype_of(q); a.B = small(q.size(0), "B"); a.Tq = small(q.size(1), "Tq"); a.Tk = small(k.size(1), "Tk"); a.H = small(q.size(2), "H"); a.Hk = small(k.size(2), "Hk");
@@ -222,7 +222,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
             dk.zero_(); dv.zero_(); dlam.zero_();
         } else {
             xva_diff_attention_args a = diff_args(q, k, v, lam, s[6], s[7], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
-            a.maps = ptr(s[4]); a.lse = (float*)ptr(s[5]); a.dout = ptr(dout); a.dq = ptr(dq); a.dk = ptr(dk); a.dv = ptr(dv); a.dlam = (float*)ptr(dlam);
+            a.maps = ptr(s[4]); a.lse = (float*)ptr(s[5]); a.dout = ptr(dout); a.dq = ptr(dq); a.dk = ptr(dk); a.dv = ptr(dv); a.dlam = ptr(dlam);
             for (int e = 0; e < 3; ++e) a.dout_stride[e] = dout.stride(e);
             const int64_t n = lib.diff_ws(&a, 1);
             const Tensor ws = workspace(n, q);
@@ -250,7 +250,7 @@ Tensor differential_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
     REFUSE(!(scale > 0.0 && std::isfinite(scale)), "scale ", scale);
     const c10::DeviceGuard guard(q_.device());
     ql = lengths(ql, B, "q_lens"); kl = lengths(kl, B, "k_lens");
-    const Tensor q = wide(q_), k = wide(k_), v = wide(v_), lam = fp32(lam_);
+    const Tensor q = wide(q_), k = wide(k_), v = wide(v_), lam = dtype_of(lam_) < 0 ? fp32(lam_) : lam_.contiguous();
     if (wants_grad({q, k, v, lam})) return DiffAttention::apply(q, k, v, lam, maybe(ql), maybe(kl), causal, scale);
     return diff_forward(q, k, v, lam, ql, kl, causal, scale, false)[0];
 }
