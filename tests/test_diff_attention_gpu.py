@@ -253,7 +253,7 @@ def test_the_gradient_by_differences():
 
 def test_repeats_graph_and_streams():
     from xva_trainer_amd import seq_ops as S
-    for Tq, Tk in ((200, 200), (1, 900)):
+    for Tq, Tk in ((200, 200), (1, 900), (700, 1500)):
         q, k, v, lam, dout = _data(2, Tq, Tk, 4, 2, 64, "bf16", seed=7)
         leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
         kl = torch.tensor([Tk, Tk // 2], device="cuda", dtype=torch.int32)
@@ -279,6 +279,26 @@ def test_repeats_graph_and_streams():
             eager = step()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(outs, eager)), turn
+
+
+def test_two_calls_at_once():
+    """Passes on two streams that cut their blocks into pieces: each has its own workspace."""
+    from xva_trainer_amd import seq_ops as S
+    sets = [[t.requires_grad_(True) for t in _data(1, 600, 1400, 2, 1, 48, "bf16", seed=s)] for s in (11, 12)]
+    def step(t):
+        out = S.differential_attention(*t[:4], causal=True)
+        return (out.detach(),) + torch.autograd.grad(out, t[:4], t[4].detach())
+    want = [step(t) for t in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for turn in range(3):
+        got = []
+        for t, s in zip(sets, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(step(t))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w)), turn
 
 
 def test_empty():

@@ -216,7 +216,7 @@ def test_empty_graph_and_stream():
         assert y.shape == shape
         assert (torch.autograd.grad(y.sum(), w)[0] == 0).all()
     del y                                        # (an eager graph of a leaf must not live while a backward pass of that leaf is captured: torch ties the two streams)
-    for B, T in ((6, 1), (2, 700)):
+    for B, T in ((6, 1), (2, 700), (1100, 20), (1, 6000)):
         x, dy = torch.randn(B, T, 32, device="cuda", requires_grad=True), torch.randn(B, T, 32, device="cuda")
         def step():
             y = S.group_norm_act(x, 4, w, act="silu")
