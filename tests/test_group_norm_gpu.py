@@ -250,3 +250,12 @@ def test_refusals():
                 lambda: S.group_norm_act(torch.zeros(1, 300, 16384, device="cuda"), 2), lambda: S.group_norm_act(torch.zeros(1, 600, 4096, device="cuda"), 4096)):
         with pytest.raises(S.XvaError):
             bad()
+
+
+@pytest.mark.parametrize("shape,G", [((0, 5000, 32), 1), ((0, 300, 64), 4), ((0, 500, 33), 1), ((0, 600, 4096), 4096), ((3, 0, 32), 4)])
+def test_no_items_or_rows_in_any_form(shape, G):
+    from xva_trainer_amd import seq_ops as S
+    x, w, b = torch.zeros(shape, device="cuda", requires_grad=True), torch.ones(shape[2], device="cuda", requires_grad=True), torch.ones(shape[2], device="cuda", requires_grad=True)
+    y = S.group_norm_act(x, G, w, b, act="silu")
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert y.shape == dx.shape == shape and (dw == 0).all() and (db == 0).all()

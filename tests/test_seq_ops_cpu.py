@@ -134,3 +134,14 @@ def test_recurrence_refuses_a_small_workspace():
     assert need > 0
     assert entry("xva_recurrence_fwd")(C.byref(RecurrenceArgs(x=A, gate=A, h=A, last=A, dtype=0, B=1, T=30000, C=64)), A, need - 1, None) == -3
     assert entry("xva_recurrence_bwd")(C.byref(RecurrenceArgs(x=A, gate=A, dtype=0, B=1, T=30000, C=64)), A, need, None) < 0
+
+
+@pytest.mark.parametrize("T,channels,G", [(1, 64, 4), (300, 64, 4), (5000, 32, 1), (500, 33, 1), (500, 1025, 1)])
+@pytest.mark.parametrize("B,T0", [(0, None), (3, 0)])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_group_norm_without_items_or_rows(T, channels, G, B, T0, dtype):
+    """At the shapes of all three forms: no workspace and nothing launched (dweight and dbias, which would be zeroed, are not asked for)."""
+    a = GroupNormArgs(dtype=dtype, B=B, T=T if T0 is None else T0, C=channels, G=G, act=0, eps=1e-5)
+    for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
+        assert entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd) == 0
+        assert call(C.byref(a), None, 0, None) == 0

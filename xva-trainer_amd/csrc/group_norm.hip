@@ -834,6 +834,7 @@ Args args_of(const xva_group_norm_args* p, const Plan& q) {
 }
 
 int64_t workspace(const xva_group_norm_args* p, bool bwd) {
+    if (p->B == 0 || p->T == 0) return 0;
     // (over the vector widths: which one runs depends on addresses and strides)
     int64_t most = 0;
     for (int vec = 8; vec > 0; vec = vec == 8 ? 2 : vec - 1) {
@@ -932,11 +933,7 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     XVA_TRY(check(p, who));
     XVA_CHECK_ARG(!bwd || p->dy || p->B == 0 || p->T == 0, "%s: null gradient", who);
     hipStream_t st = (hipStream_t)stream;
-    Plan q = {};
-    // (the forward refuses what the backward would have to)
-    XVA_CHECK_ARG((bwd || make_plan(p, allowed(p, false), true, &q)) && make_plan(p, allowed(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
-    XVA_CHECK_ARG(q.form == SLAB || (int64_t)p->B * (q.form == TILE ? q.chunks : q.w.blocks) < (1ll << 31) - 8, "%s: %d items of %d rows", who, p->B, p->T);
-    if (ws_bytes < workspace(p, bwd)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)workspace(p, bwd)); return XVA_ERR_WS; }
+    // (before any plan: it divides the workgroups among the items)
     if (p->B == 0 || p->T == 0) {
         if (bwd) {
             if (p->dweight) { void* d[1] = {p->dweight}; const int64_t n[1] = {(int64_t)p->C * 4}; XVA_TRY(xva_zero_spans(d, n, 1, stream)); }
@@ -944,6 +941,11 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
         }
         return XVA_OK;
     }
+    Plan q = {};
+    // (the forward refuses what the backward would have to)
+    XVA_CHECK_ARG((bwd || make_plan(p, allowed(p, false), true, &q)) && make_plan(p, allowed(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
+    XVA_CHECK_ARG(q.form == SLAB || (int64_t)p->B * (q.form == TILE ? q.chunks : q.w.blocks) < (1ll << 31) - 8, "%s: %d items of %d rows", who, p->B, p->T);
+    if (ws_bytes < workspace(p, bwd)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)workspace(p, bwd)); return XVA_ERR_WS; }
     Args a = args_of(p, q);
     a.part = (float*)ws;
 #define GN(DT, V) (bwd ? backward<DT, V>(a, q, st) : forward<DT, V>(a, q, st))
