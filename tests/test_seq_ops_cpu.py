@@ -145,3 +145,12 @@ def test_group_norm_without_items_or_rows(T, channels, G, B, T0, dtype):
     for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
         assert entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd) == 0
         assert call(C.byref(a), None, 0, None) == 0
+
+
+@pytest.mark.parametrize("T", [1, 200, 3000])
+def test_group_norm_refuses_a_null_workspace(T):
+    a = GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=2, T=T, C=32, G=4, act=0, eps=1e-5)
+    for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
+        need = entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd)
+        if need > 0:
+            assert call(C.byref(a), None, need, None) == -3
