@@ -738,7 +738,7 @@ typedef struct {
 int xva_rotary(const xva_rotary_args* p, void* stream);
 
 /* Group normalisation + activation, channels last.  x (B, T, C) in G groups of channels; statistics over an item's live rows and a group's channels;
- * y = act(weight * xh + bias) (weight / bias fp32 (C), null: 1 / 0).  act: 0 none, 1 relu, 2 leaky relu (slope), 3 tanh, 4 silu, 5 gelu (erf).
+ * y = act(weight * xh + bias) (weight / bias fp32 (C) at any address, null: 1 / 0).  act: 0 none, 1 relu, 2 leaky relu (slope), 3 tanh, 4 silu, 5 gelu (erf).
  * mean / rstd (B, G) are written by the forward and read by the backward.  Backward: x, dy -> out = dx, and dweight / dbias (overwritten; null: not wanted).
  * At most 2048 groups, and 1024 vectors in a row (of 16 bytes, of two elements or of one: the widest that C, strides and addresses allow), unless one group
  * of an item fits the registers of a wave (T * C / G of at most 256 vectors of 16 bytes, 512 narrower ones) or, in vectors of 16 bytes or two elements, of a

@@ -259,3 +259,20 @@ def test_no_items_or_rows_in_any_form(shape, G):
     y = S.group_norm_act(x, G, w, b, act="silu")
     dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
     assert y.shape == dx.shape == shape and (dw == 0).all() and (db == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("B,T,C,G", [(2, 300, 2048, 4), (300, 1, 512, 8), (2, 860, 384, 16), (2, 2500, 32, 4), (2, 60, 430, 5)])
+def test_weights_at_any_address(dt, B, T, C, G):
+    """Slices of a flat parameter buffer: the same results and gradients, whatever their address."""
+    from xva_trainer_amd import seq_ops as S
+    x, w, b, dy = _data(B, T, C, dt, seed=9)
+    flat = torch.zeros(2 * C + 3, device="cuda")
+    outs = []
+    for at in (None, 1, 2, 3):
+        ws = [t.clone() if at is None else flat[at + i * C:at + (i + 1) * C].copy_(t) for i, t in enumerate((w, b))]
+        leaves = [t.detach().requires_grad_(True) for t in [x] + ws]
+        y = S.group_norm_act(leaves[0], G, leaves[1], leaves[2], act="silu")
+        outs.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
+    for other in outs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(outs[0], other))

@@ -154,3 +154,13 @@ def test_group_norm_refuses_a_null_workspace(T):
         need = entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd)
         if need > 0:
             assert call(C.byref(a), None, need, None) == -3
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_group_norm_takes_weights_at_any_address(dtype):
+    """2048 channels need vectors of x; the weights' address does not take them away (the call gets as far as its workspace)."""
+    for at in (dict(weight=A + 4), dict(bias=A + 4), dict(weight=A + 8, bias=A + 12)):
+        a = GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=dtype, B=2, T=300, C=2048, G=4, act=0, eps=1e-5, x_stride0=300 * 2048, x_stride1=2048, out_stride0=300 * 2048,
+                          out_stride1=2048, dy_stride0=300 * 2048, dy_stride1=2048, **at)
+        assert entry("xva_group_norm_act_fwd")(C.byref(a), None, 0, None) == -3
+        assert entry("xva_group_norm_act_bwd")(C.byref(a), None, 0, None) == -3
