@@ -276,3 +276,31 @@ def test_weights_at_any_address(dt, B, T, C, G):
         outs.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
     for other in outs[1:]:
         assert all(torch.equal(p, q) for p, q in zip(outs[0], other))
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-1, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("B,T,C,G", [(40, 1, 64, 4), (3, 200, 64, 4), (2, 2500, 32, 4)])
+def test_tanh_of_small_weights(size, B, T, C, G):
+    """z carries the weights' size, and so do the errors allowed (`_reference`): a tanh that is off by a share of 1 would not do."""
+    from xva_trainer_amd import seq_ops as S
+    x, w, b, dy = _data(B, T, C, "fp32", seed=10)
+    w, b = (t * size for t in (w, b))
+    x.requires_grad_(True)
+    y = S.group_norm_act(x, G, w, b, act="tanh")
+    dx, = torch.autograd.grad(y, x, dy)
+    ref, err = _reference(x, w, b, dy, None, G, 1e-5, "tanh", 0.0)
+    close(y, ref[0], rounded(ref[0], x.dtype, err[0]), "y")
+    close(dx, ref[1], rounded(ref[1], x.dtype, err[1]), "dx")
+
+
+def test_tanh_far_out():
+    """Slopes of saturated values, where 1 - tanh^2 would have nothing left: 4 e / (1 + e)^2 with e = exp(-2 |z|).  The exponential's argument, up to 40, is off by
+    1.5 x 2^-24 of itself (the product with log2 e and that constant), e and the reciprocals by some units: under 40 x 1.5 x 2^-24 + 8 x 2^-24 < 2^-17 of the slope."""
+    from xva_trainer_amd import seq_ops as S
+    x = torch.tensor([1.0, -1.0], device="cuda").repeat(32)[None].requires_grad_(True)
+    b = torch.linspace(-20, 20, 64, device="cuda").requires_grad_(True)
+    y = S.group_norm_act(x, 1, torch.zeros(64, device="cuda"), b, eps=0.0, act="tanh")
+    db, = torch.autograd.grad(y, b, torch.ones_like(y))
+    z = b.detach().double().cpu()
+    close(y.detach()[0], z.tanh(), 2.0 ** -22 * z.tanh().abs(), "y")
+    close(db, z.cosh() ** -2, 2.0 ** -17 * z.cosh() ** -2, "slope")

@@ -44,8 +44,11 @@ struct Args {
 };
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
-// (off by a few 2^-24 of 1, as z itself is)
-__device__ __forceinline__ float tanh_(float z) { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * z)); }
+// tanh'(z) = 4 e / (1 + e)^2, e = exp(-2 |z|): no difference of near numbers, at any z
+__device__ __forceinline__ float tanh_slope(float z) {
+    const float e = __expf(-2.f * fabsf(z)), r = __builtin_amdgcn_rcpf(1.f + e);
+    return 4.f * e * r * r;
+}
 // (one switch to V values: a branch of every value costs more than the activations)
 template <int V, class F> __device__ __forceinline__ void each(float (&z)[V], F f) {
 #pragma unroll
@@ -55,7 +58,7 @@ template <int V> __device__ __forceinline__ void activate(float (&z)[V], int act
     switch (act) {
         case RELU: each<V>(z, [](float v) { return v > 0.f ? v : (v != v ? v : 0.f); }); break;
         case LRELU: each<V>(z, [=](float v) { return v > 0.f ? v : slope * v; }); break;
-        case TANH: each<V>(z, [](float v) { return tanh_(v); }); break;
+        case TANH: each<V>(z, [](float v) { return tanhf(v); }); break;        // (the library's: within a unit or two of z itself near zero, where small weights put it)
         case SILU: each<V>(z, [](float v) { return v * sigmoid(v); }); break;
         case GELU: each<V>(z, [](float v) { return 0.5f * v * (1.f + erff(v * 0.70710678118654752f)); }); break;
         default: break;
@@ -66,7 +69,7 @@ template <int V> __device__ __forceinline__ void slopes(float (&z)[V], int act, 
     switch (act) {
         case RELU: each<V>(z, [](float v) { return v > 0.f ? 1.f : 0.f; }); break;
         case LRELU: each<V>(z, [=](float v) { return v > 0.f ? 1.f : slope; }); break;
-        case TANH: each<V>(z, [](float v) { const float t = tanh_(v); return 1.f - t * t; }); break;
+        case TANH: each<V>(z, [](float v) { return tanh_slope(v); }); break;
         case SILU: each<V>(z, [](float v) { const float s = sigmoid(v); return s + s * v * (1.f - s); }); break;
         case GELU: each<V>(z, [](float v) { return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * 0.39894228040143268f * __expf(-0.5f * v * v); }); break;
         default: each<V>(z, [](float) { return 1.f; });
