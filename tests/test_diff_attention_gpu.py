@@ -325,3 +325,15 @@ def test_refusals():
                                                                                                           torch.zeros(1, 2, 1, 144, device="cuda").half(), lam[:1])):
         with pytest.raises(S.XvaError):
             bad()
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+@pytest.mark.parametrize("width", [2048, 2053, 2049])
+def test_one_row_of_a_projection_of_any_width(Tq, width):
+    """Dimensions of 1 may have any stride; torch calls such a slice contiguous and copies nothing."""
+    H, d, T = 16, 64, 70
+    whole = torch.randn(2, T, width, device="cuda").bfloat16()
+    q = whole[..., :H * 2 * d].unflatten(-1, (H, 2, d))[:1, :Tq]
+    k, v = whole[1:, ..., :2 * d].unflatten(-1, (1, 2, d))[:, :T if Tq > 1 else 1], whole[:1, :T if Tq > 1 else 1, 64:64 + 2 * d].unflatten(-1, (1, 2 * d))
+    dout = torch.randn(1, T, width, device="cuda").bfloat16()[:, :Tq, :H * 2 * d].unflatten(-1, (H, 2 * d))
+    _run(q, k, v, torch.rand(H, device="cuda"), dout, causal=True)

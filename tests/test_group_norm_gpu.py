@@ -304,3 +304,18 @@ def test_tanh_far_out():
     z = b.detach().double().cpu()
     close(y.detach()[0], z.tanh(), 2.0 ** -22 * z.tanh().abs(), "y")
     close(db, z.cosh() ** -2, 2.0 ** -17 * z.cosh() ** -2, "slope")
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("B,T", [(1, 300), (1, 1), (5, 1)])
+def test_one_row_or_item_at_any_stride(dt, B, T):
+    """The stride of a dimension of 1 says nothing: the same results as of a copy, also where 2048 channels in one group of long rows need vectors."""
+    from xva_trainer_amd import seq_ops as S
+    whole = torch.randn(B * 301 * 2051 + 8, device="cuda").to(DTYPES[dt])
+    for sb, st in ((301 * 2051, 2048), (2048, 2051), (2051 * 8, 3)):
+        x = whole.as_strided((B, T, 2048), (sb if B == 1 else 2048 * T, st if T == 1 else 2048)).requires_grad_(True)
+        want = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
+        dy = torch.randn(B, T, 2048, device="cuda").to(DTYPES[dt])
+        for G in (2, 32):
+            y, z = S.group_norm_act(x, G, act="gelu"), S.group_norm_act(want, G, act="gelu")
+            assert torch.equal(y, z) and torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(z, want, dy)[0])

@@ -62,6 +62,8 @@ Tensor lengths(const Tensor& lens, int64_t B, const char* what) {
     return lens.to(at::kInt).contiguous();
 }
 Tensor fp32(const Tensor& t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
+// elements from one index of dimension e to the next (a dimension of 1 has none: torch leaves any number there)
+int64_t step(const Tensor& t, int e) { return t.size(e) > 1 ? t.stride(e) : 0; }
 // with a contiguous last dimension
 Tensor rows(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 Tensor aligned(const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
@@ -99,8 +101,8 @@ std::pair<Tensor, Tensor> rotary_launch(const Tensor& q_, const Tensor& k_, cons
     xva_rotary_args a = {};
     a.q = q.data_ptr(); a.k = ptr(k); a.q_out = qo.data_ptr(); a.k_out = ptr(ko);
     for (int e = 0; e < 3; ++e) {
-        a.q_stride[e] = q.stride(e); a.q_out_stride[e] = qo.stride(e);
-        if (k.defined()) { a.k_stride[e] = k.stride(e); a.k_out_stride[e] = ko.stride(e); }
+        a.q_stride[e] = step(q, e); a.q_out_stride[e] = step(qo, e);
+        if (k.defined()) { a.k_stride[e] = step(k, e); a.k_out_stride[e] = step(ko, e); }
     }
     a.turns = (const uint64_t*)r.turns.data_ptr();
     if (r.pos.defined()) {
@@ -173,17 +175,16 @@ variable_list rotary(const Tensor& turns, int64_t rd, bool interleaved, double g
 // ------------------------------------------------------------------------------------------------------------------ differential attention ----
 // as the kernels read it: 16-byte rows, 64 of them and their maps within 32-bit offsets
 Tensor wide(const Tensor& t) {
-    const auto st = t.strides();
-    bool ok = st.back() == 1 && (uintptr_t)t.data_ptr() % 16 == 0 && st[1] < (1 << 24) && (st.size() < 5 || st[3] < (1 << 24));
-    for (size_t e = 0; e + 1 < st.size(); ++e) ok = ok && st[e] % 8 == 0;
+    bool ok = t.stride(-1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0 && step(t, 1) < (1 << 24) && (t.dim() < 5 || step(t, 3) < (1 << 24));
+    for (int e = 0; e + 1 < t.dim(); ++e) ok = ok && step(t, e) % 8 == 0;
     if (ok) return t;
     return aligned(t.contiguous());
 }
 xva_diff_attention_args diff_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& ql, const Tensor& kl, bool causal, double scale) {
     xva_diff_attention_args a = {};
     a.q = ptr(q); a.k = ptr(k); a.v = ptr(v); a.lam = ptr(lam); a.lam_dtype = dtype_of(lam); a.q_lens = (const int32_t*)ptr(ql); a.k_lens = (const int32_t*)ptr(kl);
-    for (int e = 0; e < 4; ++e) { a.q_stride[e] = q.stride(e); a.k_stride[e] = k.stride(e); }
-    for (int e = 0; e < 3; ++e) a.v_stride[e] = v.stride(e);
+    for (int e = 0; e < 4; ++e) { a.q_stride[e] = step(q, e); a.k_stride[e] = step(k, e); }
+    for (int e = 0; e < 3; ++e) a.v_stride[e] = step(v, e);
     a.dtype = dtype_of(q); a.B = small(q.size(0), "B"); a.Tq = small(q.size(1), "Tq"); a.Tk = small(k.size(1), "Tk"); a.H = small(q.size(2), "H"); a.Hk = small(k.size(2), "Hk");
     a.d = small(q.size(4), "d"); a.causal = causal; a.scale = (float)scale;
     return a;
@@ -196,7 +197,7 @@ variable_list diff_forward(const Tensor& q, const Tensor& k, const Tensor& v, co
     const Tensor maps = train ? at::empty({2, B, Tq, H, 2 * d}, q.options()) : Tensor(), lse = train ? floats({2, B, H, Tq}, q) : Tensor();
     xva_diff_attention_args a = diff_args(q, k, v, lam, ql, kl, causal, scale);
     a.out = ptr(out); a.maps = ptr(maps); a.lse = (float*)ptr(lse);
-    for (int e = 0; e < 3; ++e) a.out_stride[e] = out.stride(e);
+    for (int e = 0; e < 3; ++e) a.out_stride[e] = step(out, e);
     const int64_t n = lib.diff_ws(&a, 0);
     const Tensor ws = workspace(n, q);
     call(lib.diff_fwd(&a, ptr(ws), n, stream_of(q)), "xva_diff_attention_fwd");
@@ -223,7 +224,7 @@ struct DiffAttention : torch::autograd::Function<DiffAttention> {
         } else {
             xva_diff_attention_args a = diff_args(q, k, v, lam, s[6], s[7], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
             a.maps = ptr(s[4]); a.lse = (float*)ptr(s[5]); a.dout = ptr(dout); a.dq = ptr(dq); a.dk = ptr(dk); a.dv = ptr(dv); a.dlam = ptr(dlam);
-            for (int e = 0; e < 3; ++e) a.dout_stride[e] = dout.stride(e);
+            for (int e = 0; e < 3; ++e) a.dout_stride[e] = step(dout, e);
             const int64_t n = lib.diff_ws(&a, 1);
             const Tensor ws = workspace(n, q);
             call(lib.diff_bwd(&a, ptr(ws), n, stream_of(q)), "xva_diff_attention_bwd");
@@ -259,7 +260,7 @@ Tensor differential_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
 xva_recurrence_args rec_args(const Tensor& x, const Tensor& gate, const Tensor& lens, bool reverse, bool unit) {
     xva_recurrence_args a = {};
     a.x = ptr(x); a.gate = ptr(gate); a.lens = (const int32_t*)ptr(lens);
-    for (int e = 0; e < 2; ++e) { a.x_stride[e] = x.stride(e); a.gate_stride[e] = gate.stride(e); }
+    for (int e = 0; e < 2; ++e) { a.x_stride[e] = step(x, e); a.gate_stride[e] = step(gate, e); }
     a.dtype = dtype_of(x); a.B = small(x.size(0), "B"); a.T = small(x.size(1), "T"); a.C = small(x.size(2), "C"); a.reverse = reverse; a.unit_gain = unit;
     return a;
 }
@@ -270,7 +271,7 @@ variable_list rec_forward(const Tensor& x, const Tensor& gate, const Tensor& h0,
     const Tensor h = at::empty(x.sizes(), x.options()), last = floats({x.size(0), x.size(2)}, x);
     const Tensor states = train ? floats({lib.rec_states(a.B, a.T, a.C)}, x) : Tensor();
     a.h = ptr(h); a.h0 = (const float*)ptr(h0); a.last = (float*)ptr(last); a.states = (float*)ptr(states);
-    for (int e = 0; e < 2; ++e) a.h_stride[e] = h.stride(e);
+    for (int e = 0; e < 2; ++e) a.h_stride[e] = step(h, e);
     const int64_t n = lib.rec_ws(a.B, a.T, a.C);
     const Tensor ws = workspace(n, x);
     call(lib.rec_fwd(&a, ptr(ws), n, stream_of(x)), "xva_recurrence_fwd");
@@ -296,7 +297,7 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
         const Tensor dx = at::empty(x.sizes(), x.options()), dgate = at::empty(x.sizes(), x.options());
         const Tensor dh0 = ctx->saved_data["h0"].toBool() ? floats({x.size(0), x.size(2)}, x) : Tensor();
         a.states = (float*)ptr(s[2]); a.dh = ptr(dh); a.dlast = (const float*)ptr(dlast); a.dx = ptr(dx); a.dgate = ptr(dgate); a.dh0 = (float*)ptr(dh0);
-        for (int e = 0; e < 2; ++e) { a.dh_stride[e] = dh.stride(e); a.dx_stride[e] = dx.stride(e); a.dgate_stride[e] = dgate.stride(e); }
+        for (int e = 0; e < 2; ++e) { a.dh_stride[e] = step(dh, e); a.dx_stride[e] = step(dx, e); a.dgate_stride[e] = step(dgate, e); }
         const int64_t n = lib.rec_ws(a.B, a.T, a.C);
         const Tensor ws = workspace(n, x);
         call(lib.rec_bwd(&a, ptr(ws), n, stream_of(x)), "xva_recurrence_bwd");
@@ -329,7 +330,7 @@ xva_group_norm_args norm_args(const Tensor& x, const Tensor& weight, const Tenso
     xva_group_norm_args a = {};
     a.x = ptr(x); a.weight = (const float*)ptr(weight); a.bias = (const float*)ptr(bias); a.lens = (const int32_t*)ptr(lens);
     a.mean = (float*)ptr(stats); a.rstd = a.mean + x.size(0) * how.groups;
-    for (int e = 0; e < 2; ++e) a.x_stride[e] = x.stride(e);
+    for (int e = 0; e < 2; ++e) a.x_stride[e] = step(x, e);
     a.dtype = dtype_of(x); a.B = small(x.size(0), "B"); a.T = small(x.size(1), "T"); a.C = small(x.size(2), "C"); a.G = (int)how.groups; a.act = how.act;
     a.eps = (float)how.eps; a.slope = (float)how.slope;
     return a;
@@ -337,7 +338,7 @@ xva_group_norm_args norm_args(const Tensor& x, const Tensor& weight, const Tenso
 // as the kernels read it: one whose strides or address rule out vectors that its many channels, or groups, need is copied
 Tensor norm_rows(const Tensor& t_, int64_t groups) {
     const Tensor t = rows(t_);
-    const int64_t C = t.size(2), all = t.stride(0) | t.stride(1), wide = t.scalar_type() == at::kFloat ? 4 : 8, bytes = t.element_size();
+    const int64_t C = t.size(2), all = step(t, 0) | step(t, 1), wide = t.scalar_type() == at::kFloat ? 4 : 8, bytes = t.element_size();
     const auto at_address = [&](int64_t v) { return all % v == 0 && (uintptr_t)t.data_ptr() % (v * bytes) == 0; };
     const int64_t v = C % wide == 0 && at_address(wide) ? wide : (C % 2 == 0 && at_address(2) ? 2 : 1);
     return C / v <= 1024 && groups <= 2048 ? t : aligned(t.contiguous());
@@ -348,7 +349,7 @@ variable_list norm_forward(const Tensor& x, const Tensor& weight, const Tensor& 
     const Tensor y = at::empty(x.sizes(), x.options()), stats = floats({2, x.size(0), how.groups}, x);
     xva_group_norm_args a = norm_args(x, weight, bias, lens, stats, how);
     a.out = ptr(y);
-    for (int e = 0; e < 2; ++e) a.out_stride[e] = y.stride(e);
+    for (int e = 0; e < 2; ++e) a.out_stride[e] = step(y, e);
     const int64_t n = lib.norm_ws(&a, 0);
     const Tensor ws = workspace(n, x);
     call(lib.norm_fwd(&a, ptr(ws), n, stream_of(x)), "xva_group_norm_act_fwd");
@@ -375,7 +376,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const Tensor dw = weight.defined() && ctx->needs_input_grad(1) ? at::empty(weight.sizes(), weight.options()) : Tensor();
         const Tensor db = bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1) ? at::empty(bias.sizes(), bias.options()) : Tensor();
         a.dy = ptr(dy); a.out = ptr(dx); a.dweight = (float*)ptr(dw); a.dbias = (float*)ptr(db);
-        for (int e = 0; e < 2; ++e) { a.dy_stride[e] = dy.stride(e); a.out_stride[e] = dx.stride(e); }
+        for (int e = 0; e < 2; ++e) { a.dy_stride[e] = step(dy, e); a.out_stride[e] = step(dx, e); }
         const int64_t n = lib.norm_ws(&a, 1);
         const Tensor ws = workspace(n, x);
         call(lib.norm_bwd(&a, ptr(ws), n, stream_of(x)), "xva_group_norm_act_bwd");
