@@ -313,7 +313,7 @@ def test_one_row_or_item_at_any_stride(dt, B, T):
     from xva_trainer_amd import seq_ops as S
     whole = torch.randn(B * 301 * 2051 + 8, device="cuda").to(DTYPES[dt])
     for sb, st in ((301 * 2051, 2048), (2048, 2051), (2051 * 8, 3)):
-        x = whole.as_strided((B, T, 2048), (sb if B == 1 else 2048 * T, st if T == 1 else 2048)).requires_grad_(True)
+        x = whole.as_strided((B, T, 2048), (sb if B == 1 else 2048 * T, st if T == 1 else 2048, 1)).requires_grad_(True)
         want = x.detach().clone(memory_format=torch.contiguous_format).requires_grad_(True)
         dy = torch.randn(B, T, 2048, device="cuda").to(DTYPES[dt])
         for G in (2, 32):
