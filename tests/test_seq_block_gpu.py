@@ -92,3 +92,43 @@ def test_block_forward_and_gradient(dt, tol):
     for name, a, b in zip(["y", "last", "dx"] + ["d" + n for n in p], got, ref):
         rel = ((a.double().cpu() - b).norm() / b.norm()).item()
         assert rel < 40 * tol, (name, rel)
+
+
+def _calls(S):
+    """name -> (call, leaves): each operator, small."""
+    plan = S.RotaryPlan(8)
+    n = lambda *s: torch.randn(*s, device="cuda").requires_grad_(True)
+    half = lambda *s: torch.randn(*s, device="cuda").half().requires_grad_(True)
+    return {"rotary": (lambda q, k: S.rotary(plan, q, k)[0], [n(2, 3, 2, 8), n(2, 3, 1, 8)]),
+            "differential_attention": (S.differential_attention, [half(2, 5, 2, 2, 8), half(2, 5, 1, 2, 8), half(2, 5, 1, 16), n(2)]),
+            "gated_recurrence": (lambda x, g, h: S.gated_recurrence(x, g, h)[0], [n(2, 5, 4), n(2, 5, 4), n(2, 4)]),
+            "group_norm_act": (lambda x, w, b: S.group_norm_act(x, 2, w, b, act="silu"), [n(2, 5, 8), n(8), n(8)])}
+
+
+@pytest.mark.parametrize("op", ["differential_attention", "gated_recurrence", "group_norm_act"])
+def test_a_second_derivative_says_that_there_is_none(op):
+    """A gradient penalty added to another loss must not lose its own gradient without a word; the first gradient is the usual one."""
+    from xva_trainer_amd import seq_ops as S
+    call, leaves = _calls(S)[op]
+    want = torch.autograd.grad(call(*leaves).float().sum(), leaves)
+    y = call(*leaves).float().sum()
+    got = torch.autograd.grad(y, leaves, create_graph=True)
+    assert all(torch.equal(a, b.detach()) for a, b in zip(want, got))
+    for g in got:
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (y + g.float().square().sum()).backward(retain_graph=True)
+
+
+def test_a_rotation_of_a_constant_gradient_is_a_constant():
+    """The rotation's gradient does not depend on what is rotated: its second derivative is nothing, unless the incoming gradient is a variable."""
+    from xva_trainer_amd import seq_ops as S
+    call, (q, k) = _calls(S)["rotary"]
+    y = call(q, k)
+    g, = torch.autograd.grad(y.sum(), q, create_graph=True)
+    want, = torch.autograd.grad(y.sum(), q, retain_graph=True)
+    got, = torch.autograd.grad(y.sum() + g.square().sum(), q)
+    assert torch.equal(got, want)
+    y = call(q, k)
+    g, = torch.autograd.grad(y.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        g.sum().backward()

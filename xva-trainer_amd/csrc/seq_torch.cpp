@@ -77,10 +77,11 @@ Tensor workspace(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::emp
 Tensor floats(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options().dtype(at::kFloat)); }
 int small(int64_t v, const char* what) { REFUSE(v < 0 || v > INT32_MAX, what, " ", v); return (int)v; }
 
-// a gradient taken with create_graph is right, and says so if it is differentiated again
-variable_list once(variable_list out, const variable_list& grads) {
+// A gradient taken with create_graph is right, and says so if it is differentiated again.  Whether the incoming gradients require one does not matter: the result
+// depends on the saved inputs too (of a linear map it does not: without such a gradient it is a constant).
+variable_list once(variable_list out, const variable_list& grads, bool linear = false) {
     if (!at::GradMode::is_enabled()) return out;
-    bool any = false;
+    bool any = !linear;
     for (const Tensor& g : grads) any = any || (g.defined() && g.requires_grad());
     if (!any) return out;
     auto fn = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", (int)out.size());
@@ -139,7 +140,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
             const auto got = rotary_launch(dq, dk, r, true, false);
             out[0] = got.first; out[1] = got.second;
         } else if (dk.defined()) out[1] = rotary_launch(dk, Tensor(), r, true, false).first;
-        return once(out, grads);
+        return once(out, grads, true);
     }
 };
 
