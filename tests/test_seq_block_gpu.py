@@ -132,3 +132,14 @@ def test_a_rotation_of_a_constant_gradient_is_a_constant():
     g, = torch.autograd.grad(y.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("op", ["rotary", "differential_attention", "gated_recurrence", "group_norm_act"])
+def test_a_tangent_of_the_incoming_gradient_is_refused(op):
+    import torch.autograd.forward_ad as fwd
+    from xva_trainer_amd import seq_ops as S
+    call, leaves = _calls(S)[op]
+    y = call(*leaves)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, leaves[0], fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))

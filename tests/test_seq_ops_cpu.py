@@ -164,3 +164,28 @@ def test_group_norm_takes_weights_at_any_address(dtype):
                           out_stride1=2048, dy_stride0=300 * 2048, dy_stride1=2048, **at)
         assert entry("xva_group_norm_act_fwd")(C.byref(a), None, 0, None) == -3
         assert entry("xva_group_norm_act_bwd")(C.byref(a), None, 0, None) == -3
+
+
+def _every_call():
+    """Each operator on host tensors; (x, others): the call takes a tensor like x in x's place."""
+    plan, x, lam = S.RotaryPlan(8, device="cpu"), torch.zeros(1, 2, 2, 8), torch.zeros(2)
+    half = torch.zeros(1, 2, 2, 2, 8).half()
+    return {"rotary q": (x, lambda t: S.rotary(plan, t)), "rotary k": (x, lambda t: S.rotary(plan, x, t)),
+            "attention q": (half, lambda t: S.differential_attention(t, half, half[:, :, :, 0].repeat(1, 1, 1, 2), lam)),
+            "attention lam": (lam, lambda t: S.differential_attention(half, half, half[:, :, :, 0].repeat(1, 1, 1, 2), t)),
+            "recurrence gate": (x[0], lambda t: S.gated_recurrence(x[0], t)), "recurrence h0": (x[0, 0], lambda t: S.gated_recurrence(x[0], x[0], t)),
+            "norm x": (x[0], lambda t: S.group_norm_act(t, 2)), "norm bias": (x[0, 0, 0], lambda t: S.group_norm_act(x[0], 2, None, t))}
+
+
+@pytest.mark.parametrize("which", list(_every_call()))
+def test_forward_mode_and_tracing_are_refused(which):
+    """A tangent would be dropped and a trace would hold no launch, both without a word (refused before the device is looked at)."""
+    import torch.autograd.forward_ad as fwd
+    x, call = _every_call()[which]
+    with fwd.dual_level():
+        with pytest.raises(S.XvaError, match="forward-mode"):
+            call(fwd.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(S.XvaError, match="device tensors"):
+        call(x)
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(call, (x,), check_trace=False)

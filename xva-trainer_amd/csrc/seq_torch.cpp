@@ -7,6 +7,8 @@
 //
 // The kernel library is not linked: seq_ops.py hands over the addresses of its entry points (`bind`), so that both sides use the one that _lib.py has loaded.
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -50,8 +52,13 @@ int dtype_of(const Tensor& t) {
         default: return -1;
     }
 }
-// all of them on the GPU of the first one
+bool has_tangent(const Tensor& t) { return t.defined() && torch::autograd::isFwGradDefined(t); }
+// all of them on the GPU of the first one, and nothing of torch's under way that the launches would drop out of without a word
 void on_one_device(const Tensor& first, std::initializer_list<Tensor> others) {
+    bool dual = has_tangent(first);
+    for (const Tensor& t : others) dual = dual || has_tangent(t);
+    REFUSE(dual, "forward-mode derivatives: these operators have backward passes only");
+    REFUSE(torch::jit::tracer::isTracing(), "torch.jit.trace would record none of these operators' launches");
     REFUSE(!first.is_cuda(), "libxvahip ops need device tensors; got a ", first.device(), " tensor (no CPU fallback exists)");
     for (const Tensor& t : others) REFUSE(t.defined() && t.device() != first.device(), "tensors on ", first.device(), " and ", t.device());
 }
@@ -80,6 +87,7 @@ int small(int64_t v, const char* what) { REFUSE(v < 0 || v > INT32_MAX, what, " 
 // A gradient taken with create_graph is right, and says so if it is differentiated again.  Whether the incoming gradients require one does not matter: the result
 // depends on the saved inputs too (of a linear map it does not: without such a gradient it is a constant).
 variable_list once(variable_list out, const variable_list& grads, bool linear = false) {
+    for (const Tensor& g : grads) REFUSE(has_tangent(g), "forward-mode derivatives of a backward pass");
     if (!at::GradMode::is_enabled()) return out;
     bool any = !linear;
     for (const Tensor& g : grads) any = any || (g.defined() && g.requires_grad());

@@ -11,7 +11,8 @@ The reference has none of these (its text encoder is `RelativePositionMultiHeadA
 dimension; one that is not contiguous in the last, or not aligned as a kernel needs it, is copied first.  Ragged batches give `lens` (B,) int32: rows at or
 behind an item's length are not read, and are zero in the results.  Everything is differentiable through torch.autograd, launches on torch's current stream of
 the tensors' device, does not synchronise and can be captured into a graph (a backward pass, as with every torch operator, only while no eager graph of the same
-leaves lives: torch would tie the capture to the eager graph's stream).  There is no CPU fallback."""
+leaves lives: torch would tie the capture to the eager graph's stream).  There are no second derivatives (they raise), no forward mode and no torch.jit.trace
+(both refused).  There is no CPU fallback."""
 import ctypes as C
 import math
 
