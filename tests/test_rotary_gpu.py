@@ -159,3 +159,24 @@ def test_refusals():
         with pytest.raises(S.XvaError):
             bad()
     assert math.isclose(S.RotaryPlan(8, gain=2.0).gain, 2.0)
+
+
+def test_in_place_refuses_views_that_overlap():
+    """Views that are not dense: heads of one projection that lie on each other, and windows over it."""
+    from xva_trainer_amd import seq_ops as S
+    plan = S.RotaryPlan(32)
+    whole = torch.randn(2, 5, 8 * 32 + 3, device="cuda")
+    heads = lambda a, n: whole[..., a:a + n * 32].unflatten(-1, (n, 32))
+    for bad in (lambda: S.rotary(plan, heads(0, 5), heads(4 * 32, 2), inplace=True), lambda: S.rotary(plan, heads(0, 4), heads(4 * 32 - 1, 2), inplace=True),
+                lambda: S.rotary(plan, whole.as_strided((2, 5, 4, 32), (1295, 259, 31, 1)), inplace=True)):
+        with pytest.raises(S.XvaError, match="inplace"):
+            bad()
+    # each head's query beside its key, heads outside rows, and different projections
+    pairs = whole[..., :256].unflatten(-1, (4, 2, 32))
+    want = S.rotary(plan, pairs[..., 0, :], pairs[..., 1, :])
+    got = S.rotary(plan, pairs[..., 0, :], pairs[..., 1, :], inplace=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    cache = torch.randn(2, 6, 50, 32, device="cuda").transpose(1, 2)
+    want = S.rotary(plan, cache[:, 7:12, :4], cache[:, 7:12, 4:])
+    got = S.rotary(plan, cache[:, 7:12, :4], cache[:, 7:12, 4:], inplace=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

@@ -189,3 +189,43 @@ def test_forward_mode_and_tracing_are_refused(which):
         call(x)
     with pytest.raises(RuntimeError, match="torch.jit.trace"):
         torch.jit.trace(call, (x,), check_trace=False)
+
+
+def test_views_that_share_elements_are_told_apart_from_those_that_do_not():
+    """Every answer against the elements themselves; views as slices of projections have them, and any strides.  "Not known" (2) is refused like a meeting: it may
+    only be said of strides that no slice has."""
+    import random
+
+    from xva_trainer_amd import _seq_torch
+    rng, store = random.Random(5), torch.zeros(4000)
+    places = lambda t: [torch.arange(t.shape[3])[None] + (torch.cartesian_prod(*[torch.arange(n) for n in t.shape[:3]]) * torch.tensor(t.stride()[:3])).sum(1, keepdim=True)
+                        + t.storage_offset()][0]
+    said = {0: 0, 1: 0, 2: 0}
+    for turn in range(3000):
+        shape = [rng.randint(1, 4) for _ in range(3)] + [rng.randint(2, 6)]
+        if turn % 2:                                                    # slices of one projection, in either order of heads and rows
+            heads, width = rng.randint(1, 5), shape[3] + rng.choice([0, 0, 1, 3])
+            whole = store[:shape[0] * shape[1] * heads * width].view(shape[0], shape[1], heads, width)
+            cut = lambda: (lambda a, d: whole[:, :, a:rng.randint(a + 1, heads), d:d + shape[3]])(rng.randint(0, heads - 1), rng.randint(0, width - shape[3]))
+            q, k = cut(), cut()
+            if rng.random() < 0.3:
+                q, k = q.transpose(1, 2), k.transpose(1, 2)
+            k = k[:, :q.shape[1]]
+            q = q[:, :k.shape[1]]
+        else:
+            view = lambda n: store.as_strided(shape[:2] + [n, shape[3]], [rng.choice([0, 1, 5, 7, 24, 60, 100]) for _ in range(3)] + [1], rng.randint(0, 60))
+            q, k = view(shape[2]), view(rng.randint(1, 4))
+        at = [places(t).flatten() for t in (q, k)]
+        for t, a in zip((q, k), at):
+            own = _seq_torch.overlap(t, None)
+            said[own] += 1
+            # (elements of a head never meet: a place that comes twice belongs to two heads)
+            assert own == (1 if a.unique().numel() < a.numel() else 0), (t.shape, t.stride())
+        both = _seq_torch.overlap(q, k)
+        said[both] += 1
+        assert both == int(torch.isin(at[0], at[1]).any()), (q.shape, q.stride(), q.storage_offset(), k.shape, k.stride(), k.storage_offset())
+    assert said[0] > 500 and said[1] > 500 and said[2] == 0
+    whole = torch.zeros(64, 512, 24, 128)                                # sizes of a model
+    assert _seq_torch.overlap(whole[:, :, :16], whole[:, :, 16:]) == 0 and _seq_torch.overlap(whole[:, :, :17], whole[:, :, 16:]) == 1
+    assert _seq_torch.overlap(whole[..., :64], whole[..., 64:]) == 0 and _seq_torch.overlap(whole, torch.zeros(64, 512, 2, 128)) == 0
+    assert _seq_torch.overlap(whole.transpose(1, 2)[:, :16], whole.transpose(1, 2)[:, 16:20]) == 0

@@ -10,10 +10,11 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <algorithm>
 #include <cmath>
+#include <vector>
 #include "../../include/xva_hip.h"
 
 namespace {
@@ -101,6 +102,61 @@ variable_list once(variable_list out, const variable_list& grads, bool linear = 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------- rotary ----
+// Do elements of (items, rows, heads, D) views lie on each other: of q and k, or, without k, of two different heads of q?  torch's own answer is "too hard" for views
+// that are not dense, and slices of one projection are not.  Two elements meet where sum n_e s_e + r equals the distance of the two views, n_e a difference of indices
+// along one of the strides s_e, |r| < D: a search over the n_e from the widest stride down, which has a candidate or two each where strides enclose each other.
+enum Overlap { APART, MEETING, UNKNOWN };
+struct Search {
+    struct Dim { int64_t stride, lo, hi; };
+    std::vector<Dim> dims;
+    std::vector<std::pair<int64_t, int64_t>> rest;         // least and largest sum over dims e ..
+    bool same;                                             // all n_e = 0 is an element's own place
+    int left = 4096;                                       // candidates that are tried: beyond them nothing is promised
+    void add(const Tensor& t, bool other) {
+        for (int e = 0; e < 3; ++e) {
+            if (t.size(e) < 2) continue;
+            const int64_t n = t.size(e) - 1;
+            Dim* d = nullptr;
+            for (Dim& x : dims) d = x.stride == t.stride(e) && !same ? &x : d;
+            if (!d) { dims.push_back({t.stride(e), 0, 0}); d = &dims.back(); }
+            if (other || same) d->lo -= n;
+            if (!other || same) d->hi += n;
+        }
+    }
+    bool meets(size_t e, int64_t target, bool moved) {
+        if (--left < 0) return true;
+        if (e == dims.size()) return (moved || !same) && target >= rest[e].first && target <= rest[e].second;
+        const Dim& d = dims[e];
+        for (int64_t n = d.lo; n <= d.hi; ++n) {
+            if (d.stride > 0) {
+                const int64_t least = target - rest[e + 1].second, most = target - rest[e + 1].first;      // of n * stride
+                const int64_t first = least > 0 ? (least + d.stride - 1) / d.stride : -(-least / d.stride);
+                if (n < first) n = first;
+                if (n > d.hi || n * d.stride > most) return false;
+            }
+            if (meets(e + 1, target - n * d.stride, moved || n != 0)) return true;
+        }
+        return false;
+    }
+    Overlap run(int64_t target, int64_t D) {
+        std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+        rest.assign(dims.size() + 1, {1 - D, D - 1});
+        for (size_t e = dims.size(); e-- > 0;) rest[e] = {rest[e + 1].first + dims[e].lo * dims[e].stride, rest[e + 1].second + dims[e].hi * dims[e].stride};
+        const bool found = meets(0, target, false);
+        return left < 0 ? UNKNOWN : (found ? MEETING : APART);
+    }
+};
+Overlap overlap(const Tensor& q, const Tensor& k) {
+    if (q.numel() == 0 || (k.defined() && k.numel() == 0)) return APART;
+    Search s;
+    s.same = !k.defined();
+    s.add(q, false);
+    if (s.same) return s.run(0, q.size(3));
+    s.add(k, true);
+    const int64_t bytes = (const char*)k.data_ptr() - (const char*)q.data_ptr(), es = q.element_size();
+    return bytes % es ? UNKNOWN : s.run(bytes / es, q.size(3));       // (q + i = k + j: i - j is the distance from q to k)
+}
+
 struct RotaryArgs { Tensor turns, pos; int64_t rd; bool interleaved; double gain; };
 
 std::pair<Tensor, Tensor> rotary_launch(const Tensor& q_, const Tensor& k_, const RotaryArgs& r, bool inverse, bool inplace) {
@@ -170,9 +226,8 @@ variable_list rotary(const Tensor& turns, int64_t rd, bool interleaved, double g
     }
     if (inplace) {
         REFUSE(q.stride(3) != 1 || (k.defined() && k.stride(3) != 1), "inplace: a contiguous last dimension");
-        REFUSE(at::has_internal_overlap(q) == at::MemOverlap::Yes || (k.defined() && at::has_internal_overlap(k) == at::MemOverlap::Yes), "inplace: an expanded tensor");
-        REFUSE(k.defined() && k.numel() > 0 && (q.data_ptr() == k.data_ptr() || at::get_overlap_status(q, k) == at::MemOverlapStatus::Full || at::get_overlap_status(q, k) == at::MemOverlapStatus::Partial),
-               "inplace: q and k share memory");
+        for (const Tensor& t : {q, k}) REFUSE(t.defined() && overlap(t, Tensor()) != APART, "inplace: heads of an expanded or overlapping tensor lie on each other, or may");
+        REFUSE(k.defined() && overlap(q, k) != APART, "inplace: q and k share memory, or may");
         for (const Tensor& t : {q, k})
             if (t.defined()) t.unsafeGetTensorImpl()->bump_version();       // (a graph that saved it says so when it is run)
     }
@@ -436,6 +491,7 @@ PYBIND11_MODULE(_seq_torch, m) {
         set(lib.diff_bwd, e, "xva_diff_attention_bwd");
     });
     m.def("rotary", &rotary);
+    m.def("overlap", [](const Tensor& q, const MaybeTensor& k) { return (int)overlap(q, or_none(k)); });      // 0: apart, 1: elements meet, 2: not known
     m.def("differential_attention", &differential_attention);
     m.def("gated_recurrence", &gated_recurrence);
     m.def("group_norm_act", &group_norm_act);
