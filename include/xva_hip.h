@@ -722,8 +722,8 @@ int xva_sdp_dequant_bwd(const float* z_u, const float* dr, const float* d_z0_log
 
 /* Rotary positions.  q (B, T, H, D), k (B, T, Hk, D) (null with Hk = 0); pair i of the first rd elements of a head turns by position * turns[i]:
  * (a, b) -> gain (a cos - b sin, b cos + a sin), with (a, b) = elements (i, i + rd / 2), or (2 i, 2 i + 1) when `interleaved`; the other D - rd elements are
- * copied.  turns: rd / 2 fractions of a turn per position as 64-bit fixed point, so angles are exact at any 64-bit position.  positions: int32 or int64
- * (positions64) with strides over items and rows (0: the same for all), null: the row's index.  inverse: the angle negated — the gradient.
+ * copied.  turns: rd / 2 fractions of a turn per position as 64-bit fixed point, so the angle at position p is that of the table modulo a turn: off by
+ * p 2^-65 turns where each entry is within half a unit.  positions: int32 or int64 (positions64) with strides over items and rows (0: the same for all), null: the row's index.  inverse: the angle negated — the gradient.
  * In place: q_out == q and k_out == k with equal strides. */
 typedef struct {
     const void *q, *k;

@@ -180,3 +180,43 @@ def test_in_place_refuses_views_that_overlap():
     want = S.rotary(plan, cache[:, 7:12, :4], cache[:, 7:12, 4:])
     got = S.rotary(plan, cache[:, 7:12, :4], cache[:, 7:12, 4:], inplace=True)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("scaling,factor", [("none", 1.0), ("linear", 3.0), ("yarn", 16.0)])
+@pytest.mark.parametrize("first", [2 ** 31 - 40, 2 ** 40 + 12345, -2 ** 42 - 77, 2 ** 44])
+def test_positions_that_a_double_cannot_turn(scaling, factor, first):
+    """Angles by integers: position times the frequency in 60 digits, modulo a turn.  Allowed beside fp32's own 2^-20 (|a| + |b|): p times half a unit of the table,
+    p 2^-65 turns, 2^-18 radians at 2^44 - where a frequency in double would be off by 2^-12 of a turn."""
+    from decimal import Decimal as D, getcontext, localcontext
+
+    from xva_trainer_amd import seq_ops as S
+    torch.manual_seed(6)
+    rd = 64
+    plan = S.RotaryPlan(rd, scaling=scaling, factor=factor)
+    q = torch.randn(1, 9, 2, rd, device="cuda")
+    pos = torch.arange(first, first + 9, device="cuda")
+    with localcontext():
+        getcontext().prec = 80
+        pi, ang = D("3.14159265358979323846264338327950288419716939937510582097494459230781640628620900"), []
+        for p in pos.tolist():
+            row = []
+            for i in range(rd // 2):
+                f = D(10000) ** (D(-2 * i) / D(rd))
+                if scaling == "linear":
+                    f = f / D(factor)
+                elif scaling == "yarn":
+                    pair = lambda turns: rd * math.log(4096 / (turns * 2 * math.pi)) / (2 * math.log(10000.0))
+                    low, high = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), rd - 1)
+                    ramp = min(max(D(i - low) / D(max(high - low, 1e-3)), D(0)), D(1))
+                    f = f * (1 - ramp) + f / D(factor) * ramp
+                turn = D(p) * f / (2 * pi)
+                row.append(float((turn - turn.to_integral_value()) * 2 * pi))
+            ang.append(row)
+    ang = torch.tensor(ang, dtype=torch.float64)[None, :, None]
+    x, n = q.double().cpu(), rd // 2
+    a, b = x[..., :n], x[..., n:]
+    c, s = ang.cos() * plan.gain, ang.sin() * plan.gain
+    ref = torch.cat((a * c - b * s, b * c + a * s), -1)
+    size = (a.abs() + b.abs()) * plan.gain
+    err = torch.cat((size, size), -1) * (2.0 ** -20 + abs(first) * 2.0 ** -65 * 2 * math.pi * 1.01)
+    close(S.rotary(plan, q, positions=pos), ref, rounded(ref, q.dtype, err), "q")

@@ -229,3 +229,27 @@ def test_views_that_share_elements_are_told_apart_from_those_that_do_not():
     assert _seq_torch.overlap(whole[:, :, :16], whole[:, :, 16:]) == 0 and _seq_torch.overlap(whole[:, :, :17], whole[:, :, 16:]) == 1
     assert _seq_torch.overlap(whole[..., :64], whole[..., 64:]) == 0 and _seq_torch.overlap(whole, torch.zeros(64, 512, 2, 128)) == 0
     assert _seq_torch.overlap(whole.transpose(1, 2)[:, :16], whole.transpose(1, 2)[:, 16:20]) == 0
+
+
+@pytest.mark.parametrize("kw", [{}, {"base": 500000.0}, {"scaling": "linear", "factor": 3.0}, {"scaling": "ntk", "factor": 8.0}, {"scaling": "yarn", "factor": 16.0}])
+@pytest.mark.parametrize("rd", [2, 6, 64, 254])
+def test_turns_to_half_a_unit(kw, rd):
+    """The table against the definition in 80 digits, each power by itself: half a unit of 2^-64 of a turn (and a billionth of one for the digits)."""
+    from decimal import Decimal as D, getcontext, localcontext
+    plan = S.RotaryPlan(rd, device="cpu", **kw)
+    with localcontext():
+        getcontext().prec = 80
+        pi = D("3.141592653589793238462643383279502884197169399375105820974944592307816406286208998628034825")
+        base, factor, scaling = D(kw.get("base", 10000.0)), D(kw.get("factor", 1.0)), kw.get("scaling", "none")
+        if scaling == "ntk" and rd > 2:
+            base = base * factor ** (D(rd) / D(rd - 2))
+        for i, t in enumerate(plan.turns.tolist()):
+            f = base ** (D(-2 * i) / D(rd))
+            if scaling == "linear":
+                f = f / factor
+            elif scaling == "yarn":
+                pair = lambda turns: rd * math.log(4096 / (turns * 2 * math.pi)) / (2 * math.log(10000.0))
+                low, high = max(math.floor(pair(32.0)), 0), min(math.ceil(pair(1.0)), rd - 1)
+                ramp = min(max(D(i - low) / D(max(high - low, 1e-3)), D(0)), D(1))
+                f = f * (1 - ramp) + f / factor * ramp
+            assert abs(D(t % 2 ** 64) - f / (2 * pi) * 2 ** 64) <= D(1) / 2 + D(10) ** -9, i

@@ -10,7 +10,7 @@
 //
 // Angles of far positions: p w in fp32 is off by p w 2^-24 radians (half a radian at a position of 8 million).  The plan holds w / 2 pi as a 64-bit
 // fixed-point fraction of a turn, so that p * w modulo one turn is the low half of an integer product: exact for every 64-bit position but for the table's
-// own rounding (p 2^-65 turns).  sincospif then takes the reduced turn.
+// own rounding (half a unit: p 2^-65 turns, fp32's own step at about 2^40).  sincospif then takes the reduced turn.
 #include "xva_common.h"
 #include "../../include/xva_hip.h"
 #include "seq_vec.h"

@@ -14,7 +14,9 @@ the tensors' device, does not synchronise and can be captured into a graph (a ba
 leaves lives: torch would tie the capture to the eager graph's stream).  There are no second derivatives (they raise), no forward mode and no torch.jit.trace
 (both refused).  There is no CPU fallback."""
 import ctypes as C
+import decimal
 import math
+from decimal import Decimal
 
 import torch
 
@@ -30,6 +32,8 @@ _ENTRIES = ("xva_last_error", "xva_rotary", "xva_group_norm_workspace_bytes", "x
             "xva_recurrence_state_floats", "xva_recurrence_fwd", "xva_recurrence_bwd", "xva_diff_attention_workspace_bytes", "xva_diff_attention_fwd",
             "xva_diff_attention_bwd")
 _seq_torch.bind({n: C.cast(getattr(_lib.lib, n), C.c_void_p).value for n in _ENTRIES}, XvaError)
+
+_PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628621")
 
 
 class RotaryPlan:
@@ -53,24 +57,29 @@ class RotaryPlan:
             raise XvaError("base %g, factor %g, original_length %d, beta_fast %g, beta_slow %g" % (base, factor, original_length, beta_fast, beta_slow))
         n = rotary_dim // 2
         self.rotary_dim, self.interleaved, self.gain = rotary_dim, bool(interleaved), 1.0
-        if scaling == "ntk" and rotary_dim > 2:
-            base = base * factor ** (rotary_dim / (rotary_dim - 2.0))
-        freq = [base ** (-2.0 * i / rotary_dim) for i in range(n)]
-        if scaling == "linear":
-            freq = [f / factor for f in freq]
-        elif scaling == "yarn":
-            def pair_of(turns):
-                return rotary_dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
-            low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
-            for i in range(n):
-                ramp = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)
-                freq[i] = freq[i] * (1.0 - ramp) + freq[i] / factor * ramp
-            self.gain = 0.1 * math.log(factor) + 1.0
+        # In 60 digits: a double's 53 bits of a frequency leave 2^-56 of a turn for every position, which is 1e-4 radians at 2^40
+        with decimal.localcontext(decimal.Context(prec=60, Emin=-10 ** 6, Emax=10 ** 6)):
+            by, longer = Decimal(float(base)), Decimal(float(factor))
+            if scaling == "ntk" and rotary_dim > 2:
+                by = by * (longer.ln() * rotary_dim / (rotary_dim - 2)).exp()
+            ratio, freq = (by.ln() * -2 / rotary_dim).exp(), [Decimal(1)]
+            while len(freq) < n:
+                freq.append(freq[-1] * ratio)
+            if scaling == "linear":
+                freq = [f / longer for f in freq]
+            elif scaling == "yarn":
+                def pair_of(turns):
+                    return rotary_dim * math.log(original_length / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+                low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
+                for i in range(n):
+                    ramp = min(max(Decimal(i - low) / Decimal(max(high - low, 1e-3)), Decimal(0)), Decimal(1))
+                    freq[i] = freq[i] * (1 - ramp) + freq[i] / longer * ramp
+                self.gain = 0.1 * math.log(factor) + 1.0
+            # fractions of a turn per position as 64-bit fixed point, to half a unit (two's complement: the upper half reads as negative)
+            fixed = [int((f / (2 * _PI) * 2 ** 64).to_integral_value()) % 2 ** 64 for f in freq]
+        self.frequencies = [float(f) for f in freq]
         if gain is not None:
             self.gain = float(gain)
-        self.frequencies = freq
-        # fractions of a turn per position as 64-bit fixed point (two's complement: the upper half reads as negative)
-        fixed = [int(round(f / (2.0 * math.pi) * 2.0 ** 64)) % 2 ** 64 for f in freq]
         self.turns = torch.tensor([v - 2 ** 64 if v >= 2 ** 63 else v for v in fixed], dtype=torch.int64).to(device)
 
     def to(self, device):
