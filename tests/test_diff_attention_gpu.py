@@ -337,3 +337,58 @@ def test_one_row_of_a_projection_of_any_width(Tq, width):
     k, v = whole[1:, ..., :2 * d].unflatten(-1, (1, 2, d))[:, :T if Tq > 1 else 1], whole[:1, :T if Tq > 1 else 1, 64:64 + 2 * d].unflatten(-1, (1, 2 * d))
     dout = torch.randn(1, T, width, device="cuda").bfloat16()[:, :Tq, :H * 2 * d].unflatten(-1, (H, 2 * d))
     _run(q, k, v, torch.rand(H, device="cuda"), dout, causal=True)
+
+
+def _norm_bounds(q, k, v, lam, dout, causal):
+    """Gradients in 64 bits, and how far the norm of each one's error may be: roundings are independent, so a sum of products that are each off by u of themselves is off
+    by u of its norm or so.  P_1 - lam P_2 or dS as an operand, the maps' outputs behind D, the result itself: 4 u bounds them, fp32's own E beside them.  Besides, each
+    element of the result is off by 2^-25, and each weight that meets dO in dV."""
+    u, tiny = HALF[q.dtype], TINY[q.dtype]
+    q, k, v, lam, dout = (t.detach().double() for t in (q, k, v, lam, dout))
+    q, k, v, lam = (t.requires_grad_(True) for t in (q, k, v, lam))
+    share, n = q.shape[2] // k.shape[2], q.shape[1]
+    s = torch.matmul(q.permute(0, 2, 3, 1, 4), k.permute(0, 2, 3, 4, 1).repeat_interleave(share, 1).contiguous()) * q.shape[-1] ** -0.5
+    if causal:
+        s = s.masked_fill(torch.ones(n, k.shape[1], dtype=torch.bool, device=q.device).triu(1 + k.shape[1] - n), -math.inf)
+    p = torch.softmax(s, -1)
+    out = torch.matmul(p[:, :, 0] - lam[:, None, None] * p[:, :, 1], v.permute(0, 2, 1, 3).repeat_interleave(share, 1).contiguous()).permute(0, 2, 1, 3)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    bound = lambda g, more=0.0: (4 * u + E) * g.norm().item() + tiny * g.numel() ** 0.5 + more
+    parts = {"dq_1": grads[0][..., 0, :], "dq_2": grads[0][..., 1, :], "dk_1": grads[1][..., 0, :], "dk_2": grads[1][..., 1, :], "dv": grads[2]}
+    return {m: (g, bound(g, tiny * (k.shape[1] * dout.square().sum().item()) ** 0.5 if m == "dv" else 0.0)) for m, g in parts.items()}
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("lam_size", [0.5, 0.01, 1e-4, 30.0])
+@pytest.mark.parametrize("dout_size,H,Hk,T,d,causal", [(1.0, 2, 1, 860, 48, False), (1e-3, 4, 2, 860, 48, False), (1e-4, 1, 1, 4096, 48, False), (1e-3, 2, 2, 700, 64, True),
+                                                       (1e-3, 2, 1, 300, 32, True), (1e-3, 4, 1, 90, 16, False)])
+def test_gradients_of_any_size(dt, lam_size, dout_size, H, Hk, T, d, causal):
+    """The loss of a training step is a mean, so dO is small; lam may be: no part of the gradient sinks into fp16's subnormal numbers on the way, judged by the norm of
+    its error (values are large enough that the results themselves do not)."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(2, T, T, H, Hk, d, dt, seed=13)
+    q, k, v = (t * 4 if t is v else t for t in (q, k, v))
+    lam = lam_size * (1 + 0.2 * torch.randn(H, device="cuda"))
+    dout = (dout.float() * dout_size).to(q.dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    got = torch.autograd.grad(S.differential_attention(*leaves, causal=causal), leaves[:3], dout)
+    got = {"dq_1": got[0][..., 0, :], "dq_2": got[0][..., 1, :], "dk_1": got[1][..., 0, :], "dk_2": got[1][..., 1, :], "dv": got[2]}
+    for name, (ref, bound) in _norm_bounds(q, k, v, lam, dout, causal).items():
+        off = (got[name].double() - ref).norm().item()
+        assert off <= bound, "%s off by %.3g of %.3g, %.3g allowed" % (name, off, ref.norm().item(), bound)
+
+
+def test_gradients_beyond_the_type_on_the_way():
+    """dO . v of a quarter of a million, more than fp16 holds, on the way to gradients of a few hundred; items of very different size in one batch."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(2, 300, 300, 2, 1, 48, "fp16", seed=14)
+    q, k, v, dout = q * 0.05, k * 0.05, v * 4, dout * 5000
+    dout[1] *= 1e-7
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    got = torch.autograd.grad(S.differential_attention(*leaves, causal=True), leaves[:3], dout)
+    assert all(g.isfinite().all() for g in got)
+    for b in range(2):
+        mine = {"dq_1": got[0][b:b + 1, ..., 0, :], "dq_2": got[0][b:b + 1, ..., 1, :], "dk_1": got[1][b:b + 1, ..., 0, :], "dk_2": got[1][b:b + 1, ..., 1, :], "dv": got[2][b:b + 1]}
+        for name, (ref, bound) in _norm_bounds(q[b:b + 1], k[b:b + 1], v[b:b + 1], lam, dout[b:b + 1], True).items():
+            off = (mine[name].double() - ref).norm().item()
+            assert off <= bound, "%s of item %d off by %.3g of %.3g, %.3g allowed" % (name, b, off, ref.norm().item(), bound)

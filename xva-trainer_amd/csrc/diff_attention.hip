@@ -19,7 +19,9 @@
 // matrix units 47 - 49 % busy, vector units 59 - 66 %, two waves to a SIMD.  32 x 860 ragged frames, 4 heads of 48: 81 + 155 us: 688 query blocks on 512 places, and
 // scores of 48 columns take matrix steps of 64.  32 x 150, heads of 32: 13 + 16 us.  One query on each of 16 ragged caches of up to 8192 keys, 16 heads of 64 on 4 keys':
 // 41 us (4.7 TB/s) and 7 for the join.
-// Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands (the accumulators are fp32; sums, maxima and logsumexp stay fp32).
+// Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands, which is what the matrix units take at this rate; each map's own output, to the
+// tensors' type, kept for the backward pass, whose D_m is made from it (in fp32 it would be another 2 x 4 bytes a value, written and read).  Accumulators, scores, sums,
+// maxima, logsumexp and D stay fp32.  fp16 holds dS by powers of two in its normal range (range_kernel).
 //
 // Tiles: 64 rows x 64 columns of 16-bit values (attn_tile.h).  d <= 32: one image holds both maps' 32 columns side by side; d <= 64: one image for each map.
 // V and dO (2 d wide): one or two images.  Rows behind the last live one read that one, with P = 0.
@@ -39,6 +41,8 @@ struct Args {
     int lam_type;
     float* lam32;                                 // backward: the same in fp32, for the scalar unit (rowdot_kernel leaves it)
     float *lse, *D, *dlam_part;
+    float *norms;                                 // fp16 backward: squared norms of dO's rows (B, H, Tq), then of v's (B, Hk, Tk)
+    float *range;                                 // fp16 backward: of each (item, key head) the factors that keep dS in the type's range (see range_kernel)
     const int32_t *ql, *kl;
     int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
     int B, Tq, Tk, H, Hk, share, d, causal;
@@ -705,12 +709,27 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a, const float* __re
 }
 
 // ================================================================================ backward ====
-// D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns
+// D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns.  fp16: the squared norms of dO's rows beside it, and of v's by the workgroups behind those (`first_v`)
 template <bool F16>
-__global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
-    const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tq * a.H;
+__global__ __launch_bounds__(256) void rowdot_kernel(Args a, unsigned first_v) {
     const int c = (threadIdx.x & 15) * 8, w = 2 * a.d;
-    float s[2] = {0.f, 0.f};
+    auto join = [](float v) { v += __shfl_xor(v, 1, 64); v += __shfl_xor(v, 2, 64); v += __shfl_xor(v, 4, 64); return v + __shfl_xor(v, 8, 64); };
+    if (F16 && blockIdx.x >= first_v) {
+        const int64_t id = (int64_t)(blockIdx.x - first_v) * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tk * a.Hk, bt = id / a.Hk;
+        const int hk = (int)(id - bt * a.Hk), b = (int)(bt / a.Tk), t = (int)(bt - (int64_t)b * a.Tk);
+        float n = 0.f;
+        if (id < rows && c < w && t < len_of(a.kl, b, a.Tk)) {
+            const uint4 vr = *reinterpret_cast<const uint4*>(a.v + b * a.vb + t * a.vt + hk * a.vh + c);
+            const uint32_t vw[4] = {vr.x, vr.y, vr.z, vr.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { float v0, v1; unpack2<F16>(vw[e], v0, v1); n += v0 * v0 + v1 * v1; }
+        }
+        n = join(n);
+        if (id < rows && (threadIdx.x & 15) == 0) a.norms[(int64_t)a.B * a.H * a.Tq + ((int64_t)b * a.Hk + hk) * a.Tk + t] = n;
+        return;
+    }
+    const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tq * a.H;
+    float s[2] = {0.f, 0.f}, n = 0.f;
     const int64_t bt = id / a.H;
     const int h = (int)(id - bt * a.H), b = (int)(bt / a.Tq), t = (int)(bt - (int64_t)b * a.Tq);
     if (id < rows && c < w && t < len_of(a.ql, b, a.Tq)) {
@@ -725,15 +744,58 @@ __global__ __launch_bounds__(256) void rowdot_kernel(Args a) {
                 float g0, g1, o0, o1;
                 unpack2<F16>(gw[e], g0, g1); unpack2<F16>(ow[e], o0, o1);
                 s[m] += g0 * o0 + g1 * o1;
+                if (F16 && m == 0) n += g0 * g0 + g1 * g1;
             }
         }
     }
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-        s[m] += __shfl_xor(s[m], 1, 64); s[m] += __shfl_xor(s[m], 2, 64); s[m] += __shfl_xor(s[m], 4, 64); s[m] += __shfl_xor(s[m], 8, 64);
+    for (int m = 0; m < 2; ++m) s[m] = join(s[m]);
+    if (F16) {
+        n = join(n);
+        if (id < rows && (threadIdx.x & 15) == 0) a.norms[((int64_t)b * a.H + h) * a.Tq + t] = n;
     }
     if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
     if (id < a.H && (threadIdx.x & 15) == 0) a.lam32[id] = lam_of(a, (int)id);
+}
+
+// fp16 holds 2^-14 .. 2^16 in full: dS = P (dP - D) of a loss that is a mean over many values, or lam times it, lies below that and would be lost.  So dS is made
+// 2^up times as large, |dS| <= |dP - D| <= 2 max |dO_i| max |v_j| (norms over the 2 d columns) coming to at most 2^15, and dS_2 in dk takes lam / 2^el instead of
+// lam, 2^el >= |lam|; both are powers of two, undone in fp32 where sums are rounded.  One set of factors for all that adds up in a key head's dK, so an item whose
+// gradients are small beside another's keeps its own.  (860 keys, heads of 48, dO of 1e-3, lam 0.01: dk_2 off by
+// 9 % of its norm without this.  It costs 8 us of 226 on 32 x 860 frames, forward + backward: v's norms, a launch, a product for each pair in dK / dV.)
+// (2^up, 2^-up, el, 2^el).  A gradient or value that is not finite takes no factor: the results it reaches are lost as they are.
+struct Range {
+    float up, down, el, big;
+    template <bool F16> static __device__ __forceinline__ Range of(const Args& a, int b, int hk) {
+        if constexpr (!F16) return {1.f, 1.f, 0.f, 1.f};
+        else {
+            const int at = (b * a.Hk + hk) * 4;
+            return {uniform(a.range, at), uniform(a.range, at + 1), uniform(a.range, at + 2), uniform(a.range, at + 3)};
+        }
+    }
+};
+__global__ __launch_bounds__(1024) void range_kernel(Args a) {
+    __shared__ float sh[16];
+    const int b = blockIdx.x / a.Hk, hk = blockIdx.x - b * a.Hk;
+    const float* g = a.norms + ((int64_t)b * a.H + hk * a.share) * a.Tq;
+    const float* v = a.norms + (int64_t)a.B * a.H * a.Tq + (int64_t)blockIdx.x * a.Tk;
+    const int64_t ng = (int64_t)a.share * a.Tq;
+    float mg = 0.f, mv = 0.f;
+#pragma unroll 4
+    for (int64_t e = threadIdx.x; e < ng; e += 1024) mg = fmaxf(mg, g[e]);
+#pragma unroll 4
+    for (int e = threadIdx.x; e < a.Tk; e += 1024) mv = fmaxf(mv, v[e]);
+    mg = xva_block_max(mg, sh);
+    mv = xva_block_max(mv, sh);
+    if (threadIdx.x != 0) return;
+    const float bound = 2.002f * sqrtf(mg) * sqrtf(mv);             // (2 and some roundings)
+    float lam = 0.f;
+    for (int e = 0; e < a.share; ++e) lam = fmaxf(lam, fabsf(lam_of(a, hk * a.share + e)));
+    int up = 0, el = 0;
+    if (bound > 0.f && bound < INFINITY) { frexpf(bound, &up); up = 15 - up; }
+    if (lam > 0.f && lam < INFINITY) { frexpf(lam, &el); el = max(el, -100); }
+    float* to = a.range + (int64_t)blockIdx.x * 4;
+    to[0] = ldexpf(1.f, up); to[1] = ldexpf(1.f, -up); to[2] = (float)el; to[3] = ldexpf(1.f, el);
 }
 
 // A key block's 64-query tiles: of each query head that shares the keys, `per_head` from tile `t0` on
@@ -774,6 +836,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
     const bool any = kb.all > 0;
     const int begin = piece * a.piece, total = min(kb.all - begin, a.piece);
     if (piece > 0 && total <= 0) return;
+    const Range range = Range::of<F16>(a, b, hk);
     bf16x8 kf[2][2][S::KH], vf[2][S::VH];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -814,7 +877,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
     __syncthreads();
     auto tile = [&](const int it, const XVA_LDS uint8_t* smem, XVA_LDS uint8_t* next) {
         const int row0 = qtile * 64;
-        const float lam = uniform(a.lam32, hk * a.share + hs), loglam = __log2f(fabsf(lam)), minus = lam < 0.f ? 1.f : -1.f;
+        const float lam = uniform(a.lam32, hk * a.share + hs), loglam = __log2f(fabsf(lam)) - range.el, minus = lam < 0.f ? 1.f : -1.f, minus_big = minus * range.big;
         if (++hs == a.share) { hs = 0; --qtile; }
         if (it + 1 < total) fetch(hs, qtile * 64, next);
         const int wrow = row0 + t * 32;                       // this wave's 32 rows
@@ -856,16 +919,16 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
                             s[1][kt][r] = ok ? s[1][kt][r] : -INFINITY;
                         }
                 }
-                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768) * minus;
+                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768) * (minus * range.up);
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         // (|lam| in the exponent, its sign in the sums: no product more than without it)
-                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = exp2_(__builtin_fmaf(s[1][kt][r], a.c, loglam)), x = dp[kt][r];
+                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = exp2_(__builtin_fmaf(s[1][kt][r], a.c, loglam)), x = F16 ? dp[kt][r] * range.up : dp[kt][r];
                         s[0][kt][r] = p1 * x;
                         s[1][kt][r] = p2 * __builtin_fmaf(x, minus, dD[r]);
-                        dp[kt][r] = __builtin_fmaf(p2, minus, p1);
+                        dp[kt][r] = __builtin_fmaf(p2, minus_big, p1);
                     }
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -928,7 +991,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int dt = 0; dt < S::DT; ++dt)
-                    if (dt * 16 + ge * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + ge * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale);
+                    if (dt * 16 + ge * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + ge * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale * range.down * (m ? range.big : 1.f));
 #pragma unroll
             for (int dt = 0; dt < S::VT; ++dt)
                 if (dt * 16 + ge * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + ge * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], 1.f);
@@ -948,8 +1011,10 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
     if (kb.all <= a.piece) return;
     f32x4 v = ZERO4;
     for (int p = 0; p * a.piece < kb.all; ++p) v += *reinterpret_cast<const f32x4*>(a.part + (p * rows + row) * 2 * w + col);
-    if (col < w) xva_attn::st4<F16>(a.dk + row * w + col, v, a.scale);
-    else xva_attn::st4<F16>(a.dv + row * w + col - w, v, 1.f);
+    if (col < w) {
+        const Range range = F16 ? *reinterpret_cast<const Range*>(a.range + ((int64_t)b * a.Hk + row % a.Hk) * 4) : Range{1.f, 1.f, 0.f, 1.f};
+        xva_attn::st4<F16>(a.dk + row * w + col, v, a.scale * range.down * (col < a.d ? 1.f : range.big));
+    } else xva_attn::st4<F16>(a.dv + row * w + col - w, v, 1.f);
 }
 
 // dq of 128 queries of a head, 32 to a wave, and their part of dlam
@@ -974,6 +1039,7 @@ __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typena
         return;
     }
     Lane fr(lane, 0);
+    const Range range = Range::of<F16>(a, b, hk);
     bf16x8 qf[2][2][S::KH], of[2][S::VH];
     int limit[2];
     float L[2][2], Dr[2][2];
@@ -990,6 +1056,7 @@ __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typena
         }
         Dr[0][rt] = -Dr[0][rt];
         Dr[1][rt] = Dr[0][rt] - Dr[1][rt];
+        if (F16) { Dr[0][rt] *= range.up; Dr[1][rt] *= range.up; }
 #pragma unroll
         for (int kh = 0; kh < S::VH; ++kh) of[rt][kh] = ld_edge(a.dout + b * a.gb + h * a.gh + safe * a.gt, kh * 32 + g * 8, tiles > 0 ? w : 0);
     }
@@ -1057,8 +1124,8 @@ __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typena
                             const float p1 = exp2_(s[0][u][rt][r] * a.c - L[0][rt]), p2 = exp2_(s[1][u][rt][r] * a.c - L[1][rt]);
                             const float x = dp[u][rt][r];
                             dl += p2 * x;
-                            s[0][u][rt][r] = p1 * (x - Dr[0][rt]);
-                            s[1][u][rt][r] = p2 * (x - Dr[1][rt]);
+                            s[0][u][rt][r] = p1 * (F16 ? __builtin_fmaf(x, range.up, -Dr[0][rt]) : x - Dr[0][rt]);
+                            s[1][u][rt][r] = p2 * (F16 ? __builtin_fmaf(x, range.up, -Dr[1][rt]) : x - Dr[1][rt]);
                         }
                 }
                 bf16x8 df[2][2];
@@ -1100,7 +1167,7 @@ __device__ __forceinline__ void dq_part(const Args& a, const unsigned id, typena
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int dt = 0; dt < S::DT; ++dt)
-                if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(dst + m * a.d + dt * 16 + g * 4, dq[m][rt][dt], m ? -lam * a.scale : a.scale);
+                if (dt * 16 + g * 4 < a.d) xva_attn::st4<F16>(dst + m * a.d + dt * 16 + g * 4, dq[m][rt][dt], (m ? -lam * a.scale : a.scale) * range.down);
     }
     // (the tile loop has ended with a barrier)
     XVA_LDS float* red = (XVA_LDS float*)even;
@@ -1133,7 +1200,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
     if (all <= a.qpiece) return;
     f32x4 v = ZERO4;
     for (int p = 0; p * a.qpiece < all; ++p) v += *reinterpret_cast<const f32x4*>(a.qpart + (p * rows + R) * w + col);
-    xva_attn::st4<F16>(a.dq + R * w + col, v, col < a.d ? a.scale : -a.lam32[h] * a.scale);
+    xva_attn::st4<F16>(a.dq + R * w + col, v, (col < a.d ? a.scale : -a.lam32[h] * a.scale) * (F16 ? a.range[((int64_t)b * a.Hk + h / a.share) * 4 + 1] : 1.f));
 }
 
 // dlam[h] = - sum of the head's parts, in a fixed order, rounded once to lam's type
@@ -1244,6 +1311,8 @@ int64_t query_floats(const xva_diff_attention_args* p, bool bwd) {
     const Pieces s = query_plan(p, bwd);
     return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tq * p->H * (bwd ? 2 * p->d : 4 * p->d + 4) : 0;
 }
+int64_t norm_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->H * p->Tq + (int64_t)p->B * p->Hk * p->Tk : 0; }
+int64_t range_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->Hk * 4 : 0; }
 unsigned join_grid(const Args& a) { return (unsigned)(((int64_t)a.B * a.Tq * a.H * (a.d / 2) + 255) / 256); }
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
     const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + forward_rows(D16) - 1) / forward_rows(D16)) * a.qpieces);
@@ -1259,8 +1328,13 @@ template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t 
 template <int D16, bool F16> int backward(const Args& a, void* dlam, hipStream_t st) {
     const int nqb = (a.Tq + 127) / 128;
     const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-    rowdot_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
+    const unsigned first_v = (unsigned)((rows + 15) / 16);
+    rowdot_kernel<F16><<<first_v + (F16 ? (unsigned)(((int64_t)a.B * a.Tk * a.Hk + 15) / 16) : 0), 256, 0, st>>>(a, first_v);
     XVA_LAUNCH_CHECK();
+    if (F16) {
+        range_kernel<<<(unsigned)(a.B * a.Hk), 1024, 0, st>>>(a);
+        XVA_LAUNCH_CHECK();
+    }
     const unsigned dkv = (unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64) * a.pieces);
     grad_kernel<D16, F16><<<dkv + (unsigned)(a.B * a.H * nqb * a.qpieces), 256, 0, st>>>(a, dkv);
     XVA_LAUNCH_CHECK();
@@ -1279,7 +1353,7 @@ template <int D16, bool F16> int backward(const Args& a, void* dlam, hipStream_t
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
     const Few f = few_plan(p);
     if (!bwd) return (f.on ? few_floats(p, f) : query_floats(p, false)) * 4;
-    return (dkv_floats(p) + query_floats(p, true) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces + p->H) * 4;
+    return (dkv_floats(p) + query_floats(p, true) + range_floats(p) + norm_floats(p) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces + p->H) * 4;
 }
 }   // namespace
 
@@ -1327,7 +1401,9 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     a.pieces = s.pieces; a.piece = s.piece; a.qpieces = sq.pieces; a.qpiece = sq.piece;
     a.part = (float*)ws;
     a.qpart = a.part + dkv_floats(p);
-    a.D = a.qpart + query_floats(p, true);
+    a.range = a.qpart + query_floats(p, true);
+    a.norms = a.range + range_floats(p);
+    a.D = a.norms + norm_floats(p);
     a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
     a.lam32 = a.dlam_part + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * a.qpieces;
 #define CALL(D16, F16) backward<D16, F16>(a, p->dlam, (hipStream_t)stream)
