@@ -253,3 +253,12 @@ def test_turns_to_half_a_unit(kw, rd):
                 ramp = min(max(D(i - low) / D(max(high - low, 1e-3)), D(0)), D(1))
                 f = f * (1 - ramp) + f / factor * ramp
             assert abs(D(t % 2 ** 64) - f / (2 * pi) * 2 ** 64) <= D(1) / 2 + D(10) ** -9, i
+
+
+@pytest.mark.parametrize("T", [1 << 30, (1 << 31) - 300, (1 << 31) - 1])
+@pytest.mark.parametrize("channels", [1, 32])
+def test_group_norm_refuses_rows_that_int32_cannot_step_over(T, channels):
+    a = GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=1, T=T, C=channels, G=1, act=0, eps=1e-5)
+    for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
+        assert entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd) == -1
+        assert call(C.byref(a), None, 0, None) == -1 and "T %d" % T in _lib.lib.xva_last_error().decode()

@@ -824,7 +824,7 @@ int allowed(const xva_group_norm_args* p, bool bwd) {
 int check(const xva_group_norm_args* p, const char* who) {
     XVA_CHECK_ARG(p, "%s: null argument", who);
     XVA_CHECK_ARG(p->dtype >= 0 && p->dtype <= 2, "%s: dtype %d", who, p->dtype);
-    XVA_CHECK_ARG(p->B >= 0 && p->B < (1 << 30) && p->T >= 0 && p->C >= 1 && p->C <= 65536 && p->G >= 1 && p->C % p->G == 0, "%s: B %d T %d C %d in %d groups", who, p->B, p->T, p->C, p->G);
+    XVA_CHECK_ARG(p->B >= 0 && p->B < (1 << 30) && p->T >= 0 && p->T < (1 << 30) && p->C >= 1 && p->C <= 65536 && p->G >= 1 && p->C % p->G == 0, "%s: B %d T %d C %d in %d groups", who, p->B, p->T, p->C, p->G);
     XVA_CHECK_ARG(p->act >= NONE && p->act <= GELU, "%s: activation %d", who, p->act);
     XVA_CHECK_ARG(p->eps >= 0.f, "%s: eps %g", who, p->eps);
     XVA_CHECK_ARG(p->B == 0 || p->T == 0 || (p->x && p->out && p->mean && p->rstd), "%s: null argument", who);
@@ -969,7 +969,7 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
 }   // namespace
 
 extern "C" int64_t xva_group_norm_workspace_bytes(const xva_group_norm_args* p, int backward_pass) {
-    if (!p || p->G < 1 || p->C < 1 || p->C % p->G || p->B < 0 || p->T < 0) return -1;
+    if (!p || p->G < 1 || p->C < 1 || p->C % p->G || p->B < 0 || p->T < 0 || p->T >= (1 << 30)) return -1;
     return workspace(p, backward_pass != 0);
 }
 extern "C" int xva_group_norm_act_fwd(const xva_group_norm_args* p, void* ws, int64_t ws_bytes, void* stream) {
