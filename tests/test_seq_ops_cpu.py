@@ -262,3 +262,13 @@ def test_group_norm_refuses_rows_that_int32_cannot_step_over(T, channels):
     for bwd, call in ((0, entry("xva_group_norm_act_fwd")), (1, entry("xva_group_norm_act_bwd"))):
         assert entry("xva_group_norm_workspace_bytes", i64)(C.byref(a), bwd) == -1
         assert call(C.byref(a), None, 0, None) == -1 and "T %d" % T in _lib.lib.xva_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype,channels", [(0, 1 << 29), (1, 1 << 30), (2, (1 << 31) - 1)])
+def test_recurrence_refuses_rows_of_two_gigabytes(dtype, channels):
+    """Offsets within a row are 32 bits (h null: a call that gets past this is refused for that)."""
+    a = RecurrenceArgs(x=A, gate=A, h=None, last=A, dtype=dtype, B=1, T=1, C=channels)
+    assert entry("xva_recurrence_fwd")(C.byref(a), None, 0, None) == -1
+    assert "2^31 bytes" in _lib.lib.xva_last_error().decode()
+    assert entry("xva_recurrence_fwd")(C.byref(RecurrenceArgs(x=A, gate=A, h=None, last=A, dtype=dtype, B=1, T=1, C=channels // 2)), None, 0, None) == -1
+    assert "null" in _lib.lib.xva_last_error().decode()

@@ -525,6 +525,7 @@ int run(const xva_recurrence_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     XVA_CHECK_ARG(p, "%s: null argument", who);
     XVA_CHECK_ARG(p->dtype >= 0 && p->dtype <= 2, "%s: dtype %d", who, p->dtype);
     XVA_CHECK_ARG(p->B >= 0 && p->T >= 0 && p->T < (1 << 30) && p->C >= 1 && (int64_t)p->B * p->C < (1ll << 31), "%s: B %d T %d C %d", who, p->B, p->T, p->C);
+    XVA_CHECK_ARG((int64_t)p->C * xva_seq::elem_size(p->dtype) < (1ll << 31), "%s: C %d, rows are under 2^31 bytes", who, p->C);        // (32-bit offsets in a row)
     if (p->B == 0) return XVA_OK;
     XVA_CHECK_ARG(p->T == 0 || (p->x && p->gate), "%s: null argument", who);
     XVA_CHECK_ARG(bwd ? p->states && (p->T == 0 || (p->dh && p->dx && p->dgate)) : p->last && (p->T == 0 || p->h), "%s: null argument", who);
