@@ -143,3 +143,67 @@ def test_a_tangent_of_the_incoming_gradient_is_refused(op):
     with fwd.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(y, leaves[0], fwd.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("dt,tol", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+def test_a_captured_step_of_a_serving_loop(dt, tol):
+    """One frame of each stream: rotary positions in place, the frame's key and value into the cache, attention over it, each head's norm, the recurrence's step with its
+    state carried on; captured once, replayed frame by frame.  Every frame against the same calls made eagerly (bit for bit, also the caches and the state), and all
+    frames against one pass over the whole sequence, which takes other kernels: each of its five tensors is rounded the same way from sums that differ in fp32 alone,
+    so a value differs where a rounding flips, by one step 2 u of itself; 10 u of the norm bounds five of them."""
+    from xva_trainer_amd import seq_ops as S
+    torch.manual_seed(12)
+    B, T, H, Hk, d, C = 3, 40, 4, 2, 32, 64
+    plan = S.RotaryPlan(d)
+    q, k, v = (torch.randn(B, T, n, w, device="cuda").to(dt) for n, w in ((2 * H, d), (2 * Hk, d), (Hk, 2 * d)))
+    lam, weight = torch.rand(H, device="cuda"), 1 + 0.1 * torch.randn(H * 2 * d, device="cuda")
+    mix = (torch.randn(2 * C, H * 2 * d, device="cuda") * (H * 2 * d) ** -0.5).to(dt)
+
+    class Stream:
+        def __init__(self):
+            z = lambda *s: torch.zeros(*s, device="cuda", dtype=dt)
+            self.q, self.k, self.v, self.pos = z(B, 1, 2 * H, d), z(B, 1, 2 * Hk, d), z(B, 1, Hk, 2 * d), torch.zeros(1, device="cuda", dtype=torch.int64)
+            self.keys, self.values, self.lens = z(B, T, Hk, 2, d), z(B, T, Hk, 2 * d), torch.zeros(B, device="cuda", dtype=torch.int32)
+            self.state, self.y = torch.zeros(B, C, device="cuda"), z(B, 1, C)
+
+        def feed(self, t):
+            self.q.copy_(q[:, t:t + 1]), self.k.copy_(k[:, t:t + 1]), self.v.copy_(v[:, t:t + 1]), self.pos.fill_(t)
+
+        def step(self):
+            S.rotary(plan, self.q, self.k, positions=self.pos, inplace=True)
+            self.keys.index_copy_(1, self.pos, self.k.unflatten(2, (Hk, 2)))
+            self.values.index_copy_(1, self.pos, self.v)
+            self.lens.copy_((self.pos + 1).expand(B))
+            o = S.differential_attention(self.q.unflatten(2, (H, 2)), self.keys, self.values, lam, causal=True, k_lens=self.lens)
+            o = S.group_norm_act(o.view(B, H * 2 * d), H, weight)
+            u, gate = (o @ mix.T).view(B, 1, 2 * C).chunk(2, -1)
+            h, last = S.gated_recurrence(u, gate, self.state)
+            self.state.copy_(last), self.y.copy_(h)
+
+    with torch.no_grad():
+        warm, eager, captured = Stream(), Stream(), Stream()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            warm.feed(0), warm.step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.step()
+        ys = []
+        for t in range(T):
+            captured.feed(t), eager.feed(t)
+            graph.replay()
+            eager.step()
+            torch.cuda.synchronize()
+            for name in ("q", "k", "keys", "values", "lens", "state", "y"):
+                assert torch.equal(getattr(captured, name), getattr(eager, name)), (t, name)
+            ys.append(captured.y.clone())
+        qr, kr = S.rotary(plan, q, k)
+        o = S.differential_attention(qr.unflatten(2, (H, 2)), kr.unflatten(2, (Hk, 2)), v, lam, causal=True)
+        o = S.group_norm_act(o.reshape(B * T, H * 2 * d), H, weight)
+        u, gate = (o @ mix.T).view(B, T, 2 * C).chunk(2, -1)
+        whole, last = S.gated_recurrence(u, gate)
+        ys = torch.cat(ys, 1)
+        for a, b in ((ys, whole), (captured.state, last)):
+            assert (a.double() - b.double()).norm().item() < 10 * tol * b.double().norm().item()
