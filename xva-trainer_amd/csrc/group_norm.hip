@@ -40,7 +40,6 @@ struct Args {
     int B, T, C, G, n, act;
     float eps, slope;
     int rows_per_chunk, chunks;
-    int wide_w;                                            // w and bias at addresses that vectors of them need
 };
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
@@ -75,16 +74,20 @@ template <int V> __device__ __forceinline__ void slopes(float (&z)[V], int act, 
         default: each<V>(z, [](float) { return 1.f; });
     }
 }
-// V values of a weight vector, `none` where there is none.  A thread reads its weights once, so their address is no reason to take x in narrower vectors: one that
-// rules vectors out (a slice of a flat parameter buffer) is read value by value.
-template <int V> __device__ __forceinline__ void load_w(const Args& a, const float* w, int c, float none, float (&f)[V]) {
-    if (!w) {
+// V values of a weight vector, `none` where there is none.  Vectors of 32-bit values are loaded from any address of one (a slice of a flat parameter buffer), so the
+// weights' address has no say in how x is read.
+template <int V> __device__ __forceinline__ void load_w(const float* w, int c, float none, float (&f)[V]) {
+    typedef float Any __attribute__((ext_vector_type(V < 4 ? V : 4), aligned(4)));
+    if (w) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const Any v = *reinterpret_cast<const Any*>(w + c + e);
+#pragma unroll
+            for (int i = 0; i < (V < 4 ? V : 4); ++i) f[e + i] = v[i];
+        }
+    } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = none;
-    } else if (a.wide_w) load_v<0, V>(w, c, f);
-    else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = w[c + e];
     }
 }
 __device__ __forceinline__ int live_rows(const Args& a, int b) {
@@ -110,8 +113,8 @@ __global__ __launch_bounds__(256) void slab_kernel(Args a, SlabPlan s) {
         const int j = k * s.lpg + lane;
         row[k] = j < vecs ? j / nv : a.T;                  // a.T: no such row
         ch[k] = min(g, a.G - 1) * a.n + (j < vecs ? (j % nv) * V : 0);
-        load_w<V>(a, a.w, ch[k], 1.f, w[k]);
-        load_w<V>(a, a.bias, ch[k], 0.f, bias[k]);
+        load_w<V>(a.w, ch[k], 1.f, w[k]);
+        load_w<V>(a.bias, ch[k], 0.f, bias[k]);
 #pragma unroll
         for (int e = 0; e < V; ++e) sw[k][e] = sb[k][e] = 0.f;
     }
@@ -273,8 +276,8 @@ __global__ __launch_bounds__(512) void whole_kernel(Args a, WholePlan q) {
         }
     }
     float w[V], bias[V];
-    load_w<V>(a, a.w, on ? c : 0, 1.f, w);
-    load_w<V>(a, a.bias, on ? c : 0, 0.f, bias);
+    load_w<V>(a.w, on ? c : 0, 1.f, w);
+    load_w<V>(a.bias, on ? c : 0, 0.f, bias);
     if constexpr (!BWD) {
         float* sums = lds + q.threads;
         float s = 0.f;
@@ -533,8 +536,8 @@ __global__ __launch_bounds__(NT) void tile_apply_kernel(Args a) {
     __syncthreads();
     if (!t.on) return;
     float mu[V], w[V], bias[V];
-    load_w<V>(a, a.w, t.v * V, 1.f, w);
-    load_w<V>(a, a.bias, t.v * V, 0.f, bias);
+    load_w<V>(a.w, t.v * V, 1.f, w);
+    load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int c = t.v * V + e, g = c / a.n;
@@ -583,8 +586,8 @@ __global__ __launch_bounds__(NT) void tile_dsum_kernel(Args a) {
     for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0.f;
     if (t.on) {
         float mu[V], rs[V], w[V], bias[V];
-        load_w<V>(a, a.w, t.v * V, 1.f, w);
-        load_w<V>(a, a.bias, t.v * V, 0.f, bias);
+        load_w<V>(a.w, t.v * V, 1.f, w);
+        load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const int c = t.v * V + e, g = c / a.n;
@@ -691,8 +694,8 @@ __global__ __launch_bounds__(NT) void tile_dx_kernel(Args a) {
     __syncthreads();
     if (!t.on) return;
     float mu[V], rs[V], w[V], bias[V], k1[V], k2[V];
-    load_w<V>(a, a.w, t.v * V, 1.f, w);
-    load_w<V>(a, a.bias, t.v * V, 0.f, bias);
+    load_w<V>(a.w, t.v * V, 1.f, w);
+    load_w<V>(a.bias, t.v * V, 0.f, bias);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int c = t.v * V + e, g = c / a.n;
@@ -838,7 +841,6 @@ Args args_of(const xva_group_norm_args* p, const Plan& q) {
     a.xb = p->x_stride[0]; a.xt = p->x_stride[1]; a.ob = p->out_stride[0]; a.ot = p->out_stride[1]; a.db_ = p->dy_stride[0]; a.dt_ = p->dy_stride[1];
     a.B = p->B; a.T = p->T; a.C = p->C; a.G = p->G; a.n = p->C / p->G; a.act = p->act; a.eps = p->eps; a.slope = p->slope;
     a.rows_per_chunk = q.rows_per_chunk; a.chunks = q.chunks;
-    a.wide_w = ((uintptr_t)p->weight | (uintptr_t)p->bias) % (q.v < 4 ? 4 * q.v : 16) == 0;
     return a;
 }
 
