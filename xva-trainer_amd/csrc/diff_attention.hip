@@ -41,7 +41,8 @@ struct Args {
     int lam_type;
     float* lam32;                                 // backward: the same in fp32, for the scalar unit (rowdot_kernel leaves it)
     float *lse, *D, *dlam_part;
-    float *norms;                                 // fp16 backward: squared norms of dO's rows (B, H, Tq), then of v's (B, Hk, Tk)
+    float *norms;                                 // fp16 backward: largest squared norm of each 16 rows of dO (B, H, Tq / 16), then of v (B, Hk, Tk / 16)
+    float *start;                                 // fp16 backward: lse and D as dkv takes them (range_kernel)
     float *range;                                 // fp16 backward: of each (item, key head) the factors that keep dS in the type's range (see range_kernel)
     const int32_t *ql, *kl;
     int64_t qb, qt, qh, qm, kb, kt, kh, km, vb, vt, vh, ob, ot, oh, gb, gt, gh;
@@ -709,93 +710,126 @@ __global__ __launch_bounds__(256) void few_join_kernel(Args a, const float* __re
 }
 
 // ================================================================================ backward ====
-// D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns.  fp16: the squared norms of dO's rows beside it, and of v's by the workgroups behind those (`first_v`)
+// D_m[row] = dO . O_m; 16 lanes to a row of 2 d <= 128 columns.  fp16: a workgroup's rows are 16 of one head, and it leaves the largest squared norm of dO among them; the
+// workgroups from `first_v` on leave that of 16 of v's rows.
 template <bool F16>
 __global__ __launch_bounds__(256) void rowdot_kernel(Args a, unsigned first_v) {
-    const int c = (threadIdx.x & 15) * 8, w = 2 * a.d;
-    auto join = [](float v) { v += __shfl_xor(v, 1, 64); v += __shfl_xor(v, 2, 64); v += __shfl_xor(v, 4, 64); return v + __shfl_xor(v, 8, 64); };
-    if (F16 && blockIdx.x >= first_v) {
-        const int64_t id = (int64_t)(blockIdx.x - first_v) * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tk * a.Hk, bt = id / a.Hk;
-        const int hk = (int)(id - bt * a.Hk), b = (int)(bt / a.Tk), t = (int)(bt - (int64_t)b * a.Tk);
-        float n = 0.f;
-        if (id < rows && c < w && t < len_of(a.kl, b, a.Tk)) {
-            const uint4 vr = *reinterpret_cast<const uint4*>(a.v + b * a.vb + t * a.vt + hk * a.vh + c);
-            const uint32_t vw[4] = {vr.x, vr.y, vr.z, vr.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { float v0, v1; unpack2<F16>(vw[e], v0, v1); n += v0 * v0 + v1 * v1; }
-        }
-        n = join(n);
-        if (id < rows && (threadIdx.x & 15) == 0) a.norms[(int64_t)a.B * a.H * a.Tq + ((int64_t)b * a.Hk + hk) * a.Tk + t] = n;
-        return;
+    __shared__ float top[4];
+    const int slot = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8, w = 2 * a.d;
+    const bool keys = F16 && blockIdx.x >= first_v;
+    int64_t id;                                    // of the row in (B, Tq, H)
+    int b, h, t;
+    bool row;
+    if constexpr (F16) {
+        const int T = keys ? a.Tk : a.Tq, heads = keys ? a.Hk : a.H, blocks = (T + 15) / 16;
+        const unsigned at = blockIdx.x - (keys ? first_v : 0), bh = at / (unsigned)blocks;
+        b = bh / (unsigned)heads; h = bh - b * heads; t = (at - bh * blocks) * 16 + slot;
+        row = t < T;
+        id = ((int64_t)b * T + t) * heads + h;
+    } else {
+        id = (int64_t)blockIdx.x * 16 + slot;
+        row = id < (int64_t)a.B * a.Tq * a.H;
+        const int64_t bt = id / a.H;
+        h = (int)(id - bt * a.H); b = (int)(bt / a.Tq); t = (int)(bt - (int64_t)b * a.Tq);
     }
-    const int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (int64_t)a.B * a.Tq * a.H;
+    const int64_t rows = (int64_t)a.B * a.Tq * a.H;
     float s[2] = {0.f, 0.f}, n = 0.f;
-    const int64_t bt = id / a.H;
-    const int h = (int)(id - bt * a.H), b = (int)(bt / a.Tq), t = (int)(bt - (int64_t)b * a.Tq);
-    if (id < rows && c < w && t < len_of(a.ql, b, a.Tq)) {
-        const uint4 gr = *reinterpret_cast<const uint4*>(a.dout + b * a.gb + t * a.gt + h * a.gh + c);
+    if (row && c < w && t < (keys ? len_of(a.kl, b, a.Tk) : len_of(a.ql, b, a.Tq))) {
+        const uint4 gr = *reinterpret_cast<const uint4*>((keys ? a.v + b * a.vb + t * a.vt + h * a.vh : a.dout + b * a.gb + t * a.gt + h * a.gh) + c);
         const uint32_t gw[4] = {gr.x, gr.y, gr.z, gr.w};
+        if (F16) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const uint4 od = *reinterpret_cast<const uint4*>(a.maps + (m * rows + id) * w + c);
-            const uint32_t ow[4] = {od.x, od.y, od.z, od.w};
+            for (int e = 0; e < 4; ++e) { float g0, g1; unpack2<F16>(gw[e], g0, g1); n += g0 * g0 + g1 * g1; }
+        }
+        if (!keys) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float g0, g1, o0, o1;
-                unpack2<F16>(gw[e], g0, g1); unpack2<F16>(ow[e], o0, o1);
-                s[m] += g0 * o0 + g1 * o1;
-                if (F16 && m == 0) n += g0 * g0 + g1 * g1;
+            for (int m = 0; m < 2; ++m) {
+                const uint4 od = *reinterpret_cast<const uint4*>(a.maps + (m * rows + id) * w + c);
+                const uint32_t ow[4] = {od.x, od.y, od.z, od.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float g0, g1, o0, o1;
+                    unpack2<F16>(gw[e], g0, g1); unpack2<F16>(ow[e], o0, o1);
+                    s[m] += g0 * o0 + g1 * o1;
+                }
             }
         }
     }
+    auto join = [](float v) { v += __shfl_xor(v, 1, 64); v += __shfl_xor(v, 2, 64); v += __shfl_xor(v, 4, 64); return v + __shfl_xor(v, 8, 64); };
+    if (!keys) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) s[m] = join(s[m]);
-    if (F16) {
-        n = join(n);
-        if (id < rows && (threadIdx.x & 15) == 0) a.norms[((int64_t)b * a.H + h) * a.Tq + t] = n;
+        for (int m = 0; m < 2; ++m) s[m] = join(s[m]);
+        if (row && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
+        const int64_t first = (int64_t)blockIdx.x * 16 + slot;
+        if (first < a.H && (threadIdx.x & 15) == 0) a.lam32[first] = lam_of(a, (int)first);
     }
-    if (id < rows && (threadIdx.x & 15) < 2) a.D[(((int64_t)(threadIdx.x & 1) * a.B + b) * a.H + h) * a.Tq + t] = threadIdx.x & 1 ? s[0] - s[1] : -s[0];
-    if (id < a.H && (threadIdx.x & 15) == 0) a.lam32[id] = lam_of(a, (int)id);
+    if constexpr (F16) {
+        n = join(n);
+        n = fmaxf(n, __shfl_xor(n, 16, 64));
+        n = fmaxf(n, __shfl_xor(n, 32, 64));
+        if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = n;
+        __syncthreads();
+        if (threadIdx.x == 0) a.norms[blockIdx.x] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    }
 }
 
-// fp16 holds 2^-14 .. 2^16 in full: dS = P (dP - D) of a loss that is a mean over many values, or lam times it, lies below that and would be lost.  So dS is made
-// 2^up times as large, |dS| <= |dP - D| <= 2 max |dO_i| max |v_j| (norms over the 2 d columns) coming to at most 2^15, and dS_2 in dk takes lam / 2^el instead of
-// lam, 2^el >= |lam|; both are powers of two, undone in fp32 where sums are rounded.  One set of factors for all that adds up in a key head's dK, so an item whose
-// gradients are small beside another's keeps its own.  (860 keys, heads of 48, dO of 1e-3, lam 0.01: dk_2 off by
-// 9 % of its norm without this.  It costs 8 us of 226 on 32 x 860 frames, forward + backward: v's norms, a launch, a product for each pair in dK / dV.)
-// (2^up, 2^-up, el, 2^el).  A gradient or value that is not finite takes no factor: the results it reaches are lost as they are.
+// fp16 holds 2^-14 .. 2^16 in full: dS = P (dP - D) of a loss that is a mean over many values, or lam times it, lies below that and would be lost, and one of large
+// gradients above it.  |dS| <= |dP - D| <= 2 max |dO_i| max |v_j| (norms over the 2 d columns), so 2^U brings it to at most 2^15; 2^el >= |lam|.  All factors are powers of
+// two, undone in fp32 where sums are rounded.  One set for all that adds up in a key head's dK, so an item whose gradients are small beside another's keeps its own.
+//   dq : dS 2^U in the sum that takes D off (no product more).
+//   dkv: U > 0 in the exponents, P 2^kp, as far as P_1 - lam P_2 has room, 14 - el powers; U < 0 in v and D (2^kv).  Both are in the rows' logsumexp and D that it starts its
+//        products from (`start`), so its loop has no product more; dS_2 takes lam / 2^el instead of lam.  (A product for each pair instead: 4 - 5 % of the kernel;
+//        kp beside the exponent's factor: two constants where an instruction takes one from the scalar unit, registers spill.)
+// (860 keys, heads of 48, dO of 1e-3, lam 0.01: dk_2 off by 9 % of its norm without this.  It costs 8 us of 224, forward
+// and backward, on 32 x 860 frames: v's norms and a launch.)  A gradient or value that is not finite takes no factor: the results it reaches
+// are lost as they are.
 struct Range {
-    float up, down, el, big;
+    float up, down;                               // 2^U, 2^-U
+    float el, big, shrink;                        // el, 2^el, 2^kv
+    float undo_k, undo_v, unused;                 // 2^-(kp + kv), 2^-kp
     template <bool F16> static __device__ __forceinline__ Range of(const Args& a, int b, int hk) {
-        if constexpr (!F16) return {1.f, 1.f, 0.f, 1.f};
+        if constexpr (!F16) return {1.f, 1.f, 0.f, 1.f, 1.f, 1.f, 1.f, 0.f};
         else {
-            const int at = (b * a.Hk + hk) * 4;
-            return {uniform(a.range, at), uniform(a.range, at + 1), uniform(a.range, at + 2), uniform(a.range, at + 3)};
+            const int at = (b * a.Hk + hk) * 8;
+            auto e = [&](int i) { return uniform(a.range, at + i); };
+            return {e(0), e(1), e(2), e(3), e(4), e(5), e(6), 0.f};
         }
     }
 };
-__global__ __launch_bounds__(1024) void range_kernel(Args a) {
-    __shared__ float sh[16];
-    const int b = blockIdx.x / a.Hk, hk = blockIdx.x - b * a.Hk;
-    const float* g = a.norms + ((int64_t)b * a.H + hk * a.share) * a.Tq;
-    const float* v = a.norms + (int64_t)a.B * a.H * a.Tq + (int64_t)blockIdx.x * a.Tk;
-    const int64_t ng = (int64_t)a.share * a.Tq;
-    float mg = 0.f, mv = 0.f;
-#pragma unroll 4
-    for (int64_t e = threadIdx.x; e < ng; e += 1024) mg = fmaxf(mg, g[e]);
-#pragma unroll 4
-    for (int e = threadIdx.x; e < a.Tk; e += 1024) mv = fmaxf(mv, v[e]);
-    mg = xva_block_max(mg, sh);
-    mv = xva_block_max(mv, sh);
-    if (threadIdx.x != 0) return;
+// The range of an (item, key head), which every workgroup finds for itself from the few norms there are, and what dkv's products start from: (4, B, H, Tq), the
+// logsumexps of both maps, then D, with the range's factors.  A workgroup: 256 rows of a head, under way while it looks for the norms' maxima.
+__global__ __launch_bounds__(256) void range_kernel(Args a) {
+    __shared__ float top[3][4];
+    const int parts = (a.Tq + 255) / 256, bh = blockIdx.x / parts, part = blockIdx.x - bh * parts, b = bh / a.H, h = bh - b * a.H, hk = h / a.share;
+    const int64_t rows = (int64_t)a.B * a.H * a.Tq, at = (int64_t)bh * a.Tq + part * 256 + threadIdx.x;
+    const bool row = part * 256 + (int)threadIdx.x < a.Tq;
+    float from[4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) { from[m] = row ? a.lse[m * rows + at] : 0.f; from[2 + m] = row ? a.D[m * rows + at] : 0.f; }
+    const int nq = (a.Tq + 15) / 16, nk = (a.Tk + 15) / 16;
+    const float* g = a.norms + ((int64_t)b * a.H + hk * a.share) * nq;
+    const float* v = a.norms + (int64_t)a.B * a.H * nq + ((int64_t)b * a.Hk + hk) * nk;
+    float mg = 0.f, mv = 0.f, lam = 0.f;
+    for (int e = threadIdx.x; e < a.share * nq; e += 256) mg = fmaxf(mg, g[e]);
+    for (int e = threadIdx.x; e < nk; e += 256) mv = fmaxf(mv, v[e]);
+    for (int e = threadIdx.x; e < a.share; e += 256) lam = fmaxf(lam, fabsf(lam_of(a, hk * a.share + e)));
+    mg = xva_wave_max(mg); mv = xva_wave_max(mv); lam = xva_wave_max(lam);
+    if ((threadIdx.x & 63) == 0) { const int w = threadIdx.x >> 6; top[0][w] = mg; top[1][w] = mv; top[2][w] = lam; }
+    __syncthreads();
+    auto all = [&](int i) { return fmaxf(fmaxf(top[i][0], top[i][1]), fmaxf(top[i][2], top[i][3])); };
+    mg = all(0); mv = all(1); lam = all(2);
     const float bound = 2.002f * sqrtf(mg) * sqrtf(mv);             // (2 and some roundings)
-    float lam = 0.f;
-    for (int e = 0; e < a.share; ++e) lam = fmaxf(lam, fabsf(lam_of(a, hk * a.share + e)));
     int up = 0, el = 0;
     if (bound > 0.f && bound < INFINITY) { frexpf(bound, &up); up = 15 - up; }
     if (lam > 0.f && lam < INFINITY) { frexpf(lam, &el); el = max(el, -100); }
-    float* to = a.range + (int64_t)blockIdx.x * 4;
-    to[0] = ldexpf(1.f, up); to[1] = ldexpf(1.f, -up); to[2] = (float)el; to[3] = ldexpf(1.f, el);
+    const int kp = min(max(up, 0), 14 - max(el, 0)), kv = min(up, 0);
+    if (threadIdx.x == 0 && part == 0 && h == hk * a.share)
+        *reinterpret_cast<Range*>(a.range + ((int64_t)b * a.Hk + hk) * 8) = {ldexpf(1.f, up), ldexpf(1.f, -up), (float)el, ldexpf(1.f, el), ldexpf(1.f, kv), ldexpf(1.f, -kp - kv),
+                                                                            ldexpf(1.f, -kp), 0.f};
+    const float more = (float)kp / a.c, shrink = ldexpf(1.f, kv);
+    if (!row) return;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) { a.start[m * rows + at] = from[m] + more; a.start[(2 + m) * rows + at] = from[2 + m] * shrink; }
 }
 
 // A key block's 64-query tiles: of each query head that shares the keys, `per_head` from tile `t0` on
@@ -848,6 +882,17 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
 #pragma unroll
         for (int kh = 0; kh < S::VH; ++kh) vf[kt][kh] = ld_edge(a.v + b * a.vb + hk * a.vh + key * a.vt, kh * 32 + g * 8, any ? w : 0);
     }
+    if (F16 && range.shrink != 1.f) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int kh = 0; kh < S::VH; ++kh) {
+                u32x4 e = __builtin_bit_cast(u32x4, vf[kt][kh]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { float v0, v1; unpack2<F16>(e[i], v0, v1); e[i] = pack2<F16>(v0 * range.shrink, v1 * range.shrink); }
+                vf[kt][kh] = __builtin_bit_cast(bf16x8, e);
+            }
+    }
     XVA_LDS bf16x8* away = (XVA_LDS bf16x8*)away_raw + wave * AWAY * 64 + lane;
 #pragma unroll
     for (int e = 0; e < AWAY; ++e) away[e * 64] = vf[1][S::VH - 1 - e];
@@ -867,7 +912,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
         const Src<NI> src(lane_, wave, a.d, a.qm);
         src.fetch_qk(a.q + b * a.qb + h * a.qh + row0 * a.qt, a.qt, a.qm, a.d, ql - row0, to, wave);
         src.fetch_v(a.dout + b * a.gb + h * a.gh + row0 * a.gt, a.gt, a.d, ql - row0, to + NI * TILE, wave);
-        const float* from = (wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + row0;
+        const float* from = (F16 ? a.start + (int64_t)(wave & 2) * a.B * a.H * a.Tq : wave < 2 ? a.lse : a.D) + (((int64_t)(wave & 1) * a.B + b) * a.H + h) * a.Tq + row0;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)from, 0, (uint32_t)min(ql - row0, 64) * 4u, 0x00027000),
                                                  (XVA_LDS void*)(to + STAT + wave * 256), 4, min(lane_, ql - row0 - 1) * 4, 0, 0, 0);
     };
@@ -888,7 +933,7 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 // -D_1 under dP, lse under the scores
-                const XVA_LDS uint8_t* at = smem + STAT + t * 128 + g * 16 + u * 64;
+                const XVA_LDS uint8_t* at = smem + STAT + t * 128 + (F16 && D16 == 4 ? again(lane) >> 4 : g) * 16 + u * 64;      // (kept, it would be spilled there)
                 const f32x4 nD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 512);
                 f32x4 s[2][2], dp[2];                         // [map][key tile], [row g * 4 + r][key lane & 15]
 #pragma unroll
@@ -919,13 +964,13 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
                             s[1][kt][r] = ok ? s[1][kt][r] : -INFINITY;
                         }
                 }
-                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768) * (minus * range.up);
+                const f32x4 dD = *reinterpret_cast<const XVA_LDS f32x4*>(at + 768) * minus;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         // (|lam| in the exponent, its sign in the sums: no product more than without it)
-                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = exp2_(__builtin_fmaf(s[1][kt][r], a.c, loglam)), x = F16 ? dp[kt][r] * range.up : dp[kt][r];
+                        const float p1 = exp2_(s[0][kt][r] * a.c), p2 = exp2_(__builtin_fmaf(s[1][kt][r], a.c, loglam)), x = dp[kt][r];
                         s[0][kt][r] = p1 * x;
                         s[1][kt][r] = p2 * __builtin_fmaf(x, minus, dD[r]);
                         dp[kt][r] = __builtin_fmaf(p2, minus_big, p1);
@@ -991,10 +1036,10 @@ __device__ __forceinline__ void dkv_part(const Args& a, const unsigned id, typen
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int dt = 0; dt < S::DT; ++dt)
-                    if (dt * 16 + ge * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + ge * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale * range.down * (m ? range.big : 1.f));
+                    if (dt * 16 + ge * 4 < a.d) xva_attn::st4<F16>(a.dk + (row * 2 + m) * a.d + dt * 16 + ge * 4, dk[m][kt][dt] + xch[(m * S::DT + dt) * 64], a.scale * range.undo_k * (m ? range.big : 1.f));
 #pragma unroll
             for (int dt = 0; dt < S::VT; ++dt)
-                if (dt * 16 + ge * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + ge * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], 1.f);
+                if (dt * 16 + ge * 4 < w) xva_attn::st4<F16>(a.dv + row * w + dt * 16 + ge * 4, dv[kt][dt] + xch[(2 * S::DT + dt) * 64], range.undo_v);
         }
         __syncthreads();
     }
@@ -1011,10 +1056,9 @@ __global__ __launch_bounds__(256) void dkv_join_kernel(Args a) {
     if (kb.all <= a.piece) return;
     f32x4 v = ZERO4;
     for (int p = 0; p * a.piece < kb.all; ++p) v += *reinterpret_cast<const f32x4*>(a.part + (p * rows + row) * 2 * w + col);
-    if (col < w) {
-        const Range range = F16 ? *reinterpret_cast<const Range*>(a.range + ((int64_t)b * a.Hk + row % a.Hk) * 4) : Range{1.f, 1.f, 0.f, 1.f};
-        xva_attn::st4<F16>(a.dk + row * w + col, v, a.scale * range.down * (col < a.d ? 1.f : range.big));
-    } else xva_attn::st4<F16>(a.dv + row * w + col - w, v, 1.f);
+    const float* range = a.range + ((int64_t)b * a.Hk + row % a.Hk) * 8;
+    if (col < w) xva_attn::st4<F16>(a.dk + row * w + col, v, F16 ? a.scale * range[5] * (col < a.d ? 1.f : range[3]) : a.scale);
+    else xva_attn::st4<F16>(a.dv + row * w + col - w, v, F16 ? range[6] : 1.f);
 }
 
 // dq of 128 queries of a head, 32 to a wave, and their part of dlam
@@ -1200,7 +1244,7 @@ __global__ __launch_bounds__(256) void dq_join_kernel(Args a) {
     if (all <= a.qpiece) return;
     f32x4 v = ZERO4;
     for (int p = 0; p * a.qpiece < all; ++p) v += *reinterpret_cast<const f32x4*>(a.qpart + (p * rows + R) * w + col);
-    xva_attn::st4<F16>(a.dq + R * w + col, v, (col < a.d ? a.scale : -a.lam32[h] * a.scale) * (F16 ? a.range[((int64_t)b * a.Hk + h / a.share) * 4 + 1] : 1.f));
+    xva_attn::st4<F16>(a.dq + R * w + col, v, (col < a.d ? a.scale : -a.lam32[h] * a.scale) * (F16 ? a.range[((int64_t)b * a.Hk + h / a.share) * 8 + 1] : 1.f));
 }
 
 // dlam[h] = - sum of the head's parts, in a fixed order, rounded once to lam's type
@@ -1311,8 +1355,9 @@ int64_t query_floats(const xva_diff_attention_args* p, bool bwd) {
     const Pieces s = query_plan(p, bwd);
     return s.pieces > 1 ? (int64_t)s.pieces * p->B * p->Tq * p->H * (bwd ? 2 * p->d : 4 * p->d + 4) : 0;
 }
-int64_t norm_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->H * p->Tq + (int64_t)p->B * p->Hk * p->Tk : 0; }
-int64_t range_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->Hk * 4 : 0; }
+int64_t norm_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->H * ((p->Tq + 15) / 16) + (int64_t)p->B * p->Hk * ((p->Tk + 15) / 16) : 0; }
+int64_t range_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)p->B * p->Hk * 8 : 0; }
+int64_t start_floats(const xva_diff_attention_args* p) { return p->dtype == 2 ? (int64_t)4 * p->B * p->H * p->Tq : 0; }
 unsigned join_grid(const Args& a) { return (unsigned)(((int64_t)a.B * a.Tq * a.H * (a.d / 2) + 255) / 256); }
 template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t st) {
     const unsigned grid = (unsigned)(a.B * a.H * ((a.Tq + forward_rows(D16) - 1) / forward_rows(D16)) * a.qpieces);
@@ -1328,11 +1373,11 @@ template <int D16, bool F16> int forward(const Args& a, bool train, hipStream_t 
 template <int D16, bool F16> int backward(const Args& a, void* dlam, hipStream_t st) {
     const int nqb = (a.Tq + 127) / 128;
     const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-    const unsigned first_v = (unsigned)((rows + 15) / 16);
-    rowdot_kernel<F16><<<first_v + (F16 ? (unsigned)(((int64_t)a.B * a.Tk * a.Hk + 15) / 16) : 0), 256, 0, st>>>(a, first_v);
+    const unsigned first_v = F16 ? (unsigned)((int64_t)a.B * a.H * ((a.Tq + 15) / 16)) : (unsigned)((rows + 15) / 16);
+    rowdot_kernel<F16><<<first_v + (F16 ? (unsigned)((int64_t)a.B * a.Hk * ((a.Tk + 15) / 16)) : 0), 256, 0, st>>>(a, first_v);
     XVA_LAUNCH_CHECK();
     if (F16) {
-        range_kernel<<<(unsigned)(a.B * a.Hk), 1024, 0, st>>>(a);
+        range_kernel<<<(unsigned)((int64_t)a.B * a.H * ((a.Tq + 255) / 256)), 256, 0, st>>>(a);
         XVA_LAUNCH_CHECK();
     }
     const unsigned dkv = (unsigned)(a.B * a.Hk * ((a.Tk + 63) / 64) * a.pieces);
@@ -1353,7 +1398,7 @@ template <int D16, bool F16> int backward(const Args& a, void* dlam, hipStream_t
 int64_t workspace(const xva_diff_attention_args* p, bool bwd) {
     const Few f = few_plan(p);
     if (!bwd) return (f.on ? few_floats(p, f) : query_floats(p, false)) * 4;
-    return (dkv_floats(p) + query_floats(p, true) + range_floats(p) + norm_floats(p) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces + p->H) * 4;
+    return (dkv_floats(p) + query_floats(p, true) + range_floats(p) + start_floats(p) + norm_floats(p) + (int64_t)2 * p->B * p->H * p->Tq + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * query_plan(p, true).pieces + p->H) * 4;
 }
 }   // namespace
 
@@ -1402,7 +1447,8 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     a.part = (float*)ws;
     a.qpart = a.part + dkv_floats(p);
     a.range = a.qpart + query_floats(p, true);
-    a.norms = a.range + range_floats(p);
+    a.start = a.range + range_floats(p);
+    a.norms = a.start + start_floats(p);
     a.D = a.norms + norm_floats(p);
     a.dlam_part = a.D + (int64_t)2 * p->B * p->H * p->Tq;
     a.lam32 = a.dlam_part + (int64_t)p->H * p->B * ((p->Tq + 127) / 128) * a.qpieces;
