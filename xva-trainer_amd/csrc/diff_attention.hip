@@ -15,10 +15,10 @@
 //             query).  dlam is summed from fp32 P_2 o dP beside dq, not from rounded outputs.
 // Waves raise their priority over the products that follow a softmax (s_setprio): the other wave of a SIMD then does its exponentials meanwhile (8192 causal positions,
 // heads of 64: dq 463 -> 429 us, dK/dV 692 -> 673, forward 484 -> 476; over the score products as well: 481, 699, 474).
-// Reached (kernels' time, dense operations of the formulas): 8192 causal positions, 16 heads of 64 on 4 keys' 472 us forward (870 TFLOP/s), 1073 us dK / dV / dq (640);
-// matrix units 47 - 49 % busy, vector units 59 - 66 %, two waves to a SIMD.  32 x 860 ragged frames, 4 heads of 48: 81 + 155 us: 688 query blocks on 512 places, and
-// scores of 48 columns take matrix steps of 64.  32 x 150, heads of 32: 13 + 16 us.  One query on each of 16 ragged caches of up to 8192 keys, 16 heads of 64 on 4 keys':
-// 41 us (4.7 TB/s) and 7 for the join.
+// Reached (kernels' time, dense operations of the formulas): 8192 causal positions, 16 heads of 64 on 4 keys' 472 us forward (870 TFLOP/s), 1070 us dK / dV / dq (640):
+// CUs busy 86 and 93 % of the launch, while they are matrix units 47 and 46 %, vector units 59 and 56 %, two waves to a SIMD, at 2.0 GHz.  32 x 860 ragged frames, fp16,
+// 4 heads of 48: 82 + 158 us: 688 query blocks on 512 places, and scores of 48 columns take matrix steps of 64.  32 x 150, heads of 32: 13 + 16 us and 9 for the two
+// small launches, each a chain of latencies.  One query on each of 16 ragged caches of up to 8192 keys, 16 heads of 64 on 4 keys': 41 us (4.7 TB/s) and 7 for the join.
 // Roundings: P, P_1 - lam P_2 and dS to the tensors' 16-bit type as MFMA operands, which is what the matrix units take at this rate; each map's own output, to the
 // tensors' type, kept for the backward pass, whose D_m is made from it (in fp32 it would be another 2 x 4 bytes a value, written and read).  Accumulators, scores, sums,
 // maxima, logsumexp and D stay fp32.  fp16 holds dS by powers of two in its normal range (range_kernel).

@@ -6,14 +6,16 @@
 // Rows at or behind an item's length count for nothing: they are not read, and leave as zeros.
 //
 // Bound: HBM (a training pass moves 5 tensors; the tile form 8, at 5.2 TB/s: 64 x 8192 x 32 fp32, 4 groups, gelu: statistics 14 us, result 24, sums of dz 29 + 5,
-// dx 34, dw / dbias 4).  In the other forms latency: 27520 rows of 8 heads of 64 bf16: 14 + 22 + 4 us; 32 x 860 x 384 bf16, 16 groups, silu: 15 + 25 + 4 us, below
-// the host's time for the pass.  Three forms, by the size of one (item, group) slab of T x n values:
+// dx 34, dw / dbias 4).  In the other forms latency: 27520 rows of 8 heads of 64 bf16: 14 + 22 + 4 us; 32 x 860 x 384 bf16, 16 groups, silu: 15 + 25 + 4 us (256
+// workgroups whose registers leave room for one to a CU: it reads, reduces and writes one after the other), below the host's time for the pass.
+// Three forms, by the size of one (item, group) slab of T x n values:
 //   * slab: it fits the registers of (part of) one wave — each head's norm behind an attention (T = 1), short items.  A slab lies over a power of two of lanes, so
 //     every reduction is a few shuffles; x is read once.  dw / dbias stay in the lanes' registers over all the items that a workgroup passes, leave as one partial
 //     row per workgroup and are added in a fixed order.
 //   * whole: some groups of an item fit the registers of a workgroup: read once, kept packed, normalised from there; one kernel forward, one and the sum of
 //     dw / dbias over items backward.
-//   * tile: chunks of rows (all channels of a row, so loads are whole lines whatever n is): statistics of each chunk, then one pass that joins them and writes.
+//   * tile: chunks of rows (all channels of a row, so loads are whole lines whatever n is): statistics of each chunk, then one pass that joins them and writes.  x is
+//     read twice forward, x and dy twice backward.
 // Statistics are two-pass from registers and joined by the exact update of mean and squared deviations (Chan, Golub, LeVeque), so a mean that is large against the
 // deviation costs nothing.  Everything is held in fp32; sums over rows are made in a fixed order, so results repeat bit for bit.
 #include "xva_common.h"

@@ -99,7 +99,9 @@ def differential_attention(q, k, v, lam, scale=None, causal=False, q_lens=None, 
 
     q (B, Tq, H, 2, d): two queries a head; k (B, Tk, Hk, 2, d); v (B, Tk, Hk, 2 d); d a multiple of 8, 64 at most; query head h reads key head
     h // (H / Hk).  lam (H,): any float type, differentiable.  scale: d^-1/2 unless given.  q_lens / k_lens (B,): live queries and keys; causal: query i sees
-    keys j <= i + k_len - q_len (the last query sees all).  Returns (B, Tq, H, 2 d); a row that sees no key is zero.  With Tq = 1 and no gradient this is the
+    keys j <= i + k_len - q_len (the last query sees all).  Returns (B, Tq, H, 2 d); a row that sees no key is zero.  Rows
+    behind k_len and q_len are not read; a value that is not finite in a live row may reach every query of its item, also one that `causal` hides it from
+    (its weight is zero, its product is not a number).  With Tq = 1 and no gradient this is the
     step of a serving loop: k and v may be slices of a longer cache."""
     return _seq_torch.differential_attention(q, k, v, lam, scale, causal, q_lens, k_lens)
 
