@@ -272,3 +272,27 @@ def test_recurrence_refuses_rows_of_two_gigabytes(dtype, channels):
     assert "2^31 bytes" in _lib.lib.xva_last_error().decode()
     assert entry("xva_recurrence_fwd")(C.byref(RecurrenceArgs(x=A, gate=A, h=None, last=A, dtype=dtype, B=1, T=1, C=channels // 2)), None, 0, None) == -1
     assert "null" in _lib.lib.xva_last_error().decode()
+
+
+def test_launches_that_the_runtime_would_cut_are_refused():
+    """2^32 threads or more along a dimension run as that number modulo 2^32, without an error: refused before anything is launched (workspaces null, so that a call that
+    gets past the check is refused too, with another code)."""
+    said = lambda: _lib.lib.xva_last_error().decode()
+    rotary = RotaryArgs(q=A, q_out=2 * A, turns=A, dtype=1, B=1 << 14, T=1 << 14, H=1, D=2, rd=2, gain=1.0)
+    assert entry("xva_rotary")(C.byref(rotary), None) == -1 and "tokens" in said()
+    for T, B in ((1, 1 << 26), (5000, 1 << 23)):                       # a wave to an item, eight waves
+        a = RecurrenceArgs(x=A, gate=A, h=A, last=A, states=A, dh=A, dx=A, dgate=A, dtype=1, B=B, T=T, C=1)
+        assert entry("xva_recurrence_fwd")(C.byref(a), None, 0, None) == -1 and "too many items" in said()
+        assert entry("xva_recurrence_bwd")(C.byref(a), None, 0, None) == -1 and "too many items" in said()
+    for T, channels in ((600, 1), (1100, 8)):
+        a = GroupNormArgs(x=A, dy=A, out=A, mean=A, rstd=A, dtype=1, B=(1 << 24), T=T, C=channels, G=1, act=0, eps=1e-5, x_stride0=T * channels, x_stride1=channels,
+                          out_stride0=T * channels, out_stride1=channels, dy_stride0=T * channels, dy_stride1=channels)
+        assert entry("xva_group_norm_act_bwd")(C.byref(a), None, 0, None) == -1 and "items" in said()
+    fwd, bwd = entry("xva_diff_attention_fwd"), entry("xva_diff_attention_bwd")
+    one = dict(H=1, Hk=1, d=8)
+    for kw in (dict(B=1 << 24, Tq=1, Tk=1), dict(B=1 << 20, Tq=1 << 10, Tk=1), dict(B=1 << 20, Tq=1, Tk=1 << 10)):
+        assert fwd(C.byref(_diff(**one, **kw)), None, 0, None) == -1 and "too many" in said()
+    back = dict(dout=A, maps=A, lse=A, dq=A, dk=A, dv=A, dlam=A)
+    for kw in (dict(B=1 << 20, Tq=256, Tk=1), dict(B=1 << 20, Tq=1, Tk=256)):
+        assert bwd(C.byref(_diff(**one, **back, **kw)), None, 0, None) == -1 and "too many" in said()
+    assert bwd(C.byref(_diff(**one, **back, B=1 << 20, Tq=1, Tk=1)), None, 0, None) == -3

@@ -27,6 +27,7 @@
 // V and dO (2 d wide): one or two images.  Rows behind the last live one read that one, with P = 0.
 #include "attn_tile.h"
 #include "../../include/xva_hip.h"
+#include "seq_vec.h"
 
 namespace {
 using namespace xva_glds;
@@ -1279,7 +1280,7 @@ int check(const xva_diff_attention_args* p, const char* who) {
     for (int64_t e : near) XVA_CHECK_ARG(e >= 0 && e < (1 << 24), "%s: row and map strides are 0 .. 2^24 - 1", who);
     XVA_CHECK_ARG(ptrs % 16 == 0 && all % 8 == 0, "%s: addresses are 16-byte aligned and strides multiples of 8", who);
     const int64_t wgs = (int64_t)p->B * p->H * ((p->Tq + 63) / 64), kwgs = (int64_t)p->B * p->Hk * ((p->Tk + 63) / 64);
-    XVA_CHECK_ARG(wgs + kwgs < (1ll << 31), "%s: too many blocks", who);
+    XVA_CHECK_ARG(xva_seq::launchable(wgs + kwgs, 256), "%s: too many blocks", who);
     return XVA_OK;
 }
 Args args_of(const xva_diff_attention_args* p) {
@@ -1420,6 +1421,8 @@ extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws
     XVA_CHECK_ARG(p->out && (p->maps == nullptr) == (p->lse == nullptr), "xva_diff_attention_fwd: null argument");
     Args a = args_of(p);
     const Few f = few_plan(p);
+    XVA_CHECK_ARG(xva_seq::launchable((int64_t)p->B * p->Hk * f.nsplit, 256) && (f.nsplit == 1 || xva_seq::launchable((int64_t)p->B * p->H * p->Tq, 256)),
+                  "xva_diff_attention_fwd: too many blocks");
     const Pieces s = query_plan(p, false);
     a.qpieces = s.pieces; a.qpiece = s.piece; a.qpart = (float*)ws;
     const int64_t need = workspace(p, false);
@@ -1427,7 +1430,6 @@ extern "C" int xva_diff_attention_fwd(const xva_diff_attention_args* p, void* ws
         xva_set_error("xva_diff_attention_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
         return XVA_ERR_WS;
     }
-    XVA_CHECK_ARG((int64_t)p->B * p->Hk * f.nsplit < (1ll << 31) && (!f.on || (int64_t)p->B * p->H * p->Tq < (1ll << 31)), "xva_diff_attention_fwd: too many blocks");
 #define CALL(D16, F16) (f.on ? few<D16, F16>(a, f, (float*)ws, (hipStream_t)stream) : forward<D16, F16>(a, p->maps != nullptr, (hipStream_t)stream))
     XVA_DIFF_BY_SHAPE(CALL)
 #undef CALL
@@ -1436,6 +1438,8 @@ extern "C" int xva_diff_attention_bwd(const xva_diff_attention_args* p, void* ws
     XVA_TRY(check(p, "xva_diff_attention_bwd"));
     if (p->B == 0 || p->Tq == 0) return XVA_OK;
     XVA_CHECK_ARG(p->dout && p->maps && p->lse && p->dq && p->dlam && (p->Tk == 0 || (p->dk && p->dv)), "xva_diff_attention_bwd: null argument");
+    XVA_CHECK_ARG(xva_seq::launchable((int64_t)p->B * p->H * ((p->Tq + 15) / 16) + (int64_t)p->B * p->Hk * ((p->Tk + 15) / 16), 256),
+                  "xva_diff_attention_bwd: too many rows");
     if (ws_bytes < workspace(p, true) || !ws) {
         xva_set_error("xva_diff_attention_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)workspace(p, true));
         return XVA_ERR_WS;

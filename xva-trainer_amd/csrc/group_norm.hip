@@ -978,7 +978,8 @@ int run(const xva_group_norm_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     Plan q = {};
     // (the forward refuses what the backward would have to)
     XVA_CHECK_ARG((bwd || make_plan(p, allowed(p, false), true, &q)) && make_plan(p, allowed(p, bwd), bwd, &q), "%s: %d channels in %d groups: at most 2048 groups and 1024 vectors of %d channels", who, p->C, p->G, q.v);
-    XVA_CHECK_ARG(q.form == SLAB || (int64_t)p->B * (q.form == TILE ? q.chunks : q.w.blocks) < (1ll << 31) - 8, "%s: %d items of %d rows", who, p->B, p->T);
+    XVA_CHECK_ARG(q.form == SLAB || xva_seq::launchable((int64_t)p->B * (q.form == TILE ? q.chunks : q.w.blocks) + 7, q.form == TILE ? q.threads : q.w.threads),
+                  "%s: %d items of %d rows", who, p->B, p->T);
     const int64_t need = workspace(p, bwd);
     if (ws_bytes < need || (need && !ws)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)need); return XVA_ERR_WS; }
     Args a = args_of(p, q);

@@ -530,6 +530,7 @@ int run(const xva_recurrence_args* p, bool bwd, void* ws, int64_t ws_bytes, void
     XVA_CHECK_ARG(p->T == 0 || (p->x && p->gate), "%s: null argument", who);
     XVA_CHECK_ARG(bwd ? p->states && (p->T == 0 || (p->dh && p->dx && p->dgate)) : p->last && (p->T == 0 || p->h), "%s: null argument", who);
     const Plan q = make_plan(p->dtype, p->B, p->T, p->C, vec_of(p, bwd), bwd);
+    XVA_CHECK_ARG(xva_seq::launchable(((int64_t)p->B * q.cblocks + 7) / 8 * 8, q.threads), "%s: B %d T %d C %d: too many items", who, p->B, p->T, p->C);
     const int64_t need = map_floats(q, p->B, p->C) * 4;
     if (ws_bytes < need || (need && !ws)) { xva_set_error("%s: workspace of %lld bytes, %lld needed", who, (long long)ws_bytes, (long long)need); return XVA_ERR_WS; }
     Args a = {};

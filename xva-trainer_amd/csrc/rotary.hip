@@ -178,6 +178,7 @@ extern "C" int xva_rotary(const xva_rotary_args* p, void* stream) {
     if (per > LDS_PAIRS / np) per = LDS_PAIRS / np;
     if (per < 1) per = 1;
     const int64_t wgs = (tokens + per - 1) / per;
+    XVA_CHECK_ARG(xva_seq::launchable(wgs, THREADS), "xva_rotary: %lld tokens, %lld to a workgroup", (long long)tokens, (long long)per);
     a.per_wg = (int)per;
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)wgs);

@@ -56,6 +56,8 @@ template <int DT, int V> __device__ __forceinline__ void store_v(void* base, int
 }
 
 inline int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+// A launch of 2^32 threads or more along a dimension runs as one of that number modulo 2^32, and no error says so
+inline bool launchable(int64_t workgroups, int threads) { return workgroups * threads < (1ll << 32); }
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
