@@ -392,3 +392,72 @@ def test_gradients_beyond_the_type_on_the_way():
         for name, (ref, bound) in _norm_bounds(q[b:b + 1], k[b:b + 1], v[b:b + 1], lam, dout[b:b + 1], True).items():
             off = (mine[name].double() - ref).norm().item()
             assert off <= bound, "%s of item %d off by %.3g of %.3g, %.3g allowed" % (name, b, off, ref.norm().item(), bound)
+
+
+def test_empty_in_fp16():
+    from xva_trainer_amd import seq_ops as S
+    for B, Tq, Tk in ((0, 3, 3), (2, 0, 3), (2, 3, 0)):
+        q, k, v, lam, dout = _data(B, Tq, Tk, 2, 1, 16, "fp16")
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        out = S.differential_attention(*leaves)
+        assert out.shape == (B, Tq, 2, 32) and (out == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(out, leaves, dout))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_what_lies_behind_an_item_is_not_read_in_fp16(causal):
+    """The gradient's range is that of live rows; and an item whose gradient is not finite leaves the others theirs."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(4, 90, 90, 2, 1, 48, "fp16", seed=16)
+    dout = dout * 1e-3
+    kl = torch.tensor([90, 45, 0, 1], dtype=torch.int32)
+    dead = (torch.arange(90)[None] >= kl[:, None]).cuda()
+    outs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        leaves = [t.masked_fill(dead.view(4, 90, *[1] * (t.dim() - 2)), fill).requires_grad_(True) for t in (q, k, v)] + [lam.clone().requires_grad_(True)]
+        out = S.differential_attention(*leaves, causal=causal, q_lens=kl.cuda(), k_lens=kl.cuda())
+        outs.append((out.detach(),) + torch.autograd.grad(out, leaves, dout.masked_fill(dead[..., None, None], fill)))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+    for bad in (float("nan"), float("inf")):
+        g = dout.clone()
+        g[0, 3, 1, 5] = bad
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        got = torch.autograd.grad(S.differential_attention(*leaves, lam, causal=causal), leaves, g)
+        want = torch.autograd.grad(S.differential_attention(*leaves, lam, causal=causal), leaves, dout)
+        assert all(torch.equal(a[1:], b[1:]) for a, b in zip(got, want)) and all((~a[0].isfinite()).any() for a in got)
+
+
+def test_graph_of_gradients_of_any_size():
+    """Captured fp16 passes: the powers of two follow the data of each replay; two passes at once have their own."""
+    from xva_trainer_amd import seq_ops as S
+    for T in (150, 700):
+        q, k, v, lam, dout = _data(2, T, T, 4, 2, 48, "fp16", seed=17)
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        lens = torch.tensor([T, T // 2], device="cuda", dtype=torch.int32)
+        def step():
+            out = S.differential_attention(*leaves, q_lens=lens, k_lens=lens)
+            return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for turn, (size, number) in enumerate(((1.0, 0.5), (1e-3, 1e-3), (2000.0, 4.0), (1e-2, 0.0), (1.0, -0.5))):
+            with torch.no_grad():
+                q.normal_(), k.normal_(), v.normal_(), dout.copy_(torch.randn_like(dout, dtype=torch.float32) * size), lam.fill_(number), lens.random_(1, T + 1)
+            graph.replay()
+            eager = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, eager)), turn
+        two, streams = [], [torch.cuda.Stream() for _ in range(2)]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                two.append(step())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for got in two for a, b in zip(got, eager))
