@@ -207,3 +207,17 @@ def test_a_captured_step_of_a_serving_loop(dt, tol):
         ys = torch.cat(ys, 1)
         for a, b in ((ys, whole), (captured.state, last)):
             assert (a.double() - b.double()).norm().item() < 10 * tol * b.double().norm().item()
+
+
+def test_lengths_of_64_bits():
+    """Lengths beyond an item's rows mean all of them, those below zero none, also where 32 bits would take them for others."""
+    from xva_trainer_amd import seq_ops as S
+    T = 9
+    long = torch.tensor([2 ** 63 - 1, 2 ** 32, 2 ** 32 + 3, 2 ** 31, -2 ** 40, 5, -2 ** 32 + 4], device="cuda")
+    short = torch.tensor([T, T, T, T, 0, 5, 0], device="cuda", dtype=torch.int32)
+    B = long.numel()
+    x, g = torch.randn(B, T, 8, device="cuda"), torch.randn(B, T, 8, device="cuda")
+    q, k, v = (torch.randn(B, T, 2, *s, device="cuda").bfloat16() for s in ((2, 8), (2, 8), (16,)))
+    for call in (lambda l: S.group_norm_act(x, 2, lens=l), lambda l: S.gated_recurrence(x, g, lens=l)[0],
+                 lambda l: S.differential_attention(q, k, v, torch.ones(2, device="cuda") * 0.3, q_lens=l, k_lens=l)):
+        assert torch.equal(call(long), call(short))

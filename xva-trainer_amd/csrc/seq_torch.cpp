@@ -63,11 +63,11 @@ void on_one_device(const Tensor& first, std::initializer_list<Tensor> others) {
     REFUSE(!first.is_cuda(), "libxvahip ops need device tensors; got a ", first.device(), " tensor (no CPU fallback exists)");
     for (const Tensor& t : others) REFUSE(t.defined() && t.device() != first.device(), "tensors on ", first.device(), " and ", t.device());
 }
-Tensor lengths(const Tensor& lens, int64_t B, const char* what) {
+Tensor lengths(const Tensor& lens, int64_t B, int64_t T, const char* what) {
     if (!lens.defined()) return lens;
     REFUSE(lens.dim() != 1 || lens.size(0) != B, what, ": ", lens.sizes(), ", expected (", B, ",)");
     REFUSE(lens.scalar_type() != at::kInt && lens.scalar_type() != at::kLong, what, ": int32 or int64, got ", lens.scalar_type());
-    return lens.to(at::kInt).contiguous();
+    return (lens.scalar_type() == at::kLong ? lens.clamp(0, T) : lens).to(at::kInt).contiguous();        // (64 bits have numbers that 32 take for others)
 }
 Tensor fp32(const Tensor& t) { return t.defined() ? t.to(at::kFloat).contiguous() : t; }
 // elements from one index of dimension e to the next (a dimension of 1 has none: torch leaves any number there)
@@ -314,7 +314,7 @@ Tensor differential_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
     const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)d);
     REFUSE(!(scale > 0.0 && std::isfinite(scale)), "scale ", scale);
     const c10::DeviceGuard guard(q_.device());
-    ql = lengths(ql, B, "q_lens"); kl = lengths(kl, B, "k_lens");
+    ql = lengths(ql, B, q_.size(1), "q_lens"); kl = lengths(kl, B, Tk, "k_lens");
     const Tensor q = wide(q_), k = wide(k_), v = wide(v_), lam = dtype_of(lam_) < 0 ? fp32(lam_) : lam_.contiguous();
     if (wants_grad({q, k, v, lam})) return DiffAttention::apply(q, k, v, lam, maybe(ql), maybe(kl), causal, scale);
     return diff_forward(q, k, v, lam, ql, kl, causal, scale, false)[0];
@@ -379,7 +379,7 @@ std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x_, const Tensor& gate
     REFUSE(h0.defined() && (h0.dim() != 2 || h0.size(0) != x_.size(0) || h0.size(1) != x_.size(2) || !h0.is_floating_point()), "h0 ", h0.sizes(), ": (", x_.size(0), ", ",
            x_.size(2), "), a float type");
     const c10::DeviceGuard guard(x_.device());
-    lens = lengths(lens, x_.size(0), "lens");
+    lens = lengths(lens, x_.size(0), x_.size(1), "lens");
     const Tensor x = rows(x_), gate = rows(gate_);
     h0 = fp32(h0);
     const bool unit = gain == "unit";
@@ -465,7 +465,7 @@ Tensor group_norm_act(const Tensor& x_, int64_t groups, const MaybeTensor& weigh
     for (const Tensor& t : {weight, bias}) REFUSE(t.defined() && (t.dim() != 1 || t.size(0) != C || !t.is_floating_point()), "weight / bias ", t.sizes(), ": (", C, ",), a float type");
     const c10::DeviceGuard guard(x_.device());
     const Tensor x = norm_rows(flat ? x_.unsqueeze(1) : x_, groups);
-    lens = lengths(lens, x.size(0), "lens");
+    lens = lengths(lens, x.size(0), x.size(1), "lens");
     weight = fp32(weight); bias = fp32(bias);
     const NormHow how = {groups, which, eps, slope};
     const Tensor y = wants_grad({x, weight, bias}) ? GroupNormAct::apply(x, maybe(weight), maybe(bias), maybe(lens), groups, (int64_t)which, eps, slope) : norm_forward(x, weight, bias, lens, how)[0];
