@@ -461,3 +461,18 @@ def test_graph_of_gradients_of_any_size():
                 two.append(step())
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for got in two for a, b in zip(got, eager))
+
+
+@pytest.mark.parametrize("size", [1e-3, 1.0, 5000.0])
+@pytest.mark.parametrize("d,causal", [(16, False), (32, True), (48, False), (64, True)])
+def test_gradients_of_any_size_where_blocks_are_whole(size, d, causal):
+    """Enough key blocks that none is cut into pieces: the factors are undone where a block's own sums are rounded."""
+    from xva_trainer_amd import seq_ops as S
+    q, k, v, lam, dout = _data(24, 200, 200, 4, 4, d, "fp16", seed=18)
+    q, k, v, dout = q * 0.05, k * 0.05, v * 4, (dout.float() * size).half()
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    got = torch.autograd.grad(S.differential_attention(*leaves, causal=causal), leaves[:3], dout)
+    got = {"dq_1": got[0][..., 0, :], "dq_2": got[0][..., 1, :], "dk_1": got[1][..., 0, :], "dk_2": got[1][..., 1, :], "dv": got[2]}
+    for name, (ref, bound) in _norm_bounds(q, k, v, lam, dout, causal).items():
+        off = (got[name].double() - ref).norm().item()
+        assert off <= bound, "%s off by %.3g of %.3g, %.3g allowed" % (name, off, ref.norm().item(), bound)
