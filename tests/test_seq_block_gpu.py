@@ -221,3 +221,18 @@ def test_lengths_of_64_bits():
     for call in (lambda l: S.group_norm_act(x, 2, lens=l), lambda l: S.gated_recurrence(x, g, lens=l)[0],
                  lambda l: S.differential_attention(q, k, v, torch.ones(2, device="cuda") * 0.3, q_lens=l, k_lens=l)):
         assert torch.equal(call(long), call(short))
+
+
+def test_an_argument_without_memory_is_not_taken_for_one_left_out():
+    """A weight, bias, first state, length or position that is a wrapper has no address, as one that was not given."""
+    from test_seq_ops_cpu import Bare
+    from xva_trainer_amd import seq_ops as S
+    x, n = torch.randn(2, 5, 8, device="cuda"), torch.ones(8, device="cuda")
+    lens, plan = torch.tensor([5, 2], device="cuda", dtype=torch.int32), S.RotaryPlan(8)
+    q, k, v = (torch.randn(2, 5, 1, *s, device="cuda").half() for s in ((2, 8), (2, 8), (16,)))
+    for call in (lambda: S.group_norm_act(x, 2, Bare(n)), lambda: S.group_norm_act(x, 2, n, Bare(n)), lambda: S.group_norm_act(x, 2, lens=Bare(lens)),
+                 lambda: S.gated_recurrence(x, x, Bare(torch.zeros(2, 8))), lambda: S.gated_recurrence(x, x, lens=Bare(lens)),
+                 lambda: S.rotary(plan, x[:, :, None], positions=Bare(torch.zeros(5, dtype=torch.int64))),
+                 lambda: S.differential_attention(q, k, v, n[:1], q_lens=Bare(lens)), lambda: S.differential_attention(q, k, v, n[:1], k_lens=Bare(lens))):
+        with pytest.raises(S.XvaError, match="without memory"):
+            call()

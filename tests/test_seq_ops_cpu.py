@@ -296,3 +296,24 @@ def test_launches_that_the_runtime_would_cut_are_refused():
     for kw in (dict(B=1 << 20, Tq=256, Tk=1), dict(B=1 << 20, Tq=1, Tk=256)):
         assert bwd(C.byref(_diff(**one, **back, **kw)), None, 0, None) == -1 and "too many" in said()
     assert bwd(C.byref(_diff(**one, **back, B=1 << 20, Tq=1, Tk=1)), None, 0, None) == -3
+
+
+class Bare(torch.Tensor):
+    """A wrapper without memory of its own that says it is on a GPU."""
+    @staticmethod
+    def __new__(cls, like):
+        return torch.Tensor._make_wrapper_subclass(cls, like.shape, dtype=like.dtype, device=torch.device("cuda:0"))
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError("%s reached" % func)
+
+
+def test_tensors_without_memory_are_refused():
+    plan = S.RotaryPlan(8, device="cpu")
+    plan.turns = Bare(plan.turns)
+    x, half = Bare(torch.zeros(1, 2, 2, 8)), Bare(torch.zeros(1, 2, 2, 2, 8).half())
+    for call in (lambda: S.rotary(plan, x), lambda: S.gated_recurrence(Bare(torch.zeros(1, 2, 8)), Bare(torch.zeros(1, 2, 8))), lambda: S.group_norm_act(Bare(torch.zeros(1, 2, 8)), 2),
+                 lambda: S.differential_attention(half, half, Bare(torch.zeros(1, 2, 2, 16).half()), Bare(torch.zeros(2)))):
+        with pytest.raises(S.XvaError, match="without memory"):
+            call()

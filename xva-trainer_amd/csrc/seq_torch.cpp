@@ -62,6 +62,11 @@ void on_one_device(const Tensor& first, std::initializer_list<Tensor> others) {
     REFUSE(torch::jit::tracer::isTracing(), "torch.jit.trace would record none of these operators' launches");
     REFUSE(!first.is_cuda(), "libxvahip ops need device tensors; got a ", first.device(), " tensor (no CPU fallback exists)");
     for (const Tensor& t : others) REFUSE(t.defined() && t.device() != first.device(), "tensors on ", first.device(), " and ", t.device());
+    // (a fake tensor or a wrapper around others has no address, which would be taken for an argument that was left out)
+    auto empty_handed = [](const Tensor& t) { return t.defined() && t.numel() > 0 && !t.const_data_ptr(); };
+    bool bare = empty_handed(first);
+    for (const Tensor& t : others) bare = bare || empty_handed(t);
+    REFUSE(bare, "a tensor without memory of its own (fake, functional, or a wrapper around others)");
 }
 Tensor lengths(const Tensor& lens, int64_t B, int64_t T, const char* what) {
     if (!lens.defined()) return lens;
