@@ -236,3 +236,19 @@ def test_an_argument_without_memory_is_not_taken_for_one_left_out():
                  lambda: S.differential_attention(q, k, v, n[:1], q_lens=Bare(lens)), lambda: S.differential_attention(q, k, v, n[:1], k_lens=Bare(lens))):
         with pytest.raises(S.XvaError, match="without memory"):
             call()
+
+
+def test_inference_mode():
+    """Serving loops run in it: the same results, in place too, on its own tensors and on others."""
+    from xva_trainer_amd import seq_ops as S
+    torch.manual_seed(3)
+    plan = S.RotaryPlan(8)
+    made = lambda *s: torch.randn(*s, device="cuda")
+    outside = [made(2, 5, 2, 8), made(2, 5, 2, 2, 8).half(), made(2, 5, 1, 2, 8).half(), made(2, 5, 1, 16).half(), made(2), made(2, 5, 8), made(2, 5, 8)]
+    def calls(q, dq, dk, dv, lam, x, g):
+        return [S.rotary(plan, q), S.differential_attention(dq, dk, dv, lam), S.gated_recurrence(x, g)[0], S.group_norm_act(x, 2, g[0, 0], act="gelu"), S.rotary(plan, q, inplace=True)]
+    with torch.no_grad():
+        want = calls(*[t.clone() for t in outside])
+    with torch.inference_mode():
+        for ts in ([t.clone() for t in outside], outside):
+            assert all(torch.equal(a, b) for a, b in zip(calls(*ts), want))
