@@ -718,13 +718,14 @@ int xva_sdp_dequant_bwd(const float* z_u, const float* dr, const float* d_z0_log
  * normalisation and recurrences are what a changed acoustic model asks for next).  dtype: 0 fp32, 1 bf16, 2 fp16; strides in elements, the last dimension
  * contiguous; rows at or behind an item's length are not read and leave as zeros; workspaces are 16-byte aligned, their size asked
  * for with the arguments of the call.  Every call only enqueues; buffers of one call in flight (workspace
- * included) are not shared with another on a different stream, nor with another captured graph that may run beside it. */
+ * included) are not shared with another on a different stream, nor with another captured graph that may run beside it.
+ * T is under 2^30 (rotary: B T under 2^31), a row of the recurrence under 2^31 bytes; what would take a launch of 2^32 threads or more is refused. */
 
 /* Rotary positions.  q (B, T, H, D), k (B, T, Hk, D) (null with Hk = 0); pair i of the first rd elements of a head turns by position * turns[i]:
  * (a, b) -> gain (a cos - b sin, b cos + a sin), with (a, b) = elements (i, i + rd / 2), or (2 i, 2 i + 1) when `interleaved`; the other D - rd elements are
  * copied.  turns: rd / 2 fractions of a turn per position as 64-bit fixed point, so the angle at position p is that of the table modulo a turn: off by
- * p 2^-65 turns where each entry is within half a unit.  positions: int32 or int64 (positions64) with strides over items and rows (0: the same for all), null: the row's index.  inverse: the angle negated — the gradient.
- * In place: q_out == q and k_out == k with equal strides. */
+ * p 2^-65 turns where each entry is within half a unit.  positions: int32 or int64 (positions64) with strides over items and rows (0: the same for all), null:
+ * the row's index.  inverse: the angle negated — the gradient.  In place: q_out == q and k_out == k with equal strides, no two heads on each other. */
 typedef struct {
     const void *q, *k;
     void *q_out, *k_out;

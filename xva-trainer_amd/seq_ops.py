@@ -89,7 +89,7 @@ class RotaryPlan:
 
 def rotary(plan, q, k=None, positions=None, inplace=False):
     """Turns q (B, T, H, D) and, if given, k (B, T, Hk, D) by their positions: (B, T) or (T,), a dimension of 1 standing for all, int32 or int64;
-    None: 0 .. T - 1.  Returns q', or (q', k').  inplace: writes over q and k (no gradient)."""
+    None: 0 .. T - 1.  Returns q', or (q', k').  inplace: writes over q and k (no gradient; heads that lie on each other, or may, are refused)."""
     out = _seq_torch.rotary(plan.turns, plan.rotary_dim, plan.interleaved, plan.gain, q, k, positions, inplace)
     return out[0] if k is None else (out[0], out[1])
 
@@ -99,10 +99,9 @@ def differential_attention(q, k, v, lam, scale=None, causal=False, q_lens=None, 
 
     q (B, Tq, H, 2, d): two queries a head; k (B, Tk, Hk, 2, d); v (B, Tk, Hk, 2 d); d a multiple of 8, 64 at most; query head h reads key head
     h // (H / Hk).  lam (H,): any float type, differentiable.  scale: d^-1/2 unless given.  q_lens / k_lens (B,): live queries and keys; causal: query i sees
-    keys j <= i + k_len - q_len (the last query sees all).  Returns (B, Tq, H, 2 d); a row that sees no key is zero.  Rows
-    behind k_len and q_len are not read; a value that is not finite in a live row may reach every query of its item, also one that `causal` hides it from
-    (its weight is zero, its product is not a number).  With Tq = 1 and no gradient this is the
-    step of a serving loop: k and v may be slices of a longer cache."""
+    keys j <= i + k_len - q_len (the last query sees all).  Returns (B, Tq, H, 2 d); a row that sees no key is zero.  Rows behind k_len and q_len are not read; a
+    value that is not finite in a live row may reach every query of its item, also one that `causal` hides it from (its weight is zero, its product is not a
+    number).  With Tq = 1 and no gradient this is the step of a serving loop: k and v may be slices of a longer cache."""
     return _seq_torch.differential_attention(q, k, v, lam, scale, causal, q_lens, k_lens)
 
 
